@@ -30,27 +30,27 @@ SCALE_BLOCK = {"nvfp4": 16, "mxfp8": 32}
 def listed():
     return [
         # one token through a wide projection: the weight is read once, nothing else counts
-        dict(name="linear, one token", op="linear", fmt="bf16", m=1, n=8192, k=8192, out="bf16", activation="silu", bias=True, residual=True, save=False),
+        dict(name="linear one token", op="linear", fmt="bf16", m=1, n=8192, k=8192, out="bf16", activation="silu", bias=True, residual=True, save=False),
         # a short odd batch in half precision that keeps its pre-activation for training: launch latency
-        dict(name="linear, ragged f16", op="linear", fmt="f16", m=301, n=520, k=768, out="f16", activation="gelu", bias=True, residual=True, save=True),
+        dict(name="linear ragged f16", op="linear", fmt="f16", m=301, n=520, k=768, out="f16", activation="gelu", bias=True, residual=True, save=True),
         # an fp8 projection of a prompt with per-tensor scales folded into alpha
-        dict(name="linear, e4m3 prompt", op="linear", fmt="e4m3", m=4096, n=4096, k=4096, out="bf16", activation="gelu_tanh", bias=True, residual=True, save=False),
+        dict(name="linear e4m3 prompt", op="linear", fmt="e4m3", m=4096, n=4096, k=4096, out="bf16", activation="gelu_tanh", bias=True, residual=True, save=False),
         # an fp4 projection of a prompt, block-scaled operands
-        dict(name="linear, nvfp4 prompt", op="linear", fmt="nvfp4", m=2048, n=14336, k=4096, out="bf16", activation="relu", bias=False, residual=True, save=False),
+        dict(name="linear nvfp4 prompt", op="linear", fmt="nvfp4", m=2048, n=14336, k=4096, out="bf16", activation="relu", bias=False, residual=True, save=False),
         # gradients of a small ragged layer: launches count
-        dict(name="gradients, ragged", op="linear_backward", fmt="f16", m=1001, n=520, k=768, activation="gelu", bias=True),
+        dict(name="gradients ragged", op="linear_backward", fmt="f16", m=1001, n=520, k=768, activation="gelu", bias=True),
         # gradients of a training step's layer
-        dict(name="gradients, training", op="linear_backward", fmt="bf16", m=4096, n=8192, k=4096, activation="gelu_tanh", bias=True),
+        dict(name="gradients training", op="linear_backward", fmt="bf16", m=4096, n=8192, k=4096, activation="gelu_tanh", bias=True),
         # one token's choice among many experts in limited groups: latency
-        dict(name="route, one token", op="route", fmt="f32", tokens=1, experts=256, top_k=8, scores="sigmoid", bias=True, groups=8, top_groups=4, group_top=2, renormalise=True, scale=2.5, masked=False, backward=False),
+        dict(name="route one token", op="route", fmt="f32", tokens=1, experts=256, top_k=8, scores="sigmoid", bias=True, groups=8, top_groups=4, group_top=2, renormalise=True, scale=2.5, masked=False, backward=False),
         # a training batch's routing and the gradient of its logits, padding rows included
-        dict(name="route, training", op="route", fmt="bf16", tokens=16384, experts=128, top_k=8, scores="softmax", bias=False, groups=1, top_groups=1, group_top=1, renormalise=True, scale=1.0, masked=True, backward=True),
+        dict(name="route training", op="route", fmt="bf16", tokens=16384, experts=128, top_k=8, scores="softmax", bias=False, groups=1, top_groups=1, group_top=1, renormalise=True, scale=1.0, masked=True, backward=True),
         # decoding a small batch: every expert's weights are read for a row or two
-        dict(name="experts, decode", op="experts", fmt="bf16", tokens=16, experts=64, top_k=8, hidden=2048, inner=1024, activation="swiglu", dropped=False),
+        dict(name="experts decode", op="experts", fmt="bf16", tokens=16, experts=64, top_k=8, hidden=2048, inner=1024, activation="swiglu", dropped=False),
         # a prompt through a few wide experts, padding tokens included
-        dict(name="experts, prompt", op="experts", fmt="bf16", tokens=4096, experts=8, top_k=2, hidden=4096, inner=2048, activation="swiglu", dropped=True),
+        dict(name="experts prompt", op="experts", fmt="bf16", tokens=4096, experts=8, top_k=2, hidden=4096, inner=2048, activation="swiglu", dropped=True),
         # fp8 experts with a dequantisation factor of their own, odd counts
-        dict(name="product, e4m3", op="product", fmt="e4m3", tokens=1111, experts=32, top_k=4, k=1024, n=1536, activation="swiglu", save=False),
+        dict(name="product e4m3", op="product", fmt="e4m3", tokens=1111, experts=32, top_k=4, k=1024, n=1536, activation="swiglu", save=False),
         # a training step's gradients of the gate/up product
         dict(name="product gradients", op="product_backward", fmt="bf16", tokens=2048, experts=8, top_k=2, k=2048, n=2048, activation="swiglu"),
     ]
