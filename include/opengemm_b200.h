@@ -183,6 +183,26 @@ OG_API int32_t og_b200_launch_quantized(const OgGemm* g, const void* a, const vo
                                         void* c_scales, int32_t device, void* stream,
                                         const char* out_format);
 
+/* Fused epilogue: z = alpha * (A . B^T) + bias is written to `preactivation` (if not
+ * null), and C = activation(z) + residual.  All in float32, rounded once per tensor
+ * written.  `residual` and `preactivation` are [m, n] row-major in C's type; `residual`
+ * may be C itself, `preactivation` starts on a 16-byte boundary.  Float formats only.
+ * With `out_format` the activation's value leaves block-scaled as in
+ * og_b200_launch_quantized (no residual or pre-activation then).  Launches run the
+ * static schedule: split_k, cluster_k, use_clc and walk of `g` are not followed. */
+typedef struct OgEpilogue {
+  const void* bias;     /* float32 [n], or null */
+  const void* residual; /* or null */
+  void* preactivation;  /* or null */
+  void* out_scales;     /* with out_format: the 128x4 blocked scales */
+  float alpha;
+  int32_t activation;   /* 0 none, 1 relu, 2 gelu, 3 gelu in its tanh form, 4 silu */
+  int32_t out_format;   /* 0 C's own type, 1 nvfp4, 2 mxfp8, 3 mxfp4 */
+} OgEpilogue;
+OG_API int32_t og_b200_launch_fused(const OgGemm* g, const void* a, const void* b, const void* sfa,
+                                    const void* sfb, void* c, int32_t device, void* stream,
+                                    const OgEpilogue* epilogue);
+
 /* Do now what launches on `device` do on first use: opt every kernel into its shared
  * memory and allocate the stream-K workspaces.  Call it before capturing launches into
  * a CUDA graph, or to keep the first request of a server free of allocations. */

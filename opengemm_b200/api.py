@@ -75,8 +75,41 @@ def output(d, m, n, out, device):
     return out
 
 
+def check_bias(bias, n, device):
+    """Raise unless `bias` is what the epilogues add to a row of C."""
+    if not (bias.is_cuda and bias.device == device and bias.dtype is torch.float32 and bias.is_contiguous()
+            and bias.shape == (n,)):
+        raise TypeError(f"bias must be a contiguous float32 [{n}] on {device}")
+
+
+def check_epilogue(name, d, m, n, out, activation, residual, preactivation):
+    """Raise unless the fused epilogue's arguments fit a C of `d.out` [m, n]."""
+    if activation not in capi.ACTIVATIONS:
+        raise TypeError(f"activation must be one of {[a for a in capi.ACTIVATIONS if a]}, got {activation!r}")
+    if d.out is torch.int32:
+        raise TypeError(f"{name} accumulates integers exactly: its output takes no activation or residual")
+    for label, t in (("residual", residual), ("preactivation", preactivation)):
+        if t is not None and not (t.is_cuda and t.device == out.device and t.dtype is d.out and t.is_contiguous()
+                                  and t.shape == (m, n)):
+            raise TypeError(f"{label} must be a contiguous {d.out} [{m}, {n}] on {out.device}")
+    if preactivation is not None:
+        if preactivation.data_ptr() % 16:
+            raise ValueError("preactivation must start on a 16-byte boundary")
+        for label, t in (("out", out), ("residual", residual)):
+            if t is not None and overlap(preactivation, t):
+                raise ValueError(f"preactivation and {label} share memory")
+    if residual is not None and residual.data_ptr() != out.data_ptr() and overlap(residual, out):
+        raise ValueError("residual may be out itself, but not overlap it in part")
+
+
+def overlap(s, t):
+    """True when two contiguous tensors share memory."""
+    a, b = s.data_ptr(), t.data_ptr()
+    return a < b + t.numel() * t.element_size() and b < a + s.numel() * s.element_size()
+
+
 def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=None, alpha=None, bias=None,
-         out_format=None):
+         out_format=None, activation=None, residual=None, preactivation=None):
     """Compute C[M, N] = A[M, K] @ B[N, K].T.
 
     Args:
@@ -103,6 +136,13 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
             and `to_blocked` would give, ready to be the `a` of the next
             block-scaled GEMM (an addition of this build; float formats only,
             N a multiple of 64).  Returns `(packed, blocked scales)`.
+        activation: "relu", "gelu", "gelu_tanh" (its tanh form) or "silu",
+            applied in float32 to `alpha * A @ B.T + bias` in the epilogue (an
+            addition of this build, like the next two; float formats only).
+        residual: a contiguous `(M, N)` tensor of C's type added after the
+            activation, in float32, before the store.  It may be `out` itself.
+        preactivation: a contiguous `(M, N)` tensor of C's type that receives
+            the activation's argument, which `gemm_backward` reads.
 
     Returns:
         `(M, N)` row-major: float32 for dense formats (bfloat16 with
@@ -111,7 +151,9 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
     """
     name = dtype_name(a, b, sfa, atype, btype)
     if out_format is not None:
-        return _gemm_quantized(name, a, b, sfa, sfb, out_format)
+        if residual is not None or preactivation is not None:
+            raise TypeError("a block-scaled output takes an activation, but no residual or preactivation")
+        return _gemm_quantized(name, a, b, sfa, sfb, out_format, alpha, bias, activation)
     if out_dtype is None and out is not None and out.dtype in NARROW_OUT_SUFFIXES and DTYPES[name].out is torch.float32:
         out_dtype = out.dtype
     if out_dtype is not None and out_dtype is not DTYPES[name].out:
@@ -125,6 +167,12 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
     check_operands(d, m, n, k, a, b, sfa, sfb)
     lib, g = _bound.get((name, m, n, k, capi.independent_inputs())) or bind(name, m, n, k, a.device)
     out = output(d, m, n, out, a.device)
+    if activation is not None or residual is not None or preactivation is not None:
+        check_epilogue(name, d, m, n, out, activation, residual, preactivation)
+        if bias is not None:
+            check_bias(bias, n, a.device)
+        lib.launch_fused(g, a, b, sfa, sfb, out, alpha, bias, activation, residual, preactivation)
+        return out
     if alpha is None and bias is None:
         lib.launch(g, a, b, sfa, sfb, out)
         return out
@@ -133,14 +181,12 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
     if bias is None:
         lib.launch_alpha(g, a, b, sfa, sfb, out, alpha)
         return out
-    if not (bias.is_cuda and bias.device == a.device and bias.dtype is torch.float32 and bias.is_contiguous()
-            and bias.shape == (n,)):
-        raise TypeError(f"bias must be a contiguous float32 [{n}] on {a.device}")
+    check_bias(bias, n, a.device)
     lib.launch_bias(g, a, b, sfa, sfb, out, 1.0 if alpha is None else alpha, bias)
     return out
 
 
-def _gemm_quantized(name, a, b, sfa, sfb, out_format):
+def _gemm_quantized(name, a, b, sfa, sfb, out_format, alpha=None, bias=None, activation=None):
     """gemm() with a block-scaled C: `(packed, blocked scales)`."""
     if out_format not in ("nvfp4", "mxfp8", "mxfp4"):
         raise TypeError(f"out_format must be 'nvfp4', 'mxfp8' or 'mxfp4', got {out_format!r}")
@@ -156,7 +202,14 @@ def _gemm_quantized(name, a, b, sfa, sfb, out_format):
     lib, g = _bound.get((name, m, n, k, "quantized")) or _bind_quantized(name, m, n, k, a.device)
     packed = torch.empty((m, extent(target, n)), device=a.device, dtype=target.a)
     scales = torch.zeros(scale_bytes(target, m, n), device=a.device, dtype=torch.uint8).view(target.sf)
-    lib.launch_quantized(g, a, b, sfa, sfb, packed, scales, out_format)
+    if alpha is None and bias is None and activation is None:
+        lib.launch_quantized(g, a, b, sfa, sfb, packed, scales, out_format)
+        return packed, scales
+    if activation not in capi.ACTIVATIONS:
+        raise TypeError(f"activation must be one of {[x for x in capi.ACTIVATIONS if x]}, got {activation!r}")
+    if bias is not None:
+        check_bias(bias, n, a.device)
+    lib.launch_fused(g, a, b, sfa, sfb, packed, alpha, bias, activation, scales=scales, out_format=out_format)
     return packed, scales
 
 

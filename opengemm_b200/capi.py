@@ -44,6 +44,18 @@ class OgGemm(ctypes.Structure):
 assert ctypes.sizeof(OgGemm) == 108
 
 
+class OgEpilogue(ctypes.Structure):
+    """The fused epilogue of one launch (include/opengemm_b200.h)."""
+
+    _fields_ = [("bias", c_void_p), ("residual", c_void_p), ("preactivation", c_void_p), ("out_scales", c_void_p),
+                ("alpha", ctypes.c_float), ("activation", c_int32), ("out_format", c_int32)]
+
+
+# Activation names and their codes in the C ABI.
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+OUT_FORMATS = {None: 0, "nvfp4": 1, "mxfp8": 2, "mxfp4": 3}
+
+
 class OgPlan(ctypes.Structure):
     """The native tile plan of a bound GEMM (og_b200_plan)."""
 
@@ -165,6 +177,9 @@ class Library:
             self._quantized = lib.og_b200_launch_quantized
             self._quantized.restype = c_int32
             self._quantized.argtypes = [POINTER(OgGemm)] + [c_void_p] * 6 + [c_int32, c_void_p, c_char_p]
+            self._fused = lib.og_b200_launch_fused
+            self._fused.restype = c_int32
+            self._fused.argtypes = [POINTER(OgGemm)] + [c_void_p] * 5 + [c_int32, c_void_p, POINTER(OgEpilogue)]
             self._fixed = lib.og_b200_set_fixed_kernels
             self._fixed.restype, self._fixed.argtypes = None, [c_int32]
         self._kernels = None
@@ -278,6 +293,25 @@ class Library:
             byref(g), a.data_ptr(), b.data_ptr(),
             0 if sfa is None else sfa.data_ptr(), 0 if sfb is None else sfb.data_ptr(),
             packed.data_ptr(), scales.data_ptr(), device, raw_stream(device), out_format.encode(),
+        )
+        if status != OG_OK:
+            raise RuntimeError(self.error())
+
+    def launch_fused(self, g, a, b, sfa, sfb, out, alpha=None, bias=None, activation=None, residual=None,
+                     preactivation=None, scales=None, out_format=None):
+        """Like `launch`, with `activation(alpha * A.B^T + bias) + residual` written instead of the
+        bare product (and the activation's argument kept in `preactivation`, when given)."""
+        device = a.get_device()
+        epilogue = OgEpilogue(
+            bias=0 if bias is None else bias.data_ptr(), residual=0 if residual is None else residual.data_ptr(),
+            preactivation=0 if preactivation is None else preactivation.data_ptr(),
+            out_scales=0 if scales is None else scales.data_ptr(), alpha=1.0 if alpha is None else float(alpha),
+            activation=ACTIVATIONS[activation], out_format=OUT_FORMATS[out_format],
+        )
+        status = self._fused(
+            byref(g), a.data_ptr(), b.data_ptr(),
+            0 if sfa is None else sfa.data_ptr(), 0 if sfb is None else sfb.data_ptr(),
+            out.data_ptr(), device, raw_stream(device), byref(epilogue),
         )
         if status != OG_OK:
             raise RuntimeError(self.error())

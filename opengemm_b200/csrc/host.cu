@@ -45,16 +45,26 @@ extern const FixedKernel PLAIN_DENSE[];
 extern const int PLAIN_DENSE_COUNT;
 extern const FixedKernel PLAIN_SCALED[];
 extern const int PLAIN_SCALED_COUNT;
+// Implemented in kernels_fused_dense.cu and kernels_fused_scaled.cu.
+extern const FixedKernel FUSED_DENSE[];
+extern const int FUSED_DENSE_COUNT;
+extern const FixedKernel FUSED_SCALED[];
+extern const int FUSED_SCALED_COUNT;
 
 // One index space over the specialised kernels: fixed-shape dense, fixed-shape
-// scaled, then the feature-free ones.
+// scaled, then the feature-free ones, then those with the fused epilogue.
 inline int fixed_count() { return FIXED_DENSE_COUNT + FIXED_SCALED_COUNT; }
-inline int specialised_count() { return fixed_count() + PLAIN_DENSE_COUNT + PLAIN_SCALED_COUNT; }
+inline int unfused_count() { return fixed_count() + PLAIN_DENSE_COUNT + PLAIN_SCALED_COUNT; }
+inline int specialised_count() { return unfused_count() + FUSED_DENSE_COUNT + FUSED_SCALED_COUNT; }
 inline const FixedKernel& fixed_kernel(int index) {
   if (index < FIXED_DENSE_COUNT) return FIXED_DENSE[index];
   if (index < fixed_count()) return FIXED_SCALED[index - FIXED_DENSE_COUNT];
-  index -= fixed_count();
-  return index < PLAIN_DENSE_COUNT ? PLAIN_DENSE[index] : PLAIN_SCALED[index - PLAIN_DENSE_COUNT];
+  if (index < unfused_count()) {
+    index -= fixed_count();
+    return index < PLAIN_DENSE_COUNT ? PLAIN_DENSE[index] : PLAIN_SCALED[index - PLAIN_DENSE_COUNT];
+  }
+  index -= unfused_count();
+  return index < FUSED_DENSE_COUNT ? FUSED_DENSE[index] : FUSED_SCALED[index - FUSED_DENSE_COUNT];
 }
 
 inline cudaError_t configure_variant(int variant, int smem_bytes) {
@@ -142,7 +152,12 @@ int sm_count_of(int device) {
 // it was compiled without must be off.
 std::atomic<int> fixed_kernels_on{[] { const char* e = getenv("OPENGEMM_FIXED"); return (e && e[0] == '0') ? 0 : 1; }()};
 
-int fixed_kernel_for(const Plan& p, const GemmParams& params) {
+int fixed_kernel_for(const Plan& p, const GemmParams& params, bool fused = false) {
+  if (fused) {  // the only kernels with that epilogue
+    for (int i = unfused_count(); i < specialised_count(); ++i)
+      if (fixed_kernel(i).variant == p.variant) return i;
+    return -1;
+  }
   if (!fixed_kernels_on.load(std::memory_order_relaxed)) return -1;
   if (params.use_clc || params.stream_k || params.scale_out || params.bias || params.out_f16 || params.out_quant ||
       params.walk || params.cluster_k > 1)
@@ -156,7 +171,7 @@ int fixed_kernel_for(const Plan& p, const GemmParams& params) {
     if (t.stages == params.stages) return i;
     break;
   }
-  for (int i = fixed_count(); i < specialised_count(); ++i)
+  for (int i = fixed_count(); i < unfused_count(); ++i)
     if (fixed_kernel(i).variant == p.variant) return i;
   return -1;
 }
@@ -307,6 +322,7 @@ struct ParamsMemo {
   bool matches(unsigned gen, const LaunchPointers& o, int* status_word, const float* a, unsigned long long limit) const {
     return valid && generation == gen && io.a == o.a && io.b == o.b && io.sfa == o.sfa && io.sfb == o.sfb &&
            io.c == o.c && io.bias == o.bias && io.out_quant == o.out_quant && io.c_scales == o.c_scales &&
+           io.activation == o.activation && io.residual == o.residual && io.preact == o.preact &&
            status == status_word && scaled_out == (a != nullptr) && (!a || alpha == *a) && wait_limit == limit;
   }
 };
@@ -316,6 +332,14 @@ thread_local std::unique_ptr<ParamsMemo[]> params_memo;
 int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* stream, int* status_word,
                 int want_scaled, const float* alpha = nullptr) {
   if (!g) return fail(OG_ERR_LAUNCH, "null OgGemm");
+  const bool fused = io.fused();
+  OgGemm on_static_schedule;
+  if (fused) {  // the kernels with the fused epilogue run whole tiles, one after another, in the default walk
+    on_static_schedule = *g;
+    on_static_schedule.cluster_k = 1, on_static_schedule.split_k = 1, on_static_schedule.use_clc = 0;
+    on_static_schedule.walk = 0;
+    g = &on_static_schedule;
+  }
   if (!plan_memo.valid || std::memcmp(&plan_memo.key, g, sizeof(OgGemm)) != 0) {
     char why[256];
     plan_memo.valid = false;
@@ -383,7 +407,8 @@ int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* str
       params.sk_clusters = std::min<long long>(clusters, (long long)leftover * std::min<int>(g->split_k, p.k_blocks));
     }
   }
-  const int fixed = fixed_kernel_for(p, params);
+  const int fixed = fixed_kernel_for(p, params, fused);
+  if (fused && fixed < 0) return fail(OG_ERR_NO_KERNEL, "dtype %.16s has no kernel with a fused epilogue", g->dtype);
   if (fixed >= 0) {
     const int ready = ensure_fixed_configured(device, fixed);
     if (ready != OG_OK) return ready;
@@ -533,6 +558,20 @@ OG_API int32_t og_b200_launch_quantized(const OgGemm* g, const void* a, const vo
   io.out_quant = which;
   io.c_scales = c_scales;
   return launch_impl(g, io, device, stream, nullptr, -1);
+}
+
+OG_API int32_t og_b200_launch_fused(const OgGemm* g, const void* a, const void* b, const void* sfa, const void* sfb,
+                                    void* c, int32_t device, void* stream, const OgEpilogue* epilogue) {
+  if (!epilogue) return fail(OG_ERR_LAUNCH, "null OgEpilogue");
+  LaunchPointers io{a, b, sfa, sfb, c, epilogue->bias};
+  io.activation = epilogue->activation;
+  io.residual = epilogue->residual;
+  io.preact = epilogue->preactivation;
+  io.out_quant = epilogue->out_format;
+  io.c_scales = epilogue->out_scales;
+  if (io.out_quant < 0 || io.out_quant > 3) return fail(OG_ERR_LAUNCH, "out_format %d is none of 0..3", io.out_quant);
+  const float alpha = epilogue->alpha;
+  return launch_impl(g, io, device, stream, nullptr, -1, alpha != 1.0f ? &alpha : nullptr);
 }
 
 OG_API int32_t og_b200_status(int32_t status_word) {

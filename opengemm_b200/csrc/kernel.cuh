@@ -23,6 +23,7 @@
 // TMA loads (no cluster multicast); every wait is bounded.
 #pragma once
 
+#include "activation.cuh"
 #include "ptx.cuh"
 #include "quant_math.cuh"
 #include "raster.h"
@@ -95,6 +96,14 @@ struct alignas(64) GemmParams {
   int out_quant;          // 0 off, else 1 + QFormat: 1 nvfp4, 2 mxfp8, 3 mxfp4
   int out_k_groups;       // 512-byte scale atoms along N of `out_scales`
   uint8_t* out_scales;
+  // Fused epilogue (kernels built with FUSED only): z = alpha * acc + bias goes
+  // to `preact` when it is not null, and C = act(z) + residual; both tensors
+  // have C's type and layout.
+  const void* residual;
+  void* preact;
+  int act_shape;          // og::ActShape
+  float act_a, act_b;     // coefficients of SHAPE_SIGMOID
+  int residual_vec;       // rows of the residual may be read 16 bytes at a time
 };
 
 // Second, unused kernel argument.  On B200 with driver 580 the host cost of
@@ -296,6 +305,11 @@ __device__ __forceinline__ void fold_features_off(GemmParams& p) {
   p.walk = 0, p.use_clc = 0, p.stream_k = 0, p.scale_out = 0, p.out_f16 = 0, p.out_quant = 0, p.cluster_k = 1;
   p.bias = nullptr;
 }
+
+// A fused launch runs the static schedule in the default walk: what its kernel leaves out.
+__device__ __forceinline__ void fold_schedules_off(GemmParams& p) {
+  p.walk = 0, p.use_clc = 0, p.stream_k = 0, p.cluster_k = 1;
+}
 #endif
 
 // FIXED_N == 0: every tile-plan value is read from `params` at run time.
@@ -307,7 +321,9 @@ __device__ __forceinline__ void fold_features_off(GemmParams& p) {
 // the path it takes: bf16 128^3 spends 2.2 us between the previous grid's
 // completion and its own in the full kernel, 1.5 us in the plain one and
 // 1.0 us in one compiled for its tile shape.
-template <int KIND, int CTA_GROUP, int OUT_BYTES, int FIXED_N = 0, int FIXED_EPI = 0, bool PLAIN = false>
+// FUSED: the static schedule with the activation, residual and pre-activation
+// of the fused epilogue (which the other builds do not carry).
+template <int KIND, int CTA_GROUP, int OUT_BYTES, int FIXED_N = 0, int FIXED_EPI = 0, bool PLAIN = false, bool FUSED = false>
 __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant__ GemmParams params, const LaunchPad) {
   // `p` is the scalar view of the launch parameters.  A standalone kernel
   // emitted for one shape defines OG_FIXED_PLAN to overwrite the plan fields
@@ -326,6 +342,10 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
   } else if constexpr (PLAIN) {
     folded = params;
     fold_features_off(folded);
+    view = &folded;
+  } else if constexpr (FUSED) {
+    folded = params;
+    fold_schedules_off(folded);
     view = &folded;
   }
   const GemmParams& p = *view;
@@ -631,8 +651,29 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     WorkIter work(p, cluster_id, num_clusters, k_rank);
     if (p.use_clc) work.enable_clc(clc_state(false, lane == 0), CTA_GROUP);
     Work w;
+    // Fused epilogue: this thread's 128 bytes of the residual's next chunk.  They
+    // are requested before the accumulator is waited for, and the following
+    // chunk's as soon as these are used, so that the stores and the next
+    // tensor-memory load hide the trip to memory.  Each lane reads its own row:
+    // eight 16-byte loads of one line, which L1 serves after the first.  (Plain
+    // loads, not read-only ones: the residual may be C itself.)
+    uint4 res[FUSED ? 8 : 1];
+    const uint8_t* const residual = FUSED ? static_cast<const uint8_t*>(p.residual) : nullptr;
+    const bool residual_vec = FUSED && p.residual_vec && !transpose_out;
     for (; __all_sync(0xFFFFFFFFu, allocated) && work.next(w); ++tile_idx) {
       const TileCoord t = tile_coord(p, w.tile);
+      if constexpr (FUSED) {
+        if (residual_vec) {
+          if (p.pdl && !touched_memory) pdl_wait_prior_grids();
+          touched_memory = true;
+          const int r = t.mi * TILE_M + int(rank) * 128 + quarter * 32 + lane, c = t.ni * tile_n;
+          if (r < rows_m && c + CHUNK <= rows_n && CHUNK <= tile_n) {
+            const uint4* src = reinterpret_cast<const uint4*>(residual + (size_t(r) * ldd + c) * OUT_BYTES);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) res[FUSED ? u : 0] = src[u];
+          }
+        }
+      }
       // Stream-K roles (a cluster-K rank also holds a K slice, but exchanges it through shared memory below).
       const bool contributes = p.stream_k && w.kb0 > 0;          // publish partial sums instead of output
       const bool finishes = p.stream_k && w.kb0 == 0 && w.kb1 < p.k_blocks;  // add the sharers' partials before storing
@@ -660,7 +701,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
       // rows at a time and stores whole 128-byte segments, clipped at the
       // edges of D.  Plain st.global: nothing to wait for before the buffer
       // is reused but the warp's own reads.
-      auto store_staged = [&](const uint32_t* w, int c, int width) {
+      auto store_staged = [&](const uint32_t* w, int c, int width, uint8_t* base) {
         const uint32_t rowaddr = my_buf + lane * 128;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
@@ -669,7 +710,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
         __syncwarp();
         const int gcol = col0 + c + unit * UNIT;
         if (unit * UNIT < width && gcol < rows_n) {
-          uint8_t* dst = out + (size_t(row0 + sub_row) * ldd + gcol) * OUT_BYTES;
+          uint8_t* dst = base + (size_t(row0 + sub_row) * ldd + gcol) * OUT_BYTES;
           const size_t step = size_t(4) * ldd * OUT_BYTES;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -692,7 +733,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
             if (lane == 0) tma_store_wait_read<0>();
             __syncwarp();
           }
-          store_staged(w, c, width);
+          store_staged(w, c, width, out);
           return;
         }
         const uint32_t buf = my_buf + (buf_use & 1) * EPI_BUF_BYTES;
@@ -721,7 +762,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
       // released, and only then are the held chunks stored.
       bool handed_back = false, handed_back_late = false;
       if constexpr (OUT_BYTES == 2) {
-        if (p.acc_slots == 1 && staged && tile_n == 256 && !contributes && !finishes && !scale_out && !bias && !out_f16 &&
+        if (!FUSED && p.acc_slots == 1 && staged && tile_n == 256 && !contributes && !finishes && !scale_out && !bias && !out_f16 &&
             !p.out_quant && cluster_k == 1 && row0 < rows_m) {
           auto pack64 = [](const uint32_t* f, uint32_t* w) {
 #pragma unroll
@@ -929,6 +970,82 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
             const float mine = __ldg(bias + min(row, rows_m - 1));
 #pragma unroll
             for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + mine);
+          }
+        }
+        if constexpr (FUSED) {
+          const int gc = col0 + c;
+          auto value_bits = [&](uint32_t x) { return OUT_BYTES == 4 ? x : pack2(x, 0u) & 0xFFFFu; };
+          if (p.preact) {
+            // The pre-activation leaves by the same paths as C itself below (never by TMA store).
+            uint8_t* const pre = static_cast<uint8_t*>(p.preact);
+            if (staged && row0 < rows_m) {
+              uint32_t w[32];
+#pragma unroll
+              for (int u = 0; u < 32; ++u) w[u] = OUT_BYTES == 4 ? v[u] : pack2(v[(2 * u) % CHUNK], v[(2 * u + 1) % CHUNK]);
+              store_staged(w, c, width, pre);
+            } else if (row < rows_m) {
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j) {
+                if (j < width && gc + j < rows_n) {
+                  const size_t at = transpose_out ? size_t(gc + j) * ldd + row : size_t(row) * ldd + gc + j;
+                  if constexpr (OUT_BYTES == 4) reinterpret_cast<uint32_t*>(pre)[at] = v[j];
+                  else reinterpret_cast<uint16_t*>(pre)[at] = uint16_t(value_bits(v[j]));
+                }
+              }
+            }
+          }
+          if (p.act_shape == SHAPE_SIGMOID) {
+            const float a = p.act_a, b = p.act_b;
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(act_value<SHAPE_SIGMOID>(__uint_as_float(v[j]), a, b));
+          } else if (p.act_shape == SHAPE_PHI) {
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(act_value<SHAPE_PHI>(__uint_as_float(v[j]), 0.f, 0.f));
+          } else if (p.act_shape == SHAPE_RELU) {
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(act_value<SHAPE_RELU>(__uint_as_float(v[j]), 0.f, 0.f));
+          }
+          if (residual && row < rows_m) {
+            if (residual_vec && gc + CHUNK <= rows_n && width == CHUNK) {
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const uint32_t q[4] = {res[FUSED ? u : 0].x, res[FUSED ? u : 0].y, res[FUSED ? u : 0].z, res[FUSED ? u : 0].w};
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                  if constexpr (OUT_BYTES == 4) {
+                    v[4 * u + h] = __float_as_uint(__uint_as_float(v[4 * u + h]) + __uint_as_float(q[h]));
+                  } else {
+                    const int j = (8 * u + 2 * h) % CHUNK;
+                    const float lo = out_f16 ? half_bits_to_float(q[h]) : __uint_as_float(q[h] << 16);
+                    const float hi = out_f16 ? half_bits_to_float(q[h] >> 16) : __uint_as_float(q[h] & 0xFFFF0000u);
+                    v[j] = __float_as_uint(__uint_as_float(v[j]) + lo);
+                    v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + hi);
+                  }
+                }
+              }
+              const int next = c + CHUNK;
+              if (next + CHUNK <= tile_n && col0 + next + CHUNK <= rows_n) {
+                const uint4* src = reinterpret_cast<const uint4*>(residual + (size_t(row) * ldd + col0 + next) * OUT_BYTES);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) res[FUSED ? u : 0] = src[u];
+              }
+            } else {
+              before_global_memory();
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j) {
+                if (j < width && gc + j < rows_n) {
+                  const size_t at = transpose_out ? size_t(gc + j) * ldd + row : size_t(row) * ldd + gc + j;
+                  float add;
+                  if constexpr (OUT_BYTES == 4) {
+                    add = reinterpret_cast<const float*>(residual)[at];
+                  } else {
+                    const uint32_t bits = reinterpret_cast<const uint16_t*>(residual)[at];
+                    add = out_f16 ? half_bits_to_float(bits) : __uint_as_float(bits << 16);
+                  }
+                  v[j] = __float_as_uint(__uint_as_float(v[j]) + add);
+                }
+              }
+            }
           }
         }
         if constexpr (OUT_BYTES == 2) {

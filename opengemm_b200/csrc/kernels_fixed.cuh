@@ -28,4 +28,10 @@ struct FixedKernel {
 #define OG_PLAIN_KERNEL(VARIANT, KIND, GROUP, OUT) \
   FixedKernel { VARIANT, 0, 0, configure_one<KIND, GROUP, OUT, 0, 0, true>, launch_one<KIND, GROUP, OUT, 0, 0, true> }
 
+// The run-time-shaped kernel of a variant on the static schedule with the fused
+// epilogue (activation, residual, pre-activation).
+#define OG_FUSED_KERNEL(VARIANT, KIND, GROUP, OUT)                        \
+  FixedKernel { VARIANT, 0, 0, configure_one<KIND, GROUP, OUT, 0, 0, false, true>, \
+                launch_one<KIND, GROUP, OUT, 0, 0, false, true> }
+
 }  // namespace og

@@ -142,6 +142,11 @@ struct LaunchPointers {
   // Block-scaled output: `c` receives packed codes, `c_scales` the blocked scales.
   int out_quant = 0;        // 0 off, else 1 nvfp4, 2 mxfp8, 3 mxfp4
   void* c_scales = nullptr;
+  // Fused epilogue: og::Activation, and tensors of C's type and layout (may be null).
+  int activation = 0;
+  const void* residual = nullptr;
+  void* preact = nullptr;
+  bool fused() const { return activation || residual || preact; }
 };
 
 // Checks every launch entry point makes before touching the device.
@@ -178,6 +183,28 @@ inline int check_pointers(const OgGemm& g, const Plan& p, const LaunchPointers& 
     snprintf(why, why_cap, "dtype %.16s accumulates integers exactly: its output cannot be scaled or biased", g.dtype);
     return OG_ERR_LAUNCH;
   }
+  if (io.fused()) {
+    if (p.format->out == OUT_S32) {
+      snprintf(why, why_cap, "dtype %.16s accumulates integers exactly: its output takes no activation or residual", g.dtype);
+      return OG_ERR_LAUNCH;
+    }
+    if (io.activation < ACT_NONE || io.activation > ACT_SILU) {
+      snprintf(why, why_cap, "activation %d is none of 0..%d", io.activation, int(ACT_SILU));
+      return OG_ERR_LAUNCH;
+    }
+    if (io.out_quant && (io.residual || io.preact)) {
+      snprintf(why, why_cap, "a block-scaled output takes an activation, but no residual or pre-activation");
+      return OG_ERR_LAUNCH;
+    }
+    if (io.preact && (reinterpret_cast<uintptr_t>(io.preact) & 15)) {
+      snprintf(why, why_cap, "the pre-activation must start on a 16-byte boundary");
+      return OG_ERR_LAUNCH;
+    }
+    if (reinterpret_cast<uintptr_t>(io.residual) & (p.out_bytes - 1)) {
+      snprintf(why, why_cap, "the residual must start on an element boundary");
+      return OG_ERR_LAUNCH;
+    }
+  }
   return OG_OK;
 }
 
@@ -203,7 +230,8 @@ inline int fill_params(const Plan& p, const OgGemm& g, const LaunchPointers& io,
   if (rc != OG_OK) return rc;
   const bool c_aligned = (reinterpret_cast<uintptr_t>(io.c) & 15) == 0;
   const int epi_staged = p.epi_staged && c_aligned;
-  const int epi_tma = p.epi_tma && c_aligned && !io.out_quant;  // block-scaled C is stored by its own path
+  const int epi_tma = p.epi_tma && c_aligned && !io.out_quant &&  // block-scaled C is stored by its own path,
+                      !io.preact;  // and a kept pre-activation shares C's staging buffer
   if (epi_tma) {
     const int type = p.format->out == OUT_S32    ? int(CU_TENSOR_MAP_DATA_TYPE_INT32)
                      : p.format->out == OUT_BF16 ? int(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)
@@ -266,6 +294,10 @@ inline int fill_params(const Plan& p, const OgGemm& g, const LaunchPointers& io,
     params.scale_out = 1;
     params.alpha = *alpha;
   }
+  params.residual = io.residual;
+  params.preact = io.preact;
+  act_constants(io.activation, &params.act_shape, &params.act_a, &params.act_b);
+  params.residual_vec = io.residual && (reinterpret_cast<uintptr_t>(io.residual) & 15) == 0 && (int64_t(g.n) * p.out_bytes) % 16 == 0;
   if (io.out_quant) {
     params.out_quant = io.out_quant;
     params.out_scales = static_cast<uint8_t*>(io.c_scales);

@@ -493,6 +493,13 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return v;
 }
 
+// The IEEE half in the low 16 bits, as float32.
+__device__ __forceinline__ float half_bits_to_float(uint32_t bits) {
+  float v;
+  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.f32.f16 %0, h;\n\t}" : "=f"(v) : "r"(bits));
+  return v;
+}
+
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
                                              uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
