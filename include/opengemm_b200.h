@@ -280,6 +280,87 @@ OG_API int32_t og_b200_launch_no_alloc(const OgGemm* g, const void* a, const voi
                                        const void* sfa, const void* sfb, void* c, int32_t device,
                                        void* stream, char* error_text, int32_t error_text_cap);
 
+/* ---- gradients of a product, and mixtures of experts: no counterpart in the reference ----
+ *
+ * Element types are 1 (bfloat16) and 2 (float16), for router logits also 0 (float32).
+ * Activations are those of OgEpilogue, and the gated pairs 5 (silu(gate) * up) and
+ * 6 (gelu(gate) * up), where gate and up are the first and the second half of the columns.
+ * All calls are asynchronous on `stream`; none allocates or synchronises. */
+
+/* A product whose rows fall into groups, each with a matrix of its own.
+ *   mode 0  out[r] = act(alpha_e * x[r] . w_e^T)           x [rows, k], w [groups, n, k], out [rows, n] (gated: n/2)
+ *   mode 1  out[r] = x[r] . w_e                            x [rows, n], w [groups, n, k], out [rows, k]
+ *   mode 2  out[e] = sum over e's rows of x[r]^T w[r]      x [rows, n], w [rows, k],      out [groups, n, k]
+ * Group e has the rows offsets[e] .. offsets[e + 1]; rows of `out` past the last group are
+ * left as they were.  With `tokens` row r of mode 0's x (mode 2's w) is row tokens[r] of a
+ * [x_rows, k] tensor.  dtype "bf16" or "f16", for mode 0 also "e4m3" (written as bfloat16).
+ * Rows of all operands are multiples of 16 bytes and start on such boundaries.  A single
+ * group needs no table: offsets may be null.  Errors: og_b200_experts_error(). */
+typedef struct OgExpertProduct {
+  const void* x;
+  const void* w;
+  const int32_t* offsets; /* device, [groups + 1], or null */
+  const int32_t* tokens;  /* device, [rows], or null */
+  const float* alpha;     /* device, [groups], or null; mode 0 */
+  void* out;
+  void* preactivation;    /* mode 0: [rows, n], the activation's argument, or null */
+  int32_t mode, groups, rows, x_rows, n, k;
+  int32_t activation;     /* mode 0 */
+  int32_t out_f32;        /* modes 1 and 2: write float32 */
+  float factor;           /* on every product, before the activation (beside alpha) */
+  char dtype[16];
+} OgExpertProduct;
+OG_API int32_t og_b200_expert_product(const OgExpertProduct* product, int32_t device, void* stream);
+OG_API const char* og_b200_experts_error(void);
+
+/* The choice of experts.  Scores are softmax (or logistic, `sigmoid`) values of the logits
+ * [tokens, experts]; the choice is by score + bias (float32 [experts], or null), the lowest
+ * index first among equals.  With groups > 1 only the `top_groups` groups of experts with
+ * the largest sum of their best `group_top` (1 or 2) choice scores are open.  Weights
+ * [tokens, top_k] are the chosen scores (divided by their sum if `renormalise`) times
+ * `scale`.  A logit of -infinity is never chosen; a token with fewer than top_k experts
+ * left has index -1 and weight 0 in the places that stay empty.  Errors: og_b200_routing_error(). */
+typedef struct OgRoute {
+  int64_t tokens;
+  int32_t dtype, experts, top_k, sigmoid, groups, top_groups, group_top, renormalise;
+  float scale;
+} OgRoute;
+OG_API int32_t og_b200_route(const OgRoute* route, const void* logits, const float* bias, float* weights,
+                             int32_t* indices, int32_t device, void* stream);
+/* Gradient of the logits (their type) for a gradient of the weights; `indices` as chosen. */
+OG_API int32_t og_b200_route_gradient(const OgRoute* route, const float* grad_weights, const void* logits,
+                                      const int32_t* indices, void* grad_logits, int32_t device, void* stream);
+
+/* Order of the rows by expert, in the order of the (token, choice) pairs inside one.
+ * offsets [experts + 1]: first row of each expert; token_of_row [tokens * top_k]; positions
+ * [tokens, top_k]: the row of each pair, -1 where the index is outside 0 .. experts - 1
+ * (then rows past offsets[experts] do not exist).  workspace: ceil(tokens * top_k / 4096) *
+ * experts integers (null up to 4096 pairs). */
+OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32_t top_k, int32_t experts,
+                                   int32_t* offsets, int32_t* token_of_row, int32_t* positions,
+                                   int32_t* workspace, int32_t device, void* stream);
+
+/* out[t] = residual[t] + sum over j of weights[t, j] * y[positions[t, j]] in float32, in the
+ * order of j; weights null: ones; residual null: zero.  y [rows, n] of `dtype`, or float32
+ * if y_is_f32; out and residual [tokens, n] of `dtype`. */
+OG_API int32_t og_b200_expert_combine(int32_t dtype, int32_t y_is_f32, const void* y, const float* weights,
+                                      const int32_t* positions, const void* residual, void* out, int64_t tokens,
+                                      int32_t top_k, int32_t n, int32_t device, void* stream);
+/* grad_y[positions[t, j]] = weights[t, j] * grad[t] (rows that no pair has are left as they
+ * were) and grad_weights[t, j] = <grad[t], y[positions[t, j]]>, 0 where there is no row. */
+OG_API int32_t og_b200_expert_combine_gradient(int32_t dtype, const void* grad, const void* y, const float* weights,
+                                               const int32_t* positions, void* grad_y, float* grad_weights,
+                                               int64_t tokens, int32_t top_k, int32_t n, int32_t device, void* stream);
+
+/* dz = grad * act'(z) for rows [0, rows), or [0, *row_limit) if row_limit (device) is given.
+ * z, dz [rows, n]; grad [rows, n] (gated: n/2).  bias_gradient (float32 [n], or null; not for
+ * a gated activation): column sums of dz before it is rounded, through a workspace of
+ * ceil(rows / 64) * n floats.  Without an activation z and dz are not used. */
+OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, const void* grad, const void* z, void* dz,
+                                           float* bias_gradient, float* workspace, const int32_t* row_limit,
+                                           int64_t rows, int32_t n, int32_t device, void* stream);
+OG_API const char* og_b200_routing_error(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,13 +10,19 @@ The public names are those of the reference package (opengemm/__init__.py:10-28)
 Additions of this build, all optional: `og.gemm(..., out_dtype=torch.bfloat16)`
 and `og.gemm(..., alpha=0.5)` (output variants), `og.quantize_blocked` (values ->
 packed data + blocked scales in one kernel), `python -m opengemm_b200.tune`
-and `python -m opengemm_b200.benchmark` (tuner and suite runner).
+and `python -m opengemm_b200.benchmark` (tuner and suite runner); the
+feed-forward operators around the product: `og.gemm(..., activation=,
+residual=, preactivation=)` with `og.gemm_backward`, and mixtures of experts -
+`og.route`, `og.expert_plan`, `og.expert_gemm`, `og.expert_combine` and their
+`_backward`s.
 """
 
-from .api import gemm
+from .api import gemm, gemm_backward
 from .build import prebuild
 from .dtypes import DTYPES, dtype_name
 from .emit import emit_kernel
+from .experts import (ExpertPlan, expert_combine, expert_combine_backward, expert_gemm, expert_gemm_backward,
+                      expert_plan, route, route_backward)
 from .quant import pack, quantize, quantize_blocked, to_blocked, unpack
 from .run import run_kernel
 

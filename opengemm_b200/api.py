@@ -186,6 +186,75 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
     return out
 
 
+def gemm_backward(grad, a, b, activation=None, preactivation=None, alpha=None, want=("a", "b"), out_dtype=None):
+    """Gradients of `gemm(a, b, alpha=, bias=, activation=, residual=)` with 16-bit operands.
+
+    With `dz = grad * activation'(preactivation)`: `a`'s gradient is
+    `alpha * dz @ b`, `b`'s is `alpha * dz.T @ a`, the bias's the column sums of
+    `dz`; a residual's is `grad` itself.  `dz` is rounded to the operands' type,
+    which the matrix instructions read; the bias's sums are taken before that.
+
+    Args:
+        grad: contiguous `(M, N)` gradient of C, of the operands' dtype.
+        a, b: the operands, bfloat16 or float16, `(M, K)` and `(N, K)`; N and K
+            multiples of 8.
+        activation: as in the forward call.
+        preactivation: the tensor the forward call filled, in the operands' dtype;
+            required with an activation.
+        alpha: as in the forward call.
+        want: which of "a", "b" and "bias" to compute.
+        out_dtype: dtype of the operands' gradients: the operands' (default) or
+            `torch.float32`.
+
+    Returns:
+        `(grad_a, grad_b, grad_bias)`, None in the place of what is not wanted;
+        `grad_bias` is float32.
+    """
+    if not a.is_cuda or a.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"gradients are served for bfloat16 and float16 CUDA operands, got {a.dtype} on {a.device}")
+    name = "bf16" if a.dtype is torch.bfloat16 else "f16"
+    d = DTYPES[name]
+    if a.dim() != 2 or b.dim() != 2:
+        raise TypeError("a and b must be contiguous 2-D CUDA tensors")
+    m, n, k = a.size(0), b.size(0), a.size(1)
+    check_operands(d, m, n, k, a, b, None, None)
+    if n % 8 or k % 8 or not n or not k:
+        raise ValueError(f"N and K must be positive multiples of 8, got {n} and {k}")
+    if not set(want) <= {"a", "b", "bias"}:
+        raise TypeError(f"want names gradients out of 'a', 'b' and 'bias', got {want!r}")
+    if activation not in capi.ACTIVATIONS:
+        raise TypeError(f"activation must be one of {[x for x in capi.ACTIVATIONS if x]}, got {activation!r}")
+    if (activation is None) != (preactivation is None):
+        raise TypeError("an activation and its preactivation come together")
+    for label, t in (("grad", grad), ("preactivation", preactivation)):
+        if t is not None and not (t.is_cuda and t.device == a.device and t.dtype is a.dtype and t.is_contiguous()
+                                  and t.shape == (m, n)):
+            raise TypeError(f"{label} must be a contiguous {a.dtype} [{m}, {n}] on {a.device}")
+    if out_dtype not in (None, a.dtype, torch.float32):
+        raise TypeError(f"gradients leave as {a.dtype} or torch.float32, not {out_dtype}")
+    for label, t in (("grad", grad), ("preactivation", preactivation), ("a", a), ("b", b)):
+        if t is not None and t.data_ptr() % 16:
+            raise ValueError(f"{label} must start on a 16-byte boundary")
+    out_dtype = out_dtype or a.dtype
+    lib = capi.library("mm")
+    dz, grad_a, grad_b, grad_bias, workspace = grad, None, None, None, None
+    if activation is not None:
+        dz = torch.empty_like(grad)
+    if "bias" in want:
+        grad_bias = torch.empty(n, device=a.device, dtype=torch.float32)
+        workspace = torch.empty((-(-m // 64), n), device=a.device, dtype=torch.float32)
+    if activation is not None or grad_bias is not None:
+        lib.activation_gradient(capi.ACTIVATIONS[activation], grad, preactivation, None if dz is grad else dz, n, grad_bias, workspace)
+    alpha = 1.0 if alpha is None else float(alpha)
+    if "a" in want:
+        grad_a = torch.empty((m, k), device=a.device, dtype=out_dtype)
+        lib.expert_product(capi.ROWS_GRADIENT, name.encode(), dz, b, grad_a, 1, m, n, k, factor=alpha)
+    if "b" in want:
+        grad_b = torch.empty((n, k), device=a.device, dtype=out_dtype)
+        lib.expert_product(capi.WEIGHTS_GRADIENT, name.encode(), dz, a, grad_b, 1, m, n, k, factor=alpha)
+    return grad_a, grad_b, grad_bias
+
+
 def _gemm_quantized(name, a, b, sfa, sfb, out_format, alpha=None, bias=None, activation=None):
     """gemm() with a block-scaled C: `(packed, blocked scales)`."""
     if out_format not in ("nvfp4", "mxfp8", "mxfp4"):

@@ -51,8 +51,27 @@ class OgEpilogue(ctypes.Structure):
                 ("alpha", ctypes.c_float), ("activation", c_int32), ("out_format", c_int32)]
 
 
+class OgExpertProduct(ctypes.Structure):
+    """One product of experts, or a gradient of a product (include/opengemm_b200.h)."""
+
+    _fields_ = ([(f, c_void_p) for f in ("x", "w", "offsets", "tokens", "alpha", "out", "preactivation")]
+                + [(f, c_int32) for f in ("mode", "groups", "rows", "x_rows", "n", "k", "activation", "out_f32")]
+                + [("factor", ctypes.c_float), ("dtype", c_char * 16)])
+
+
+class OgRoute(ctypes.Structure):
+    """How experts are chosen (include/opengemm_b200.h)."""
+
+    _fields_ = ([("tokens", ctypes.c_int64)]
+                + [(f, c_int32) for f in ("dtype", "experts", "top_k", "sigmoid", "groups", "top_groups", "group_top", "renormalise")]
+                + [("scale", ctypes.c_float)])
+
+
 # Activation names and their codes in the C ABI.
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+GATED_ACTIVATIONS = {"swiglu": 5, "geglu": 6}  # experts' products only
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+FORWARD, ROWS_GRADIENT, WEIGHTS_GRADIENT = 0, 1, 2  # modes of OgExpertProduct
 OUT_FORMATS = {None: 0, "nvfp4": 1, "mxfp8": 2, "mxfp4": 3}
 
 
@@ -180,6 +199,22 @@ class Library:
             self._fused = lib.og_b200_launch_fused
             self._fused.restype = c_int32
             self._fused.argtypes = [POINTER(OgGemm)] + [c_void_p] * 5 + [c_int32, c_void_p, POINTER(OgEpilogue)]
+            for name, argtypes in {
+                "expert_product": [POINTER(OgExpertProduct), c_int32, c_void_p],
+                "route": [POINTER(OgRoute)] + [c_void_p] * 4 + [c_int32, c_void_p],
+                "route_gradient": [POINTER(OgRoute)] + [c_void_p] * 4 + [c_int32, c_void_p],
+                "expert_plan": [c_void_p, ctypes.c_int64, c_int32, c_int32] + [c_void_p] * 4 + [c_int32, c_void_p],
+                "expert_combine": [c_int32, c_int32] + [c_void_p] * 5 + [ctypes.c_int64, c_int32, c_int32, c_int32, c_void_p],
+                "expert_combine_gradient": [c_int32] + [c_void_p] * 6 + [ctypes.c_int64, c_int32, c_int32, c_int32, c_void_p],
+                "activation_gradient": [c_int32, c_int32] + [c_void_p] * 6 + [ctypes.c_int64, c_int32, c_int32, c_void_p],
+            }.items():
+                fn = getattr(lib, "og_b200_" + name)
+                fn.restype, fn.argtypes = c_int32, argtypes
+                setattr(self, "_" + name, fn)
+            for name in ("experts_error", "routing_error"):
+                fn = getattr(lib, "og_b200_" + name)
+                fn.restype, fn.argtypes = c_char_p, []
+                setattr(self, "_" + name, fn)
             self._fixed = lib.og_b200_set_fixed_kernels
             self._fixed.restype, self._fixed.argtypes = None, [c_int32]
         self._kernels = None
@@ -315,6 +350,61 @@ class Library:
         )
         if status != OG_OK:
             raise RuntimeError(self.error())
+
+    def expert_product(self, mode, dtype, x, w, out, groups, rows, n, k, offsets=None, tokens=None, x_rows=0, alpha=None,
+                       activation=0, preactivation=None, factor=1.0):
+        """One launch of og_b200_expert_product on CUDA tensors, on the current stream of `out`'s device."""
+        device = out.get_device()
+        product = OgExpertProduct(
+            x.data_ptr(), w.data_ptr(), 0 if offsets is None else offsets.data_ptr(), 0 if tokens is None else tokens.data_ptr(),
+            0 if alpha is None else alpha.data_ptr(), out.data_ptr(), 0 if preactivation is None else preactivation.data_ptr(),
+            mode, groups, rows, x_rows, n, k, activation, out.dtype is torch.float32, factor, dtype,
+        )
+        if self._expert_product(byref(product), device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._experts_error().decode())
+
+    def route(self, how, logits, bias, weights, indices):
+        device = logits.get_device()
+        if self._route(byref(how), logits.data_ptr(), 0 if bias is None else bias.data_ptr(), weights.data_ptr(),
+                       indices.data_ptr(), device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._routing_error().decode())
+
+    def route_gradient(self, how, grad_weights, logits, indices, grad_logits):
+        device = logits.get_device()
+        if self._route_gradient(byref(how), grad_weights.data_ptr(), logits.data_ptr(), indices.data_ptr(),
+                                grad_logits.data_ptr(), device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._routing_error().decode())
+
+    def expert_plan(self, indices, experts, offsets, tokens, positions, workspace):
+        device = indices.get_device()
+        if self._expert_plan(indices.data_ptr(), indices.size(0), indices.size(1), experts, offsets.data_ptr(),
+                             tokens.data_ptr(), positions.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
+                             device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._routing_error().decode())
+
+    def expert_combine(self, y, weights, positions, residual, out):
+        device = out.get_device()
+        if self._expert_combine(ELEMENT_TYPES[out.dtype], y.dtype is torch.float32, y.data_ptr(), 0 if weights is None else weights.data_ptr(),
+                                positions.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(),
+                                out.size(0), positions.size(1), out.size(1), device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._routing_error().decode())
+
+    def expert_combine_gradient(self, grad, y, weights, positions, grad_y, grad_weights):
+        device = grad.get_device()
+        if self._expert_combine_gradient(ELEMENT_TYPES[grad.dtype], grad.data_ptr(), y.data_ptr(), weights.data_ptr(),
+                                         positions.data_ptr(), grad_y.data_ptr(), grad_weights.data_ptr(), grad.size(0),
+                                         positions.size(1), grad.size(1), device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._routing_error().decode())
+
+    def activation_gradient(self, activation, grad, z, dz, n, bias_gradient=None, workspace=None, row_limit=None):
+        """dz = grad * act'(z) (and its column sums); `activation` is a code of the C ABI."""
+        device = grad.get_device()
+        if self._activation_gradient(ELEMENT_TYPES[grad.dtype], activation, grad.data_ptr(), 0 if z is None else z.data_ptr(),
+                                     0 if dz is None else dz.data_ptr(),
+                                     0 if bias_gradient is None else bias_gradient.data_ptr(),
+                                     0 if workspace is None else workspace.data_ptr(),
+                                     0 if row_limit is None else row_limit, grad.size(0), n, device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._routing_error().decode())
 
     def status(self, word):
         """OG_OK for a zero status word of `launch_checked`, else OG_ERR_TIMEOUT with

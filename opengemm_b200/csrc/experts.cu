@@ -1,0 +1,231 @@
+// Host side of the experts' products and of the gradients of products: tile
+// choice, tensor maps and the launch (experts.cuh has the kernel).
+#include <algorithm>
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "../../include/opengemm_b200.h"
+#include "experts_launch.h"
+#include "launch_common.h"
+
+namespace og {
+
+extern const ExpertKernel EXPERT_FORWARD16[];
+extern const int EXPERT_FORWARD16_COUNT;
+extern const ExpertKernel EXPERT_FORWARD8[];
+extern const int EXPERT_FORWARD8_COUNT;
+extern const ExpertKernel EXPERT_GRADIENT[];
+extern const int EXPERT_GRADIENT_COUNT;
+
+namespace {
+
+thread_local char experts_error[320];
+
+int experts_fail(int code, const char* format, ...) {
+  va_list args;
+  va_start(args, format);
+  vsnprintf(experts_error, sizeof experts_error, format, args);
+  va_end(args);
+  return code;
+}
+
+constexpr int XP_DEVICES = 64;
+constexpr int XP_STATIC_SMEM = 9 * 1024;  // barriers and the group tables
+
+// What a launch runs with.
+struct ExpertPlan {
+  int cta_group, tile_n;
+};
+
+// The tile of a launch.  Only bounds of the groups' sizes are known here (the
+// table of offsets is on the device), so they are taken as equal.
+//
+// A tile costs its K blocks plus about 2500 cycles outside them.  A K block
+// costs the larger of the MMAs (half the tile width per instruction, 8192
+// multiply-adds a cycle and SM for 16 bits) and, where a group has no more rows
+// than one tile and its weights are therefore read from memory exactly once,
+// the SM's share of the memory bandwidth (24 bytes a cycle).  Pairs of CTAs
+// share the N-side operand, which is what lets wide tiles run at the tensor
+// pipe's rate; narrow tiles exist to give every SM work when there are few.
+ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count) {
+  const int busy = std::max(1, std::min(groups, rows));
+  const int rows_each = ceil_div(std::max(rows, 1), busy);
+  static const ExpertPlan menu[] = {{2, 256}, {2, 128}, {1, 256}, {1, 128}, {1, 64}};
+  static const int mma_cycles[] = {560, 340, 620, 340, 220};
+  ExpertPlan best = menu[0];
+  double best_cost = 0;
+  for (int i = 0; i < 5; ++i) {
+    const ExpertPlan& c = menu[i];
+    if (glu && c.tile_n < 128) continue;
+    const int out_n = glu ? c.tile_n / 2 : c.tile_n;
+    const int m_tiles = mode == MODE_DW ? ceil_div(m_out, 128 * c.cta_group) : ceil_div(rows_each, 128 * c.cta_group);
+    const double tiles = double(mode == MODE_DW ? groups : busy) * m_tiles * ceil_div(cols, out_n);
+    const int blocks = mode == MODE_DW ? ceil_div(rows_each, 64) : blocks_fixed;
+    double block = mma_cycles[i];
+    if (mode != MODE_DW && m_tiles == 1) block = std::max(block, c.tile_n / c.cta_group * 128 / 24.0);
+    const double slots = sm_count / c.cta_group;
+    const double waves = std::max(1.0, double(int64_t((tiles + slots - 1) / slots)));
+    const double cost = waves * (blocks * block + 2500);
+    if (i == 0 || cost < best_cost) best = c, best_cost = cost;
+  }
+  return best;
+}
+
+int experts_sm_count(int device) {
+  static std::atomic<int> known[XP_DEVICES];
+  int count = known[device].load(std::memory_order_relaxed);
+  if (!count) {
+    if (cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || count <= 0) count = 148;
+    known[device].store(count, std::memory_order_relaxed);
+  }
+  return count;
+}
+
+const ExpertKernel* find_kernel(int kind, int cta_group, int mode, bool gather, bool glu, int out_bytes, int* index) {
+  const ExpertKernel* const lists[] = {EXPERT_FORWARD16, EXPERT_FORWARD8, EXPERT_GRADIENT};
+  const int counts[] = {EXPERT_FORWARD16_COUNT, EXPERT_FORWARD8_COUNT, EXPERT_GRADIENT_COUNT};
+  int at = 0;
+  for (int l = 0; l < 3; ++l)
+    for (int i = 0; i < counts[l]; ++i, ++at) {
+      const ExpertKernel& k = lists[l][i];
+      if (k.kind == kind && k.cta_group == cta_group && k.mode == mode && k.gather == int(gather) && k.glu == int(glu) && k.out_bytes == out_bytes) {
+        *index = at;
+        return &k;
+      }
+    }
+  return nullptr;
+}
+
+int launch_product(const OgExpertProduct& g, int device, void* stream) {
+  char why[256];
+  const int mode = g.mode;
+  if (mode < MODE_FORWARD || mode > MODE_DW) return experts_fail(OG_ERR_LAUNCH, "mode %d is none of 0..2", mode);
+  const bool bf16 = !std::strncmp(g.dtype, "bf16", 16), f16 = !std::strncmp(g.dtype, "f16", 16), e4m3 = !std::strncmp(g.dtype, "e4m3", 16);
+  if (!bf16 && !f16 && !(e4m3 && mode == MODE_FORWARD))
+    return experts_fail(OG_ERR_LAUNCH, "dtype %.16s is not served: bf16, f16, and e4m3 for the forward product", g.dtype);
+  if (g.groups < 1 || g.groups > XP_MAX_GROUPS) return experts_fail(OG_ERR_LAUNCH, "%d experts: 1 to %d are served", g.groups, XP_MAX_GROUPS);
+  if (!g.offsets && g.groups != 1) return experts_fail(OG_ERR_LAUNCH, "%d experts without a table of their rows", g.groups);
+  if (g.rows < 0 || g.n <= 0 || g.k <= 0) return experts_fail(OG_ERR_LAUNCH, "rows = %d, n = %d, k = %d", g.rows, g.n, g.k);
+  const int elem = e4m3 ? 1 : 2, multiple = 16 / elem;
+  if (g.k % multiple || (mode != MODE_FORWARD && g.n % multiple))
+    return experts_fail(OG_ERR_LAUNCH, "n = %d, k = %d: rows must be multiples of 16 bytes", g.n, g.k);
+  const bool glu = g.activation == ACT_SWIGLU || g.activation == ACT_GEGLU;
+  if (g.activation < ACT_NONE || g.activation > ACT_GEGLU || (g.activation && mode != MODE_FORWARD))
+    return experts_fail(OG_ERR_LAUNCH, "activation %d is not one of the forward product's", g.activation);
+  if (glu && g.n % 16) return experts_fail(OG_ERR_LAUNCH, "a gated activation takes a multiple of 16 weight rows, got %d", g.n);
+  if (g.out_f32 && mode == MODE_FORWARD) return experts_fail(OG_ERR_LAUNCH, "the forward product writes 16-bit values");
+  const bool gather = g.tokens != nullptr;
+  if (gather && mode == MODE_DX) return experts_fail(OG_ERR_LAUNCH, "the rows' gradient gathers nothing");
+  if (device < 0 || device >= XP_DEVICES) return experts_fail(OG_ERR_LAUNCH, "device %d is out of range: this library serves devices 0..%d", device, XP_DEVICES - 1);
+  int current = -1;
+  if (cudaGetDevice(&current) != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaGetDevice failed");
+  if (current != device && cudaSetDevice(device) != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaSetDevice(%d) failed", device);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int out_bytes = g.out_f32 ? 4 : 2;
+  if (g.rows == 0 || (gather && g.x_rows == 0)) {  // nothing to multiply: sums over no rows are zero
+    if (mode == MODE_DW && cudaMemsetAsync(g.out, 0, size_t(g.groups) * g.n * g.k * out_bytes, s) != cudaSuccess)
+      return experts_fail(OG_ERR_LAUNCH, "cudaMemsetAsync failed");
+    return OG_OK;
+  }
+  if (!g.x || !g.w || !g.out) return experts_fail(OG_ERR_LAUNCH, "x, w and out must be device pointers, got null");
+  if ((reinterpret_cast<uintptr_t>(g.x) | reinterpret_cast<uintptr_t>(g.w)) & 15)
+    return experts_fail(OG_ERR_LAUNCH, "operands must start on 16-byte boundaries");
+
+  ExpertParams p;
+  std::memset(&p, 0, sizeof p);
+  const int sm_count = experts_sm_count(device);
+  p.groups = g.groups;
+  p.rows = g.rows;
+  p.glu_offset = glu ? g.n / 2 : 0;
+  p.cols = mode == MODE_FORWARD ? (glu ? g.n / 2 : g.n) : g.k;
+  p.m_out = g.n;
+  p.k = mode == MODE_FORWARD ? g.k : g.n;
+  p.block_k = 128 / elem;
+  p.k_blocks = ceil_div(p.k, p.block_k);
+  const ExpertPlan plan = choose_plan(mode, glu, g.groups, g.rows, p.m_out, p.cols, p.k_blocks, sm_count);
+  p.tile_n = plan.tile_n;
+  p.out_tile_n = glu ? plan.tile_n / 2 : plan.tile_n;
+  p.tiles_n = ceil_div(p.cols, p.out_tile_n);
+  p.tiles_m_fixed = ceil_div(p.m_out, 128 * plan.cta_group);
+  p.band = 8;
+  p.y_bytes = plan.tile_n / plan.cta_group * 128;
+  p.stage_bytes = 16384 + p.y_bytes;
+  p.stages = std::min(XP_MAX_STAGES, (SMEM_LIMIT - XP_STATIC_SMEM - 1024 - 4 * XP_STAGING) / p.stage_bytes);
+  p.tmem_cols = pow2_at_least(2 * plan.tile_n);
+  const uint32_t x_columns = mode == MODE_DW, y_columns = mode != MODE_FORWARD;
+  const uint32_t fmt = bf16 ? 1u : 0u;  // e4m3 is code 0 of its kind, f16 of its own
+  p.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (x_columns << 15) | (y_columns << 16) | (uint32_t(plan.tile_n >> 3) << 17) |
+            (uint32_t(128 * plan.cta_group >> 4) << 24);
+  p.offsets = g.offsets;
+  p.tokens = g.tokens;
+  p.alpha = g.alpha;
+  p.factor = g.factor;
+  p.d = g.out;
+  p.preact = g.preactivation;
+  p.wait_limit_ns = current_wait_limit_ns();
+  p.ldd = p.cols;
+  p.ldz = g.n;
+  p.out_f16 = f16 && !g.out_f32;
+  p.vec_ok = ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.preactivation)) & 15) == 0 && (int64_t(p.cols) * out_bytes) % 16 == 0;
+  act_constants(g.activation, &p.act_shape, &p.act_a, &p.act_b);
+
+  const int type = e4m3 ? int(CU_TENSOR_MAP_DATA_TYPE_UINT8) : bf16 ? int(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16) : int(CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+  const CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B;
+  const uint32_t box = uint32_t(p.block_k);
+  const uint64_t k = uint64_t(g.k), n = uint64_t(g.n), x_rows = uint64_t(gather ? g.x_rows : g.rows);
+  int rc = OG_OK;
+  auto map = [&](CUtensorMap* out, const void* base, uint64_t inner, uint64_t rows, uint32_t box1, const char* which, uint64_t matrices = 0) {
+    if (rc == OG_OK) rc = encode_2d(out, base, type, inner, rows, inner * elem, box, box1, swizzle, 2, which, why, sizeof why, matrices);
+  };
+  if (mode == MODE_DW) {  // dz [rows, n] against x [rows, k], both along their rows
+    map(&p.map_x, g.x, n, uint64_t(g.rows), 64, "the output's gradient");
+    map(&p.map_y, g.w, k, x_rows, 64, "the rows");
+    if (gather) map(&p.map_x32, g.w, k, x_rows, 1, "the gathered rows");
+  } else {
+    const uint64_t inner = mode == MODE_FORWARD ? k : n;
+    map(&p.map_x, g.x, inner, x_rows, 128, "the rows");
+    map(&p.map_x32, g.x, inner, x_rows, gather ? 1 : 32, "the rows");
+    const uint32_t y_rows = mode == MODE_DX ? 64 : uint32_t(glu ? plan.tile_n / 2 : plan.tile_n / plan.cta_group);
+    map(&p.map_y, g.w, k, n, y_rows, "the weights", uint64_t(g.groups));
+  }
+  if (rc != OG_OK) return experts_fail(rc, "%s", why);
+
+  int index = 0;
+  const ExpertKernel* kernel = find_kernel(e4m3 ? KIND_F8F6F4 : KIND_F16, plan.cta_group, mode, gather, glu, out_bytes, &index);
+  if (!kernel) return experts_fail(OG_ERR_NO_KERNEL, "no kernel for this product");
+  static std::atomic<uint64_t> configured[XP_DEVICES];
+  if (!(configured[device].load(std::memory_order_acquire) >> index & 1)) {
+    const cudaError_t status = kernel->configure(SMEM_LIMIT - XP_STATIC_SMEM);
+    if (status != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(status));
+    configured[device].fetch_or(1ull << index, std::memory_order_release);
+  }
+  // At most this many tiles: every group may end in a partial one.
+  const int64_t m_tiles = mode == MODE_DW ? int64_t(g.groups) * p.tiles_m_fixed
+                                          : int64_t(g.rows) / (128 * plan.cta_group) + std::min(g.groups, g.rows);
+  const int clusters = int(std::min<int64_t>(sm_count / plan.cta_group, m_tiles * p.tiles_n));
+  const int smem = p.stages * p.stage_bytes + 4 * XP_STAGING + 1024;
+  const cudaError_t launched = kernel->launch(p, std::max(1, clusters) * plan.cta_group, smem, s);
+  if (launched != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "kernel launch failed: %s", cudaGetErrorString(launched));
+  return OG_OK;
+}
+
+}  // namespace
+}  // namespace og
+
+using namespace og;
+
+extern "C" {
+
+OG_API const char* og_b200_experts_error(void) { return experts_error; }
+
+OG_API int32_t og_b200_expert_product(const OgExpertProduct* product, int32_t device, void* stream) {
+  if (!product) return experts_fail(OG_ERR_LAUNCH, "null OgExpertProduct");
+  return launch_product(*product, device, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,578 @@
+// One persistent, warp-specialised tcgen05 kernel for products whose rows fall
+// into groups, each group with its own matrix (experts), and for the gradients
+// of such a product.  A single group without an offset table is the plain
+// matrix product, which makes it the kernel of gemm's gradients too.
+//
+//   MODE_FORWARD  out[r, :]    = act(alpha_e * x[r, :] . w_e^T)      r in expert e's rows
+//   MODE_DX       out[r, :]    = dz[r, :] . w_e
+//   MODE_DW       out[e, :, :] = sum over e's rows r of dz[r, :]^T x[r, :]
+//
+// The MMA reduces along the innermost (contiguous) extent of both operands in
+// the forward product; the gradients reduce along a row extent instead.  The
+// 16-bit MMA reads such an operand as it lies: a stage then holds boxes of 64
+// reduction rows x 64 columns (128 bytes, swizzled), and the matrix
+// descriptor says that the columns, not the reduction, are contiguous.  So no
+// operand is transposed through memory.
+//
+// Rows of a group may start anywhere (offsets come from a table on the device;
+// the host never sees them): tiles start at the group's first row, rows past
+// its end are computed from whatever lies there and not stored.  Only the
+// weight gradient, which sums over rows, has to cut its last block of 64 rows
+// short: warp 6 waits for that stage's data and clears the rows past the end
+// in shared memory before the MMA reads it.
+//
+// Roles as in kernel.cuh: warp 0 loads (one thread; all lanes when rows are
+// gathered, four rows a lane and instruction), warp 1 issues the MMAs, warps
+// 2-5 store.  Every wait is bounded.
+#pragma once
+
+#include "activation.cuh"
+#include "ptx.cuh"
+
+namespace og {
+
+enum ExpertMode : int { MODE_FORWARD = 0, MODE_DX = 1, MODE_DW = 2 };
+
+constexpr int XP_MAX_STAGES = 12;
+constexpr int XP_MAX_GROUPS = 1024;
+constexpr int XP_STAGING = 32 * 128;  // per epilogue warp: 32 rows of one 128-byte line
+
+__host__ __device__ constexpr int xp_threads(int mode) { return mode == MODE_DW ? 224 : 192; }
+
+struct alignas(64) ExpertParams {
+  CUtensorMap map_x;    // MMA-M side, boxes of 128 rows (64 x 64 in MODE_DW)
+  CUtensorMap map_x32;  // the same in boxes of 32 rows, for a group's last, short tile; gathered: one row
+  CUtensorMap map_y;    // MMA-N side
+  const int* offsets;   // [groups + 1] first row of each group; null: one group of all rows
+  const int* tokens;    // gathered operand: its row for each sorted row
+  const float* alpha;   // [groups], or null
+  float factor;         // on every sum, beside alpha
+  void* d;
+  void* preact;
+  unsigned long long wait_limit_ns;
+  int groups, rows;
+  int cols;             // output columns
+  int m_out;            // MODE_DW: output rows of each group
+  int k;                // reduction extent (MODE_DW: the group's rows)
+  int k_blocks, block_k;
+  int tile_n, out_tile_n, tiles_n, tiles_m_fixed;  // tiles_m_fixed: MODE_DW
+  int glu_offset;       // first row of the up half of the weights; 0 without a gate
+  int stages, stage_bytes, y_bytes;
+  unsigned idesc;
+  int band;             // M tiles per band of the tile order
+  int ldd, ldz;         // elements per row of `d` and `preact`
+  int vec_ok;           // rows of d and preact take 16-byte stores
+  int act_shape;
+  float act_a, act_b;
+  int out_f16;
+  int tmem_cols;
+};
+
+// One tile of work: group, its rows, and the tile's place.
+struct ExpertTile {
+  int group, first_row, rows;  // rows of the group
+  int mi, ni;
+};
+
+// Gathered rows: four rows of `tmap` (one-row boxes) into 512 consecutive bytes.
+template <int CTA_GROUP>
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
+  if constexpr (CTA_GROUP == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(tmap), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(tmap), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+        : "memory");
+}
+
+template <int CTA_GROUP>
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
+  if constexpr (CTA_GROUP == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+// Operand whose columns (the M or N extent) are contiguous: 128-byte swizzled
+// boxes of 64 columns x 64 reduction rows, 8 KiB each.  Leading offset: from
+// one box of 64 columns to the next; stride offset: eight reduction rows on.
+__device__ __forceinline__ uint64_t column_operand_desc(uint32_t smem_addr) {
+  return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(8192 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+template <int KIND, int CTA_GROUP, int MODE, bool GATHER, bool GLU, int OUT_BYTES>
+__global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __grid_constant__ ExpertParams p) {
+  constexpr int TILE_M = 128 * CTA_GROUP;
+  constexpr bool X_COLUMNS = MODE == MODE_DW, Y_COLUMNS = MODE != MODE_FORWARD;
+  constexpr int CHUNK = OUT_BYTES == 2 ? 64 : 32;  // columns of a 128-byte staging row
+  constexpr int UNIT = 16 / OUT_BYTES;
+
+  extern __shared__ uint8_t dyn_smem[];
+  __shared__ __align__(8) uint64_t bars[4 * XP_MAX_STAGES + 5];
+  __shared__ int group_row[XP_MAX_GROUPS + 1];   // first row of each group
+  __shared__ int group_tile[XP_MAX_GROUPS + 1];  // first tile of each group
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CTA_GROUP == 2 ? cluster_cta_rank() : 0u;
+  const int cluster_id = blockIdx.x / CTA_GROUP, num_clusters = gridDim.x / CTA_GROUP;
+  const uint32_t ring = (smem_u32(dyn_smem) + 1023u) & ~1023u;
+  const uint32_t staging = ring + p.stages * p.stage_bytes;
+  const uint32_t bar_full = smem_u32(bars);
+  const uint32_t bar_empty = bar_full + 8 * XP_MAX_STAGES;
+  const uint32_t bar_ready = bar_empty + 8 * XP_MAX_STAGES;  // MODE_DW: a short block's rows past the end are cleared
+  const uint32_t bar_go = bar_ready + 8 * XP_MAX_STAGES;     // MODE_DW, a short block: asked for (leader), landed (pair's second CTA)
+  const uint32_t bar_acc_full = bar_go + 8 * XP_MAX_STAGES, bar_acc_empty = bar_acc_full + 16;
+  const uint32_t bar_tmem = bar_acc_empty + 16;
+  const WaitCtx ctx{&abort_flag, nullptr, p.wait_limit_ns};
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&p.map_x);
+    prefetch_tmap(&p.map_y);
+    if (MODE == MODE_FORWARD || GATHER) prefetch_tmap(&p.map_x32);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+      mbar_init(bar_ready + 8 * s, CTA_GROUP);
+      mbar_init(bar_go + 8 * s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_acc_full + 8 * s, 1);
+      mbar_init(bar_acc_empty + 8 * s, 4 * CTA_GROUP);
+    }
+    mbar_init(bar_tmem, CTA_GROUP);
+    abort_flag = 0;
+    mbar_init_fence();
+  }
+  __syncthreads();
+  if (CTA_GROUP == 2) cluster_sync_all();
+  if (warp == 1) {
+    tmem_alloc<CTA_GROUP>(smem_u32(&tmem_slot), p.tmem_cols);
+    tmem_relinquish<CTA_GROUP>();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(bar_tmem);
+      if constexpr (CTA_GROUP == 2) mbar_arrive_cluster(map_to_cta(bar_tmem, rank ^ 1u));
+    }
+  }
+  // The offsets are an earlier kernel's output, like everything else read here.
+  pdl_wait_prior_grids();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+
+  // Group table: rows and tiles before each group.  Warp 2 sums; a lane takes a
+  // contiguous run of groups.
+  const int groups = p.groups;
+  for (int i = threadIdx.x; i <= groups; i += xp_threads(MODE)) group_row[i] = p.offsets ? p.offsets[i] : i * p.rows;
+  __syncthreads();
+  if (warp == 2) {
+    auto tiles_of = [&](int e) {
+      const int m_tiles = MODE == MODE_DW ? p.tiles_m_fixed : (group_row[e + 1] - group_row[e] + TILE_M - 1) / TILE_M;
+      return m_tiles * p.tiles_n;
+    };
+    const int per = (groups + 31) / 32, first = min(lane * per, groups), last = min(first + per, groups);
+    int sum = 0;
+    for (int e = first; e < last; ++e) sum += tiles_of(e);
+    int before = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xFFFFFFFFu, before, d);
+      if (lane >= d) before += other;
+    }
+    before -= sum;
+    for (int e = first; e < last; ++e) {
+      group_tile[e] = before;
+      before += tiles_of(e);
+    }
+    if (lane == 31) group_tile[groups] = before;
+  }
+  __syncthreads();
+  const int num_tiles = group_tile[groups];
+
+  // Tile t: the last group that starts at or before it (empty groups share
+  // their successor's start), then bands of `band` M tiles, M fastest inside a
+  // band, so that tiles running together share weights and rows in L2.
+  auto find_tile = [&](int t, ExpertTile& w) {
+    int lo = 0, hi = groups;  // group_tile[lo] <= t < group_tile[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (group_tile[mid] <= t) lo = mid; else hi = mid;
+    }
+    w.group = lo;
+    w.first_row = group_row[lo];
+    w.rows = group_row[lo + 1] - w.first_row;
+    const int m_tiles = MODE == MODE_DW ? p.tiles_m_fixed : (w.rows + TILE_M - 1) / TILE_M;
+    const int local = t - group_tile[lo];
+    const int band = local / (p.band * p.tiles_n);
+    const int height = min(p.band, m_tiles - band * p.band);
+    const int rest = local - band * p.band * p.tiles_n;
+    w.ni = rest / height;
+    w.mi = band * p.band + rest - w.ni * height;
+  };
+  auto k_blocks_of = [&](const ExpertTile& w) { return MODE == MODE_DW ? (w.rows + 63) / 64 : p.k_blocks; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (GATHER || elect_one()) {
+      const int stages = p.stages, block_k = p.block_k, tile_n = p.tile_n;
+      const uint32_t stage_bytes = p.stage_bytes, y_bytes = p.y_bytes;
+      const int y_rows = tile_n / CTA_GROUP;       // MMA-N rows this CTA loads
+      const int y_boxes = (y_rows + 63) / 64;      // column boxes of a Y_COLUMNS operand
+      const bool leads = !GATHER || lane == 0;     // the one thread that credits bytes and loads whole boxes
+      int stage = 0;
+      uint32_t phase = 0, issued = 0;
+      bool ok = true;
+      for (int t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+        ExpertTile w;
+        find_tile(t, w);
+        const int blocks = k_blocks_of(w);
+        const int left = w.rows - w.mi * TILE_M;   // rows of the group from this tile on
+        const int x_row = w.first_row + w.mi * TILE_M + int(rank) * 128;
+        // Rows of the M side that each CTA of the pair loads, in pieces of 32 (gathered: 4).
+        int mine = 128, whole = 128 * CTA_GROUP;
+        if constexpr (MODE != MODE_DW) {
+          constexpr int PIECE = GATHER ? 4 : 32;
+          const int l0 = min(max(left, 0), 128), l1 = CTA_GROUP == 2 ? min(max(left - 128, 0), 128) : 0;
+          const int p0 = (l0 + PIECE - 1) / PIECE * PIECE, p1 = (l1 + PIECE - 1) / PIECE * PIECE;
+          mine = rank == 0 ? p0 : p1;
+          whole = p0 + p1;
+        }
+        const uint32_t tx = uint32_t(whole) * 128 + CTA_GROUP * y_bytes;
+        int token[4];
+        if constexpr (GATHER && MODE == MODE_FORWARD) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)  // rows past the group's end repeat its last row
+            token[i] = 4 * lane < mine ? p.tokens[min(x_row + 4 * lane + i, w.first_row + w.rows - 1)] : 0;
+        }
+        auto tokens_of = [&](int kb) {
+          if constexpr (GATHER && MODE == MODE_DW) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) token[i] = p.tokens[w.first_row + min(kb * 64 + 4 * (lane & 15) + i, w.rows - 1)];
+          }
+        };
+        if (blocks > 0) tokens_of(0);
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, ctx, SITE_PRODUCER_EMPTY)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full_local = bar_full + 8 * stage;
+          const uint32_t full = CTA_GROUP == 2 ? map_to_cta(full_local, 0) : full_local;
+          const uint32_t sx = ring + stage * stage_bytes, sy = sx + 16384;
+          if (leads) {
+            if (rank == 0) mbar_expect_tx(full_local, tx);
+            if constexpr (MODE == MODE_FORWARD) {
+              const int n0 = w.ni * p.out_tile_n;
+              if constexpr (GLU) {  // gate rows first, up rows behind them: one half per CTA of a pair
+                if constexpr (CTA_GROUP == 2) {
+                  tma_load_3d<2>(sy, &p.map_y, kb * block_k, n0 + (rank ? p.glu_offset : 0), w.group, full);
+                } else {
+                  tma_load_3d<1>(sy, &p.map_y, kb * block_k, n0, w.group, full);
+                  tma_load_3d<1>(sy + y_bytes / 2, &p.map_y, kb * block_k, n0 + p.glu_offset, w.group, full);
+                }
+              } else {
+                tma_load_3d<CTA_GROUP>(sy, &p.map_y, kb * block_k, n0 + int(rank) * y_rows, w.group, full);
+              }
+            } else if constexpr (MODE == MODE_DX) {
+              const int c0 = w.ni * tile_n + int(rank) * y_rows;
+              for (int b = 0; b < y_boxes; ++b) tma_load_3d<CTA_GROUP>(sy + b * 8192, &p.map_y, c0 + 64 * b, kb * 64, w.group, full);
+            } else {
+              const int r = w.first_row + kb * 64, m0 = w.mi * TILE_M + int(rank) * 128;
+              tma_load_2d<CTA_GROUP>(sx, &p.map_x, m0, r, full);
+              tma_load_2d<CTA_GROUP>(sx + 8192, &p.map_x, m0 + 64, r, full);
+              if constexpr (!GATHER) {
+                const int c0 = w.ni * tile_n + int(rank) * y_rows;
+                for (int b = 0; b < y_boxes; ++b) tma_load_2d<CTA_GROUP>(sy + b * 8192, &p.map_y, c0 + 64 * b, r, full);
+              }
+            }
+            if constexpr (MODE != MODE_DW && !GATHER) {
+              if (mine == 128) tma_load_2d<CTA_GROUP>(sx, &p.map_x, kb * block_k, x_row, full);
+              else
+                for (int r = 0; r < mine; r += 32) tma_load_2d<CTA_GROUP>(sx + r * 128, &p.map_x32, kb * block_k, x_row + r, full);
+            }
+          }
+          if constexpr (GATHER && MODE == MODE_FORWARD) {
+            if (4 * lane < mine)
+              tma_gather4<CTA_GROUP>(sx + lane * 512, &p.map_x32, kb * block_k, token[0], token[1], token[2], token[3], full);
+          }
+          if constexpr (GATHER && MODE == MODE_DW) {
+            const int c0 = w.ni * tile_n + int(rank) * y_rows;
+            for (int b = lane >> 4; b < y_boxes; b += 2)
+              tma_gather4<CTA_GROUP>(sy + b * 8192 + (lane & 15) * 512, &p.map_x32, c0 + 64 * b, token[0], token[1], token[2], token[3], full);
+            if (kb + 1 < blocks) tokens_of(kb + 1);
+          }
+          if constexpr (MODE == MODE_DW) {  // a short block is on its way: warp 6 may look for it
+            if (leads && rank == 0 && kb == blocks - 1 && (w.rows & 63)) mbar_arrive(bar_go + 8 * stage);
+          }
+          ++issued;
+          if (++stage == stages) stage = 0, phase ^= 1;
+        }
+      }
+      if (!ok && rank == 0 && leads) {
+        // Loads in flight still land: give each armed barrier a bounded chance before teardown.
+        int s = stage;
+        uint32_t ph = phase;
+        const uint32_t pending = issued < uint32_t(p.stages) ? issued : uint32_t(p.stages);
+        for (uint32_t back = 0; back < pending; ++back) {
+          if (--s < 0) s = p.stages - 1, ph ^= 1;
+          const uint64_t start = global_timer_ns();
+          while (!mbar_try_wait(bar_full + 8 * s, ph) && global_timer_ns() - start < 1000000ull) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- MMA issuer
+    if (rank == 0 && elect_one()) {
+      const uint64_t desc_stage = uint64_t(p.stage_bytes >> 4);
+      const uint64_t dx0 = X_COLUMNS ? column_operand_desc(ring) : operand_desc(ring);
+      const uint64_t dy0 = Y_COLUMNS ? column_operand_desc(ring + 16384) : operand_desc(ring + 16384);
+      // Operand start from one MMA to the next: 32 bytes of K, or 16 rows of a column box.
+      constexpr uint64_t X_STEP = X_COLUMNS ? 128 : 2, Y_STEP = Y_COLUMNS ? 128 : 2;
+      const int stages = p.stages, block_k = p.block_k, mma_k = block_k / 4;
+      const uint32_t idesc = p.idesc;
+      int stage = 0, tile_idx = 0;
+      uint32_t phase = 0, cleared = 0;  // bit s: parity of stage s's next short block
+      uint64_t stage_off = 0;
+      bool ok = mbar_wait(bar_tmem, 0, ctx, SITE_TMEM_READY);
+      tc_fence_after_sync();
+      const uint32_t tmem_base = tmem_slot;
+      for (int t = cluster_id; ok && t < num_tiles; t += num_clusters, ++tile_idx) {
+        ExpertTile w;
+        find_tile(t, w);
+        const int blocks = k_blocks_of(w);
+        const int slot = tile_idx & 1;
+        if (!mbar_wait(bar_acc_empty + 8 * slot, ((tile_idx >> 1) & 1) ^ 1, ctx, SITE_MMA_ACC_EMPTY)) break;
+        tc_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + slot * p.tile_n;
+        uint32_t accumulate = 0;
+        int k_left = MODE == MODE_DW ? w.rows : p.k;
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(bar_full + 8 * stage, phase, ctx, SITE_MMA_FULL)) {
+            ok = false;
+            break;
+          }
+          if constexpr (MODE == MODE_DW) {
+            if (k_left < 64) {
+              if (!mbar_wait(bar_ready + 8 * stage, (cleared >> stage) & 1, ctx, SITE_MMA_FULL)) {
+                ok = false;
+                break;
+              }
+              cleared ^= 1u << stage;
+            }
+          }
+#pragma unroll
+          for (int ki = 0; ki < 4; ++ki) {
+            if (ki == 0 || ki * mma_k < k_left) {  // an MMA that would read zeros only is skipped
+              mma_dense<KIND, CTA_GROUP>(d_tmem, dx0 + stage_off + ki * X_STEP, dy0 + stage_off + ki * Y_STEP, idesc, accumulate);
+              accumulate = 1;
+            }
+          }
+          mma_commit<CTA_GROUP>(bar_empty + 8 * stage);
+          k_left -= block_k;
+          stage_off += desc_stage;
+          if (++stage == stages) stage = 0, phase ^= 1, stage_off = 0;
+        }
+        if (ok) mma_commit<CTA_GROUP>(bar_acc_full + 8 * slot);
+      }
+    }
+  } else if (MODE == MODE_DW && warp == 6) {
+    // ------------------------------------------------------- short blocks
+    // Counts the stages as the producer does.  Once the producer has asked for
+    // a short block, the leader waits for its data (its barrier counts both
+    // CTAs' bytes), tells the pair's other CTA, and each clears its own rows past
+    // the group's end.  The full barrier is looked at only after the producer's
+    // word: until the MMA has used the block, its phase then cannot pass by.
+    int stage = 0;
+    uint32_t phase = 0, told = 0;
+    bool ok = true;
+    const int boxes = 2 + p.tile_n / CTA_GROUP / 64;
+    for (int t = cluster_id; ok && t < num_tiles; t += num_clusters) {
+      ExpertTile w;
+      find_tile(t, w);
+      const int blocks = k_blocks_of(w), tail = w.rows & 63;
+      if (blocks == 0) continue;
+      for (int kb = 0; kb < blocks; ++kb) {
+        if (kb == blocks - 1 && tail) {
+          ok = mbar_wait(bar_go + 8 * stage, (told >> stage) & 1, ctx, SITE_MMA_FULL);
+          if (ok && rank == 0) ok = mbar_wait(bar_full + 8 * stage, phase, ctx, SITE_MMA_FULL);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          told ^= 1u << stage;
+          if (CTA_GROUP == 2 && rank == 0 && lane == 0) mbar_arrive_cluster(map_to_cta(bar_go + 8 * stage, 1));
+          // Rows tail .. 63 of every 64 x 128-byte box: whole lines, so the swizzle does not matter.
+          const uint32_t base = ring + stage * p.stage_bytes;
+          for (int b = 0; b < boxes; ++b)
+            for (int i = tail * 8 + lane; i < 512; i += 32) st_shared_v4(base + b * 8192 + i * 16, 0u, 0u, 0u, 0u);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CTA_GROUP == 2) mbar_arrive_cluster(map_to_cta(bar_ready + 8 * stage, 0));
+            else mbar_arrive(bar_ready + 8 * stage);
+          }
+        }
+        if (++stage == p.stages) stage = 0, phase ^= 1;
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int quarter = warp & 3;
+    const uint32_t lane_base = uint32_t(quarter * 32) << 16;
+    const uint32_t acc_empty_leader = CTA_GROUP == 2 ? map_to_cta(bar_acc_empty, 0) : bar_acc_empty;
+    const uint32_t my_buf = staging + (warp - 2) * XP_STAGING;
+    const int sub_row = lane >> 3, unit = lane & 7;
+    const int out_tile_n = p.out_tile_n, cols = p.cols;
+    const bool out_f16 = p.out_f16 != 0, vec_ok = p.vec_ok != 0;
+    auto pack2 = [&](float lo, float hi) { return out_f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
+    const bool allocated = mbar_wait(bar_tmem, 0, ctx, SITE_TMEM_READY);
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_slot;
+    int tile_idx = 0;
+    for (int t = cluster_id; __all_sync(0xFFFFFFFFu, allocated) && t < num_tiles; t += num_clusters, ++tile_idx) {
+      ExpertTile w;
+      find_tile(t, w);
+      const int slot = tile_idx & 1;
+      const bool ready = mbar_wait(bar_acc_full + 8 * slot, (tile_idx >> 1) & 1, ctx, SITE_EPI_ACC_FULL);
+      if (!__all_sync(0xFFFFFFFFu, ready)) break;
+      tc_fence_after_sync();
+      const int local_row = w.mi * TILE_M + int(rank) * 128 + quarter * 32;  // this warp's first row of the group's output
+      const int group_rows = MODE == MODE_DW ? p.m_out : w.rows;
+      const int valid = min(max(group_rows - local_row, 0), 32);             // rows this warp stores
+      const size_t row0 = size_t(MODE == MODE_DW ? size_t(w.group) * p.m_out : size_t(w.first_row)) + local_row;
+      const int col0 = w.ni * out_tile_n;
+      const uint32_t acc = tmem_base + lane_base + slot * p.tile_n;
+      const bool nothing = MODE == MODE_DW && w.rows == 0;                   // no rows: the sum is zero
+      const float alpha = MODE == MODE_FORWARD && p.alpha ? p.alpha[w.group] * p.factor : p.factor;
+
+      // CHUNK columns of this lane's row, through the warp's swizzled buffer, as
+      // whole 128-byte segments of four rows an instruction; unaligned rows
+      // element by element.
+      auto store = [&](const float* v, uint8_t* base, int ld, int col, int limit) {
+        if (vec_ok) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            uint32_t q[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              q[h] = OUT_BYTES == 4 ? __float_as_uint(v[(4 * u + h) % CHUNK]) : pack2(v[(8 * u + 2 * h) % CHUNK], v[(8 * u + 2 * h + 1) % CHUNK]);
+            st_shared_v4(my_buf + lane * 128 + ((u ^ (lane & 7)) << 4), q[0], q[1], q[2], q[3]);
+          }
+          __syncwarp();
+          const int gcol = col + unit * UNIT;
+          if (gcol < limit) {
+            uint8_t* dst = base + ((row0 + sub_row) * ld + gcol) * OUT_BYTES;
+            const size_t step = size_t(4) * ld * OUT_BYTES;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + sub_row;
+              if (r < valid) *reinterpret_cast<uint4*>(dst + i * step) = ld_shared_v4(my_buf + r * 128 + ((unit ^ (r & 7)) << 4));
+            }
+          }
+          __syncwarp();
+        } else if (lane < valid) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            if (col + j < limit) {
+              const size_t at = (row0 + lane) * ld + col + j;
+              if constexpr (OUT_BYTES == 4) reinterpret_cast<float*>(base)[at] = v[j];
+              else reinterpret_cast<uint16_t*>(base)[at] = uint16_t(pack2(v[j], 0.0f) & 0xFFFFu);
+            }
+          }
+        }
+      };
+      auto load = [&](int c, float* v) {
+        uint32_t* raw = reinterpret_cast<uint32_t*>(v);
+        tmem_ld_32(acc + c, raw);
+        if constexpr (CHUNK == 64) tmem_ld_32(acc + c + 32, raw + 32);
+      };
+      auto settle = [&](float* v) {
+        uint32_t* raw = reinterpret_cast<uint32_t*>(v);
+        tmem_ld_settle_32(raw);
+        if constexpr (CHUNK == 64) tmem_ld_settle_32(raw + 32);
+      };
+      auto activate = [&](float* v) {
+        if (p.act_shape == SHAPE_SIGMOID) {
+          const float a = p.act_a, b = p.act_b;
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_SIGMOID>(v[j], a, b);
+        } else if (p.act_shape == SHAPE_PHI) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_PHI>(v[j], 0.f, 0.f);
+        } else if (p.act_shape == SHAPE_RELU) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_RELU>(v[j], 0.f, 0.f);
+        }
+      };
+
+      if (valid > 0) {
+        for (int c = 0; c < out_tile_n && col0 + c < cols; c += CHUNK) {
+          float v[CHUNK];
+          if (nothing) {
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) v[j] = 0.0f;
+          } else {
+            load(c, v);
+            if constexpr (GLU) {
+              float up[CHUNK];
+              load(out_tile_n + c, up);
+              tmem_ld_wait();
+              settle(v);
+              settle(up);
+              if (alpha != 1.0f) {
+#pragma unroll
+                for (int j = 0; j < CHUNK; ++j) v[j] *= alpha, up[j] *= alpha;
+              }
+              if (p.preact) {
+                store(v, static_cast<uint8_t*>(p.preact), p.ldz, col0 + c, cols);
+                store(up, static_cast<uint8_t*>(p.preact), p.ldz, p.glu_offset + col0 + c, p.glu_offset + cols);
+              }
+              activate(v);
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j) v[j] *= up[j];
+            } else {
+              tmem_ld_wait();
+              settle(v);
+              if (alpha != 1.0f) {
+#pragma unroll
+                for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
+              }
+              if constexpr (MODE == MODE_FORWARD) {
+                if (p.preact) store(v, static_cast<uint8_t*>(p.preact), p.ldz, col0 + c, cols);
+                activate(v);
+              }
+            }
+          }
+          store(v, static_cast<uint8_t*>(p.d), p.ldd, col0 + c, cols);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CTA_GROUP == 2) mbar_arrive_cluster(acc_empty_leader + 8 * slot);
+        else mbar_arrive(bar_acc_empty + 8 * slot);
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (CTA_GROUP == 2) cluster_sync_all();
+  tc_fence_after_sync();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc<CTA_GROUP>(tmem_slot, p.tmem_cols);
+  }
+}
+
+}  // namespace og

@@ -48,8 +48,9 @@ struct MapKey {
   uint64_t dim0, dim1, stride;
   uint32_t box0, box1;
   int type, swizzle, l2;
+  uint64_t dim2 = 0;  // 0: a 2-D map
   bool operator==(const MapKey& o) const {
-    return base == o.base && dim0 == o.dim0 && dim1 == o.dim1 && stride == o.stride &&
+    return dim2 == o.dim2 && base == o.base && dim0 == o.dim0 && dim1 == o.dim1 && stride == o.stride &&
            box0 == o.box0 && box1 == o.box1 && type == o.type && swizzle == o.swizzle && l2 == o.l2;
   }
 };
@@ -81,17 +82,19 @@ inline uint64_t mix_hash(uint64_t h, uint64_t v) {
   return h;
 }
 
-// A 2-D tiled map over `base`: dim0 innermost (elements), rows `stride` bytes
-// apart.  Out-of-bounds parts of a box read as zero and are clipped on store.
+// A tiled map over `base`: dim0 innermost (elements), rows `stride` bytes
+// apart; with `dim2` > 0 a 3-D one over that many such matrices, one behind
+// the other, in boxes of one.  Out-of-bounds parts of a box read as zero and
+// are clipped on store.
 // Returns OG_OK, or OG_ERR_TENSORMAP with the reason in `why`.
 inline int encode_2d(CUtensorMap* out, const void* base, int type, uint64_t dim0, uint64_t dim1,
                      uint64_t stride, uint32_t box0, uint32_t box1, CUtensorMapSwizzle swizzle, int l2,
-                     const char* which, char* why, size_t why_cap) {
-  const MapKey key{base, dim0, dim1, stride, box0, box1, type, int(swizzle), l2};
+                     const char* which, char* why, size_t why_cap, uint64_t dim2 = 0) {
+  const MapKey key{base, dim0, dim1, stride, box0, box1, type, int(swizzle), l2, dim2};
   uint64_t h = mix_hash(0, reinterpret_cast<uint64_t>(base));
   h = mix_hash(h, dim0 * 1315423911ull + dim1);
   h = mix_hash(h, (uint64_t(box0) << 32) | box1);
-  h = mix_hash(h, stride * 31 + uint64_t(type) * 7 + uint64_t(swizzle) * 3 + uint64_t(l2));
+  h = mix_hash(h, stride * 31 + uint64_t(type) * 7 + uint64_t(swizzle) * 3 + uint64_t(l2) + (dim2 << 20));
   MapSet& set = map_cache[(h >> 8) % MAP_SETS];
   const uint64_t tag = h | 1;
   for (int w = 0; w < MAP_WAYS; ++w)
@@ -106,15 +109,15 @@ inline int encode_2d(CUtensorMap* out, const void* base, int type, uint64_t dim0
     snprintf(why, why_cap, "cuTensorMapEncodeTiled is not available: no CUDA driver");
     return OG_ERR_TENSORMAP;
   }
-  const cuuint64_t dims[2] = {dim0, dim1};
-  const cuuint64_t strides[1] = {stride};
-  const cuuint32_t box[2] = {box0, box1};
-  const cuuint32_t elem_strides[2] = {1, 1};
+  const cuuint64_t dims[3] = {dim0, dim1, dim2};
+  const cuuint64_t strides[2] = {stride, stride * dim1};
+  const cuuint32_t box[3] = {box0, box1, 1};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
   const CUtensorMapL2promotion promo = l2 == 2   ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B
                                        : l2 == 1 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
                                                  : CU_TENSOR_MAP_L2_PROMOTION_NONE;
   const CUresult status =
-      encode(out, CUtensorMapDataType(type), 2, const_cast<void*>(base), dims, strides, box,
+      encode(out, CUtensorMapDataType(type), dim2 ? 3 : 2, const_cast<void*>(base), dims, strides, box,
              elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promo,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (status != CUDA_SUCCESS) {

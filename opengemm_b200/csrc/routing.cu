@@ -1,0 +1,784 @@
+// Routing of tokens to experts and what surrounds the experts' products: the
+// choice (route) and its gradient, the order of rows by expert (plan), the
+// weighted sum of a token's rows (combine) and its gradient, and the gradient
+// of an activation.  None of them multiplies matrices: they are bound by
+// memory, or by launch latency for the few tokens of a decoding step.
+//
+// All kernels wait for the previous grid before they touch memory and let the
+// next one start early (programmatic dependent launch).
+#include <algorithm>
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/opengemm_b200.h"
+#include "activation.cuh"
+#include "ptx.cuh"
+
+namespace og {
+namespace {
+
+constexpr unsigned ALL = 0xFFFFFFFFu;
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// Two 16-bit values of a 32-bit word, and back.
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return make_float2(half_bits_to_float(w), half_bits_to_float(w >> 16));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2_of(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2_of<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack2_of<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* at, float* v) {
+  const uint4 q = *reinterpret_cast<const uint4*>(at);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(w[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load8(const float* at, float* v) {
+  const float4 a = reinterpret_cast<const float4*>(at)[0], b = reinterpret_cast<const float4*>(at)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* at, const float* v) {
+  *reinterpret_cast<uint4*>(at) =
+      make_uint4(pack2_of<T>(v[0], v[1]), pack2_of<T>(v[2], v[3]), pack2_of<T>(v[4], v[5]), pack2_of<T>(v[6], v[7]));
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d /= 2) v += __shfl_xor_sync(ALL, v, d);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d; d /= 2) v = fmaxf(v, __shfl_xor_sync(ALL, v, d));
+  return v;
+}
+
+// ------------------------------------------------------------------- route
+
+// Order of scores as unsigned integers: 0 for what may not be chosen (a score
+// of -infinity included), NaN above everything, -0 equal to 0.
+__device__ __forceinline__ uint32_t score_key(float c, bool open) {
+  if (!open || c == -INFINITY) return 0u;
+  if (c != c) return 0xFFFFFFFFu;
+  const uint32_t bits = __float_as_uint(c + 0.0f);
+  return (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float key_score(uint32_t key) {
+  if (key == 0xFFFFFFFFu) return __uint_as_float(0x7FC00000u);
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
+}
+
+struct RouteParams {
+  const void* logits;
+  const float* bias;
+  float* weights;
+  int* indices;
+  const float* grad_weights;
+  void* grad_logits;
+  long long tokens;
+  int experts, top_k, sigmoid, groups, each, top_groups, group_top, renormalise;
+  float scale;
+};
+
+// A row's scores: exp(l - top) / sum, or the logistic function.  `top` and
+// `inverse` come from row_scale; a row without any finite logit scores 0.
+struct RowScale {
+  float top, inverse;
+};
+template <int VALUES>
+__device__ __forceinline__ RowScale row_scale(const float (&l)[VALUES], bool sigmoid) {
+  RowScale r{0.0f, 1.0f};
+  if (sigmoid) return r;
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) top = fmaxf(top, l[j]);
+  r.top = warp_max(top);
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) sum += l[j] == -INFINITY ? 0.0f : expf(l[j] - r.top);
+  sum = warp_sum(sum);
+  r.inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  return r;
+}
+__device__ __forceinline__ float score_of(float l, const RowScale& r, bool sigmoid) {
+  if (l == -INFINITY) return 0.0f;
+  return sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - r.top) * r.inverse;
+}
+
+constexpr int ROUTE_WARPS = 4;
+
+// One warp per token; lane `lane` holds the experts lane, lane + 32, ...  A
+// choice is one warp-wide maximum of the keys and one minimum of the indices
+// that reach it, and only the winning lane rescans its values: top_k * 2
+// reductions a token.  Without a bias the order of the scores is that of the
+// logits, which no rounding blurs, so those are compared.
+template <int VALUES, typename T>
+__global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RouteParams p) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const long long token = (long long)blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5);
+  if (token >= p.tokens) return;
+  const T* row = static_cast<const T*>(p.logits) + token * p.experts;
+  float l[VALUES];
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) l[j] = j * 32 + lane < p.experts ? to_float(row[j * 32 + lane]) : -INFINITY;
+  const bool sigmoid = p.sigmoid != 0;
+  const RowScale r = row_scale(l, sigmoid);
+  uint32_t key[VALUES];
+  const bool by_score = p.bias != nullptr || p.groups > 1;
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) {
+    const int id = j * 32 + lane;
+    float c = l[j];
+    if (by_score && c != -INFINITY) c = score_of(l[j], r, sigmoid) + (p.bias && id < p.experts ? p.bias[id] : 0.0f);
+    key[j] = score_key(c, l[j] != -INFINITY);
+  }
+  if (p.groups > 1) {
+    uint32_t group_key = 0;  // of group `lane`
+    for (int g = 0; g < p.groups; ++g) {
+      const int first = g * p.each, last = first + p.each;
+      uint32_t best = 0;
+      int at = 0x7FFFFFFF;
+#pragma unroll
+      for (int j = 0; j < VALUES; ++j) {
+        const int id = j * 32 + lane;
+        if (id >= first && id < last && key[j] > best) best = key[j], at = id;
+      }
+      const uint32_t one = __reduce_max_sync(ALL, best);
+      float score = key_score(one);
+      if (p.group_top == 2 && one) {
+        const int winner = int(__reduce_min_sync(ALL, unsigned(best == one ? at : 0x7FFFFFFF)));
+        uint32_t second = 0;
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) {
+          const int id = j * 32 + lane;
+          if (id >= first && id < last && id != winner) second = max(second, key[j]);
+        }
+        second = __reduce_max_sync(ALL, second);
+        if (second) score += key_score(second);
+      }
+      if (lane == g) group_key = one ? score_key(score, true) : 0u;
+    }
+    uint32_t open = 0;
+    for (int i = 0; i < p.top_groups; ++i) {
+      const uint32_t best = __reduce_max_sync(ALL, group_key);
+      if (!best) break;
+      const int winner = __ffs(__ballot_sync(ALL, group_key == best)) - 1;
+      open |= 1u << winner;
+      if (lane == winner) group_key = 0;
+    }
+#pragma unroll
+    for (int j = 0; j < VALUES; ++j) {
+      const int id = j * 32 + lane;
+      if (id < p.experts && !(open >> (id / p.each) & 1)) key[j] = 0;
+      if (!p.bias && key[j]) key[j] = score_key(l[j], true);  // inside the open groups the logits decide
+    }
+  }
+  uint32_t best = 0;
+  int at = 0x7FFFFFFF;
+  auto rescan = [&] {
+    best = 0, at = 0x7FFFFFFF;
+#pragma unroll
+    for (int j = 0; j < VALUES; ++j)
+      if (key[j] > best) best = key[j], at = j * 32 + lane;
+  };
+  rescan();
+  int mine = -1;  // choice number `lane`
+  for (int i = 0; i < p.top_k; ++i) {
+    const uint32_t top = __reduce_max_sync(ALL, best);
+    if (!top) break;
+    const int winner = int(__reduce_min_sync(ALL, unsigned(best == top ? at : 0x7FFFFFFF)));
+    if (lane == i) mine = winner;
+    if (at == winner) {
+#pragma unroll
+      for (int j = 0; j < VALUES; ++j)
+        if (j * 32 + lane == winner) key[j] = 0;
+      rescan();
+    }
+  }
+  float w = mine >= 0 ? score_of(to_float(row[mine]), r, sigmoid) : 0.0f;
+  if (p.renormalise) {
+    const float total = warp_sum(w);
+    w = total == 0.0f ? 0.0f : w / total;
+  }
+  if (lane < p.top_k) {
+    p.weights[token * p.top_k + lane] = w * p.scale;
+    p.indices[token * p.top_k + lane] = mine;
+  }
+}
+
+// d weights -> d logits.  q: the chosen scores, S their sum, g' the incoming
+// gradient times the factor:  dq = (g' - sum(g' q) / S) / S when renormalised,
+// else g'.  Softmax: dl = s (ds - sum(ds s)), where the sum vanishes after a
+// renormalisation; logistic: dl = ds s (1 - s).
+template <int VALUES, typename T>
+__global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const RouteParams p) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const long long token = (long long)blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5);
+  if (token >= p.tokens) return;
+  const T* row = static_cast<const T*>(p.logits) + token * p.experts;
+  float l[VALUES];
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) l[j] = j * 32 + lane < p.experts ? to_float(row[j * 32 + lane]) : -INFINITY;
+  const bool sigmoid = p.sigmoid != 0;
+  const RowScale r = row_scale(l, sigmoid);
+  int mine = lane < p.top_k ? p.indices[token * p.top_k + lane] : -1;
+  if (mine >= p.experts) mine = -1;
+  const float q = mine >= 0 ? score_of(to_float(row[mine]), r, sigmoid) : 0.0f;
+  float g = mine >= 0 ? p.grad_weights[token * p.top_k + lane] * p.scale : 0.0f;
+  if (p.renormalise) {
+    const float total = warp_sum(q), dot = warp_sum(g * q);
+    g = mine >= 0 && total != 0.0f ? (g - dot / total) / total : 0.0f;
+  }
+  const float through = sigmoid || p.renormalise ? 0.0f : warp_sum(g * q);
+  float ds[VALUES];
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) ds[j] = 0.0f;
+  for (int i = 0; i < p.top_k; ++i) {
+    const int id = __shfl_sync(ALL, mine, i);
+    const float add = __shfl_sync(ALL, g, i);
+    if (id >= 0 && (id & 31) == lane) {
+#pragma unroll
+      for (int j = 0; j < VALUES; ++j)
+        if (j == id >> 5) ds[j] += add;
+    }
+  }
+  T* out = static_cast<T*>(p.grad_logits) + token * p.experts;
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) {
+    const int id = j * 32 + lane;
+    if (id < p.experts) {
+      const float s = score_of(l[j], r, sigmoid);
+      out[id] = from_float<T>(sigmoid ? ds[j] * s * (1.0f - s) : s * (ds[j] - through));
+    }
+  }
+}
+
+// -------------------------------------------------------------------- plan
+
+// Rows in order of their expert, in the order of the pairs inside one: a
+// stable counting sort.  A block takes a chunk of pairs and each of its warps a
+// contiguous part, so ranks follow from counts in order: before the chunk
+// (histograms of a first kernel), before the warp's part (counts in shared
+// memory), inside it (lanes with the same expert, match_any).  No atomics
+// decide an order, so the plan is the same every time.
+constexpr int PLAN_WARPS = 16;
+constexpr int PLAN_CHUNK = 4096;  // pairs per block; fewer pairs than this need no histogram
+
+struct PlanParams {
+  const int* indices;
+  int* offsets;    // [experts + 1]
+  int* tokens;     // [pairs] the token of each sorted row
+  int* positions;  // [pairs] the sorted row of each pair, -1 for one that goes nowhere
+  int* histogram;  // [chunks, experts]
+  int pairs, top_k, experts, chunks;
+};
+
+__global__ void __launch_bounds__(PLAN_WARPS * 32) plan_histogram_kernel(const PlanParams p) {
+  extern __shared__ int counts[];
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) counts[e] = 0;
+  __syncthreads();
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int first = blockIdx.x * PLAN_CHUNK, last = min(first + PLAN_CHUNK, p.pairs);
+  for (int i = first + threadIdx.x; i < last; i += blockDim.x) {
+    const int e = p.indices[i];
+    if (e >= 0 && e < p.experts) atomicAdd(&counts[e], 1);  // a count, whatever the order
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.histogram[blockIdx.x * p.experts + e] = counts[e];
+}
+
+__global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams p) {
+  extern __shared__ int shared[];
+  int* const counts = shared;                            // [warps][experts], then the warp's next row
+  int* const base = shared + PLAN_WARPS * p.experts;     // [experts] rows of all chunks, then the chunk's first row
+  int* const ahead = base + p.experts;                   // [experts] rows of earlier chunks
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < PLAN_WARPS * p.experts; i += blockDim.x) counts[i] = 0;
+  __syncthreads();
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int first = blockIdx.x * PLAN_CHUNK, size = min(PLAN_CHUNK, p.pairs - first);
+  const int part = (size + PLAN_WARPS * 32 - 1) / (PLAN_WARPS * 32) * 32;
+  const int begin = first + min(warp * part, size), end = first + min((warp + 1) * part, size);
+  int* const own = counts + warp * p.experts;
+  for (int i = begin + lane; i - lane < end; i += 32) {
+    const int e = i < end ? p.indices[i] : -1;
+    const unsigned same = __match_any_sync(ALL, e);
+    if (e >= 0 && e < p.experts && lane == __ffs(same) - 1) own[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
+    int run = 0;
+#pragma unroll
+    for (int w = 0; w < PLAN_WARPS; ++w) {
+      const int c = counts[w * p.experts + e];
+      counts[w * p.experts + e] = run;
+      run += c;
+    }
+    int before = 0, total = run;
+    if (p.chunks > 1) {
+      total = 0;
+#pragma unroll 8
+      for (int c = 0; c < p.chunks; ++c) {
+        const int n = p.histogram[c * p.experts + e];
+        if (c < int(blockIdx.x)) before += n;
+        total += n;
+      }
+    }
+    base[e] = total;
+    ahead[e] = before;
+  }
+  __syncthreads();
+  if (warp == 0) {  // exclusive sums over the experts
+    const int per = (p.experts + 31) / 32, e0 = min(lane * per, p.experts), e1 = min(e0 + per, p.experts);
+    int sum = 0;
+    for (int e = e0; e < e1; ++e) sum += base[e];
+    int run = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(ALL, run, d);
+      if (lane >= d) run += other;
+    }
+    run -= sum;
+    for (int e = e0; e < e1; ++e) {
+      const int n = base[e];
+      if (blockIdx.x == 0) p.offsets[e] = run;
+      base[e] = run + ahead[e];
+      run += n;
+    }
+    if (blockIdx.x == 0 && lane == 31) p.offsets[p.experts] = run;
+  }
+  __syncthreads();
+  for (int i = begin + lane; i - lane < end; i += 32) {
+    const int e = i < end ? p.indices[i] : -1;
+    const unsigned same = __match_any_sync(ALL, e);
+    const bool goes = e >= 0 && e < p.experts;
+    const int row = goes ? base[e] + own[e] + __popc(same & ((1u << lane) - 1)) : -1;
+    __syncwarp();
+    if (goes && lane == __ffs(same) - 1) own[e] += __popc(same);
+    __syncwarp();
+    if (i < end) {
+      p.positions[i] = row;
+      if (goes) p.tokens[row] = i / p.top_k;
+    }
+  }
+}
+
+// ----------------------------------------------------------------- combine
+
+struct CombineParams {
+  const void* y;          // [rows, n]
+  const float* weights;   // [tokens, top_k], or null for ones
+  const int* positions;   // [tokens, top_k]
+  const void* residual;   // [tokens, n], or null
+  void* out;              // [tokens, n]; gradient: grad_y [rows, n]
+  const void* grad;       // gradient: of out
+  float* grad_weights;    // gradient: [tokens, top_k]
+  long long tokens;
+  int n, top_k;
+};
+
+constexpr int COMBINE_THREADS = 128;
+
+// out[t] = residual[t] + sum over j of weights[t, j] * y[positions[t, j]], added
+// in the order of j in float32.  A thread takes eight columns (one when rows
+// are not multiples of 16 bytes); its top_k loads do not depend on one another.
+// Y: type of the rows (float32 where a gradient's parts must not be rounded
+// before they are added).
+template <typename T, typename Y, bool VECTOR>
+__global__ void __launch_bounds__(COMBINE_THREADS) combine_kernel(const CombineParams p) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  constexpr int WIDE = VECTOR ? 8 : 1;
+  const long long token = blockIdx.x;
+  const int col = (blockIdx.y * COMBINE_THREADS + threadIdx.x) * WIDE;
+  if (col >= p.n) return;
+  const Y* y = static_cast<const Y*>(p.y);
+  const T* residual = static_cast<const T*>(p.residual);
+  float sum[WIDE];
+#pragma unroll
+  for (int i = 0; i < WIDE; ++i) sum[i] = 0.0f;
+#pragma unroll 4
+  for (int j = 0; j < p.top_k; ++j) {
+    const int row = p.positions[token * p.top_k + j];
+    if (row < 0) continue;
+    const float w = p.weights ? p.weights[token * p.top_k + j] : 1.0f;
+    float v[WIDE];
+    if constexpr (VECTOR) load8(y + (long long)row * p.n + col, v);
+    else v[0] = to_float(y[(long long)row * p.n + col]);
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) sum[i] = fmaf(w, v[i], sum[i]);
+  }
+  if (residual) {
+    float v[WIDE];
+    if constexpr (VECTOR) load8(residual + token * p.n + col, v);
+    else v[0] = to_float(residual[token * p.n + col]);
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) sum[i] += v[i];
+  }
+  T* out = static_cast<T*>(p.out) + token * p.n + col;
+  if constexpr (VECTOR) store8(out, sum);
+  else *out = from_float<T>(sum[0]);
+}
+
+// grad_y[positions[t, j]] = weights[t, j] * grad[t] and grad_weights[t, j] =
+// <grad[t], y[positions[t, j]]>: one block per pair, its threads' parts of the
+// product added in a fixed order.
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(COMBINE_THREADS) combine_gradient_kernel(const CombineParams p) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  constexpr int WIDE = VECTOR ? 8 : 1;
+  const long long pair = blockIdx.x;
+  const int row = p.positions[pair];
+  if (row < 0) {
+    if (threadIdx.x == 0) p.grad_weights[pair] = 0.0f;
+    return;
+  }
+  const T* grad = static_cast<const T*>(p.grad) + pair / p.top_k * p.n;
+  const T* y = static_cast<const T*>(p.y) + (long long)row * p.n;
+  T* out = static_cast<T*>(p.out) + (long long)row * p.n;
+  const float w = p.weights[pair];
+  float dot = 0.0f;
+  for (int col = threadIdx.x * WIDE; col < p.n; col += COMBINE_THREADS * WIDE) {
+    float g[WIDE], v[WIDE];
+    if constexpr (VECTOR) load8(grad + col, g), load8(y + col, v);
+    else g[0] = to_float(grad[col]), v[0] = to_float(y[col]);
+#pragma unroll
+    for (int i = 0; i < WIDE; ++i) {
+      dot = fmaf(g[i], v[i], dot);
+      g[i] *= w;
+    }
+    if constexpr (VECTOR) store8(out + col, g);
+    else out[col] = from_float<T>(g[0]);
+  }
+  __shared__ float parts[COMBINE_THREADS / 32];
+  dot = warp_sum(dot);
+  if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = dot;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < COMBINE_THREADS / 32; ++i) total += parts[i];
+    p.grad_weights[pair] = total;
+  }
+}
+
+// ---------------------------------------------------- gradient of activation
+
+struct ActGradientParams {
+  const void* grad;   // [rows, width]
+  const void* z;      // [rows, n], or null without an activation
+  void* dz;           // [rows, n], or null when it is grad itself
+  float* partial;     // [row blocks, n] column sums, or null
+  const int* limit;   // rows to work on (device), or null for all
+  long long rows;
+  int n, width, shape, glu;
+  float a, b;
+};
+
+constexpr int GRADIENT_ROWS = 64;  // rows a block works on: 8 row lanes of 8 rows
+
+// dz = grad * act'(z), eight columns a thread; a gated pair writes both halves,
+// gate: grad * up * act'(gate), up: grad * act(gate).  Column sums (of the
+// unrounded values) are added per thread down its rows, across the block's row
+// lanes in a fixed order, and across blocks by column_sum_kernel.
+template <typename T>
+__global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientParams p) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const long long rows = p.limit ? *p.limit : p.rows;
+  const long long first = (long long)blockIdx.x * GRADIENT_ROWS;
+  if (first >= rows) return;
+  const int lane = threadIdx.x & 31, row_lane = threadIdx.x >> 5;
+  const int col = (blockIdx.y * 32 + lane) * 8;
+  const bool live = col < p.width;
+  const T* grad = static_cast<const T*>(p.grad);
+  const T* z = static_cast<const T*>(p.z);
+  T* dz = static_cast<T*>(p.dz);
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto slopes = [&](const float* x, float* value, float* slope) {
+    if (p.shape == SHAPE_SIGMOID) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) act_both<SHAPE_SIGMOID>(x[i], p.a, p.b, value + i, slope + i);
+    } else if (p.shape == SHAPE_PHI) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) act_both<SHAPE_PHI>(x[i], 0.f, 0.f, value + i, slope + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) act_both<SHAPE_RELU>(x[i], 0.f, 0.f, value + i, slope + i);
+    }
+  };
+#pragma unroll 2
+  for (int r = row_lane; r < GRADIENT_ROWS; r += 8) {
+    const long long row = first + r;
+    if (!live || row >= rows) break;
+    float g[8], x[8], value[8], slope[8];
+    load8(grad + row * p.width + col, g);
+    if (p.glu) {
+      float up[8];
+      load8(z + row * p.n + col, x);
+      load8(z + row * p.n + p.width + col, up);
+      slopes(x, value, slope);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        slope[i] *= g[i] * up[i];
+        value[i] *= g[i];
+      }
+      store8(dz + row * p.n + col, slope);
+      store8(dz + row * p.n + p.width + col, value);
+      continue;
+    }
+    if (z) {
+      load8(z + row * p.n + col, x);
+      slopes(x, value, slope);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) g[i] *= slope[i];
+      store8(dz + row * p.n + col, g);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += g[i];
+  }
+  if (!p.partial) return;
+  __shared__ float parts[8][256];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) parts[row_lane][i * 32 + lane] = sum[i];
+  __syncthreads();
+  float total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total += parts[i][threadIdx.x];
+  const int at = blockIdx.y * 256 + (threadIdx.x & 31) * 8 + (threadIdx.x >> 5);
+  if (at < p.n) p.partial[(long long)blockIdx.x * p.n + at] = total;
+}
+
+__global__ void __launch_bounds__(128) column_sum_kernel(const float* partial, float* out, int blocks, int n) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int col = blockIdx.x * 128 + threadIdx.x;
+  if (col >= n) return;
+  float sum = 0.0f;
+#pragma unroll 8
+  for (int b = 0; b < blocks; ++b) sum += partial[(long long)b * n + col];
+  out[col] = sum;
+}
+
+// -------------------------------------------------------------------- host
+
+thread_local char routing_error[256];
+
+int routing_fail(const char* format, ...) {
+  va_list args;
+  va_start(args, format);
+  vsnprintf(routing_error, sizeof routing_error, format, args);
+  va_end(args);
+  return OG_ERR_LAUNCH;
+}
+
+int use_device(int device) {
+  int current = -1;
+  if (cudaGetDevice(&current) != cudaSuccess) return routing_fail("cudaGetDevice failed");
+  if (current != device && cudaSetDevice(device) != cudaSuccess) return routing_fail("cudaSetDevice(%d) failed", device);
+  return OG_OK;
+}
+
+template <typename... Args>
+int dependent_launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, void* stream, Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads, 1, 1);
+  config.dynamicSmemBytes = smem;
+  config.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, args...);
+  if (launched != cudaSuccess) return routing_fail("kernel launch failed: %s", cudaGetErrorString(launched));
+  return OG_OK;
+}
+
+enum ElementType : int { TYPE_F32 = 0, TYPE_BF16 = 1, TYPE_F16 = 2 };
+
+template <template <int, typename> class Picker, typename T>
+auto pick_values(int experts) {
+  const int values = (experts + 31) / 32;
+  return values <= 1 ? Picker<1, T>::kernel : values <= 2 ? Picker<2, T>::kernel : values <= 4 ? Picker<4, T>::kernel
+         : values <= 8 ? Picker<8, T>::kernel : values <= 16 ? Picker<16, T>::kernel : Picker<32, T>::kernel;
+}
+template <int VALUES, typename T> struct RouteForward { static constexpr void (*kernel)(RouteParams) = route_kernel<VALUES, T>; };
+template <int VALUES, typename T> struct RouteGradient { static constexpr void (*kernel)(RouteParams) = route_gradient_kernel<VALUES, T>; };
+
+int check_route(const OgRoute& r) {
+  if (r.dtype < TYPE_F32 || r.dtype > TYPE_F16) return routing_fail("dtype %d is none of 0 (float32), 1 (bfloat16), 2 (float16)", r.dtype);
+  if (r.experts < 1 || r.experts > 1024) return routing_fail("%d experts: 1 to 1024 are served", r.experts);
+  if (r.top_k < 1 || r.top_k > 32 || r.top_k > r.experts) return routing_fail("top_k = %d: 1 to 32 of the %d experts", r.top_k, r.experts);
+  if (r.tokens < 0 || r.tokens > 0x7FFFFFFFll * ROUTE_WARPS) return routing_fail("tokens = %lld", (long long)r.tokens);
+  return OG_OK;
+}
+
+}  // namespace
+}  // namespace og
+
+using namespace og;
+
+extern "C" {
+
+OG_API const char* og_b200_routing_error(void) { return routing_error; }
+
+OG_API int32_t og_b200_route(const OgRoute* route, const void* logits, const float* bias, float* weights, int32_t* indices,
+                             int32_t device, void* stream) {
+  if (!route) return routing_fail("null OgRoute");
+  const OgRoute& r = *route;
+  if (const int bad = check_route(r)) return bad;
+  if (r.groups < 1 || r.groups > 32 || r.experts % r.groups) return routing_fail("%d groups: 1 to 32 that divide the %d experts", r.groups, r.experts);
+  if (r.top_groups < 1 || r.top_groups > r.groups) return routing_fail("top_groups = %d of %d groups", r.top_groups, r.groups);
+  if (r.group_top != 1 && r.group_top != 2) return routing_fail("group_top = %d: 1 or 2", r.group_top);
+  if (r.top_k > r.top_groups * (r.experts / r.groups)) return routing_fail("top_k = %d is more than the %d experts of the open groups", r.top_k, r.top_groups * (r.experts / r.groups));
+  if (!r.tokens) return OG_OK;
+  if (!logits || !weights || !indices) return routing_fail("logits, weights and indices must be device pointers, got null");
+  if (const int bad = use_device(device)) return bad;
+  RouteParams p{};
+  p.logits = logits, p.bias = bias, p.weights = weights, p.indices = indices, p.tokens = r.tokens, p.experts = r.experts;
+  p.top_k = r.top_k, p.sigmoid = r.sigmoid, p.groups = r.groups, p.each = r.experts / r.groups, p.top_groups = r.top_groups;
+  p.group_top = r.group_top, p.renormalise = r.renormalise, p.scale = r.scale;
+  const auto kernel = r.dtype == TYPE_F32    ? pick_values<RouteForward, float>(r.experts)
+                      : r.dtype == TYPE_BF16 ? pick_values<RouteForward, __nv_bfloat16>(r.experts)
+                                             : pick_values<RouteForward, __half>(r.experts);
+  return dependent_launch(kernel, dim3(unsigned((r.tokens + ROUTE_WARPS - 1) / ROUTE_WARPS)), ROUTE_WARPS * 32, 0, stream, p);
+}
+
+OG_API int32_t og_b200_route_gradient(const OgRoute* route, const float* grad_weights, const void* logits, const int32_t* indices,
+                                      void* grad_logits, int32_t device, void* stream) {
+  if (!route) return routing_fail("null OgRoute");
+  const OgRoute& r = *route;
+  if (const int bad = check_route(r)) return bad;
+  if (!r.tokens) return OG_OK;
+  if (!grad_weights || !logits || !indices || !grad_logits) return routing_fail("gradients, logits and indices must be device pointers, got null");
+  if (const int bad = use_device(device)) return bad;
+  RouteParams p{};
+  p.logits = logits, p.grad_weights = grad_weights, p.indices = const_cast<int32_t*>(indices), p.grad_logits = grad_logits;
+  p.tokens = r.tokens, p.experts = r.experts, p.top_k = r.top_k, p.sigmoid = r.sigmoid, p.renormalise = r.renormalise, p.scale = r.scale;
+  const auto kernel = r.dtype == TYPE_F32    ? pick_values<RouteGradient, float>(r.experts)
+                      : r.dtype == TYPE_BF16 ? pick_values<RouteGradient, __nv_bfloat16>(r.experts)
+                                             : pick_values<RouteGradient, __half>(r.experts);
+  return dependent_launch(kernel, dim3(unsigned((r.tokens + ROUTE_WARPS - 1) / ROUTE_WARPS)), ROUTE_WARPS * 32, 0, stream, p);
+}
+
+OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32_t top_k, int32_t experts, int32_t* offsets,
+                                   int32_t* token_of_row, int32_t* positions, int32_t* workspace, int32_t device, void* stream) {
+  if (experts < 1 || experts > 1024) return routing_fail("%d experts: 1 to 1024 are served", experts);
+  if (top_k < 1 || tokens < 0 || tokens * top_k >= 0x7FFFFFFFll) return routing_fail("%lld tokens with %d experts each are too many", (long long)tokens, top_k);
+  if (!offsets || (tokens && (!indices || !token_of_row || !positions))) return routing_fail("indices and the plan's arrays must be device pointers, got null");
+  if (const int bad = use_device(device)) return bad;
+  PlanParams p{};
+  p.indices = indices, p.offsets = offsets, p.tokens = token_of_row, p.positions = positions, p.histogram = workspace;
+  p.pairs = int(tokens * top_k), p.top_k = top_k, p.experts = experts;
+  p.chunks = std::max(1, (p.pairs + PLAN_CHUNK - 1) / PLAN_CHUNK);
+  if (p.chunks > 1) {
+    if (!workspace) return routing_fail("%d pairs take a workspace of %lld integers", p.pairs, (long long)p.chunks * experts);
+    if (const int bad = dependent_launch(plan_histogram_kernel, dim3(p.chunks), PLAN_WARPS * 32, experts * sizeof(int), stream, p)) return bad;
+  }
+  const size_t smem = size_t(PLAN_WARPS + 2) * experts * sizeof(int);
+  if (smem > 48 * 1024) {
+    const cudaError_t status = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (PLAN_WARPS + 2) * 1024 * int(sizeof(int)));
+    if (status != cudaSuccess) return routing_fail("cudaFuncSetAttribute: %s", cudaGetErrorString(status));
+  }
+  return dependent_launch(plan_kernel, dim3(p.chunks), PLAN_WARPS * 32, smem, stream, p);
+}
+
+static bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
+
+OG_API int32_t og_b200_expert_combine(int32_t dtype, int32_t y_is_f32, const void* y, const float* weights, const int32_t* positions, const void* residual,
+                                      void* out, int64_t tokens, int32_t top_k, int32_t n, int32_t device, void* stream) {
+  if (dtype != TYPE_BF16 && dtype != TYPE_F16) return routing_fail("dtype %d is none of 1 (bfloat16), 2 (float16)", dtype);
+  if (tokens < 0 || tokens > 0x7FFFFFFFll || top_k < 1 || n < 1) return routing_fail("tokens = %lld, top_k = %d, n = %d", (long long)tokens, top_k, n);
+  if (!tokens) return OG_OK;
+  if (!positions || !out) return routing_fail("positions and out must be device pointers, got null");
+  if (const int bad = use_device(device)) return bad;
+  CombineParams p{};
+  p.y = y, p.weights = weights, p.positions = positions, p.residual = residual, p.out = out, p.tokens = tokens, p.n = n, p.top_k = top_k;
+  const bool wide = n % 8 == 0 && aligned16(y) && aligned16(residual) && aligned16(out);
+  const int columns = COMBINE_THREADS * (wide ? 8 : 1);
+  if ((n + columns - 1) / columns > 65535) return routing_fail("n = %d is too wide", n);
+  const dim3 grid(unsigned(tokens), unsigned((n + columns - 1) / columns));
+#define OG_COMBINE(T) (y_is_f32 ? (wide ? combine_kernel<T, float, true> : combine_kernel<T, float, false>) \
+                                : (wide ? combine_kernel<T, T, true> : combine_kernel<T, T, false>))
+  const auto kernel = dtype == TYPE_BF16 ? OG_COMBINE(__nv_bfloat16) : OG_COMBINE(__half);
+#undef OG_COMBINE
+  return dependent_launch(kernel, grid, COMBINE_THREADS, 0, stream, p);
+}
+
+OG_API int32_t og_b200_expert_combine_gradient(int32_t dtype, const void* grad, const void* y, const float* weights, const int32_t* positions,
+                                               void* grad_y, float* grad_weights, int64_t tokens, int32_t top_k, int32_t n, int32_t device,
+                                               void* stream) {
+  if (dtype != TYPE_BF16 && dtype != TYPE_F16) return routing_fail("dtype %d is none of 1 (bfloat16), 2 (float16)", dtype);
+  if (tokens < 0 || top_k < 1 || n < 1 || tokens * top_k > 0x7FFFFFFFll) return routing_fail("tokens = %lld, top_k = %d, n = %d", (long long)tokens, top_k, n);
+  if (!tokens) return OG_OK;
+  if (!grad || !weights || !positions || !grad_weights) return routing_fail("the gradient's tensors must be device pointers, got null");
+  if (const int bad = use_device(device)) return bad;
+  CombineParams p{};
+  p.y = y, p.weights = weights, p.positions = positions, p.grad = grad, p.out = grad_y, p.grad_weights = grad_weights;
+  p.tokens = tokens, p.n = n, p.top_k = top_k;
+  const bool wide = n % 8 == 0 && aligned16(y) && aligned16(grad) && aligned16(grad_y);
+  const auto kernel = dtype == TYPE_BF16 ? (wide ? combine_gradient_kernel<__nv_bfloat16, true> : combine_gradient_kernel<__nv_bfloat16, false>)
+                                         : (wide ? combine_gradient_kernel<__half, true> : combine_gradient_kernel<__half, false>);
+  return dependent_launch(kernel, dim3(unsigned(tokens * top_k)), COMBINE_THREADS, 0, stream, p);
+}
+
+OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, const void* grad, const void* z, void* dz, float* bias_gradient,
+                                           float* workspace, const int32_t* row_limit, int64_t rows, int32_t n, int32_t device, void* stream) {
+  if (dtype != TYPE_BF16 && dtype != TYPE_F16) return routing_fail("dtype %d is none of 1 (bfloat16), 2 (float16)", dtype);
+  if (activation < ACT_NONE || activation > ACT_GEGLU) return routing_fail("activation %d is none of 0..%d", activation, int(ACT_GEGLU));
+  const bool glu = activation == ACT_SWIGLU || activation == ACT_GEGLU;
+  if (rows < 0 || n < 1 || n % (glu ? 16 : 8)) return routing_fail("rows = %lld, n = %d: columns come in eights", (long long)rows, n);
+  if (glu && bias_gradient) return routing_fail("a gated activation has no bias gradient here");
+  if ((rows + GRADIENT_ROWS - 1) / GRADIENT_ROWS > 0x7FFFFFFFll) return routing_fail("rows = %lld are too many", (long long)rows);
+  if (const int bad = use_device(device)) return bad;
+  const int blocks = int((rows + GRADIENT_ROWS - 1) / GRADIENT_ROWS);
+  if (rows) {
+    if (!grad || (activation && (!z || !dz)) || (bias_gradient && !workspace)) return routing_fail("the gradient's tensors must be device pointers, got null");
+    if (!aligned16(grad) || !aligned16(z) || !aligned16(dz)) return routing_fail("gradients and pre-activations must start on 16-byte boundaries");
+    ActGradientParams p{};
+    p.grad = grad, p.z = activation ? z : nullptr, p.dz = dz, p.partial = bias_gradient ? workspace : nullptr, p.limit = row_limit;
+    p.rows = rows, p.n = n, p.width = glu ? n / 2 : n, p.glu = glu;
+    act_constants(activation, &p.shape, &p.a, &p.b);
+    if (!activation && !bias_gradient) return OG_OK;
+    const dim3 grid(unsigned(blocks), unsigned((p.width + 255) / 256));
+    if (grid.y > 65535) return routing_fail("n = %d is too wide", n);
+    const auto kernel = dtype == TYPE_BF16 ? act_gradient_kernel<__nv_bfloat16> : act_gradient_kernel<__half>;
+    if (const int bad = dependent_launch(kernel, grid, 256, 0, stream, p)) return bad;
+  }
+  if (!bias_gradient) return OG_OK;
+  return dependent_launch(column_sum_kernel, dim3(unsigned((n + 127) / 128)), 128, 0, stream, (const float*)workspace, bias_gradient, blocks, int(n));
+}
+
+}  // extern "C"
