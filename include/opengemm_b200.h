@@ -292,15 +292,15 @@ OG_API int32_t og_b200_launch_no_alloc(const OgGemm* g, const void* a, const voi
  *   mode 1  out[r] = x[r] . w_e                            x [rows, n], w [groups, n, k], out [rows, k]
  *   mode 2  out[e] = sum over e's rows of x[r]^T w[r]      x [rows, n], w [rows, k],      out [groups, n, k]
  * Group e has the rows offsets[e] .. offsets[e + 1]; rows of `out` past the last group are
- * left as they were.  With `tokens` row r of mode 0's x (mode 2's w) is row tokens[r] of a
- * [x_rows, k] tensor.  dtype "bf16" or "f16", for mode 0 also "e4m3" (written as bfloat16).
+ * left as they were.  With `tokens` row r of mode 0's x is row tokens[r] of a [x_rows, k]
+ * tensor.  dtype "bf16" or "f16", for mode 0 also "e4m3" (written as bfloat16).
  * Rows of all operands are multiples of 16 bytes and start on such boundaries.  A single
  * group needs no table: offsets may be null.  Errors: og_b200_experts_error(). */
 typedef struct OgExpertProduct {
   const void* x;
   const void* w;
   const int32_t* offsets; /* device, [groups + 1], or null */
-  const int32_t* tokens;  /* device, [rows], or null */
+  const int32_t* tokens;  /* device, [rows], or null; mode 0 */
   const float* alpha;     /* device, [groups], or null; mode 0 */
   void* out;
   void* preactivation;    /* mode 0: [rows, n], the activation's argument, or null */
@@ -334,11 +334,16 @@ OG_API int32_t og_b200_route_gradient(const OgRoute* route, const float* grad_we
 /* Order of the rows by expert, in the order of the (token, choice) pairs inside one.
  * offsets [experts + 1]: first row of each expert; token_of_row [tokens * top_k]; positions
  * [tokens, top_k]: the row of each pair, -1 where the index is outside 0 .. experts - 1
- * (then rows past offsets[experts] do not exist).  workspace: ceil(tokens * top_k / 4096) *
- * experts integers (null up to 4096 pairs). */
+ * (then rows past offsets[experts] do not exist).  workspace: ceil(tokens * top_k / 8192) *
+ * experts integers (null up to 8192 pairs). */
 OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32_t top_k, int32_t experts,
                                    int32_t* offsets, int32_t* token_of_row, int32_t* positions,
                                    int32_t* workspace, int32_t device, void* stream);
+
+/* out[r] = x[token_of_row[r]] for the rows r < min(rows, *row_limit); rows of row_bytes, a
+ * multiple of 16, on 16-byte boundaries. */
+OG_API int32_t og_b200_expert_gather(const void* x, const int32_t* token_of_row, const int32_t* row_limit, void* out,
+                                     int64_t row_bytes, int32_t rows, int32_t device, void* stream);
 
 /* out[t] = residual[t] + sum over j of weights[t, j] * y[positions[t, j]] in float32, in the
  * order of j; weights null: ones; residual null: zero.  y [rows, n] of `dtype`, or float32

@@ -204,6 +204,7 @@ class Library:
                 "route": [POINTER(OgRoute)] + [c_void_p] * 4 + [c_int32, c_void_p],
                 "route_gradient": [POINTER(OgRoute)] + [c_void_p] * 4 + [c_int32, c_void_p],
                 "expert_plan": [c_void_p, ctypes.c_int64, c_int32, c_int32] + [c_void_p] * 4 + [c_int32, c_void_p],
+                "expert_gather": [c_void_p] * 4 + [ctypes.c_int64, c_int32, c_int32, c_void_p],
                 "expert_combine": [c_int32, c_int32] + [c_void_p] * 5 + [ctypes.c_int64, c_int32, c_int32, c_int32, c_void_p],
                 "expert_combine_gradient": [c_int32] + [c_void_p] * 6 + [ctypes.c_int64, c_int32, c_int32, c_int32, c_void_p],
                 "activation_gradient": [c_int32, c_int32] + [c_void_p] * 6 + [ctypes.c_int64, c_int32, c_int32, c_void_p],
@@ -380,6 +381,13 @@ class Library:
         if self._expert_plan(indices.data_ptr(), indices.size(0), indices.size(1), experts, offsets.data_ptr(),
                              tokens.data_ptr(), positions.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
                              device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._routing_error().decode())
+
+    def expert_gather(self, x, tokens, row_limit, out):
+        """out[r] = x[tokens[r]] for the rows below the device integer at address `row_limit`."""
+        device = out.get_device()
+        if self._expert_gather(x.data_ptr(), tokens.data_ptr(), row_limit, out.data_ptr(), x.size(1) * x.element_size(),
+                               out.size(0), device, raw_stream(device)) != OG_OK:
             raise RuntimeError(self._routing_error().decode())
 
     def expert_combine(self, y, weights, positions, residual, out):

@@ -120,7 +120,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
   if (glu && g.n % 16) return experts_fail(OG_ERR_LAUNCH, "a gated activation takes a multiple of 16 weight rows, got %d", g.n);
   if (g.out_f32 && mode == MODE_FORWARD) return experts_fail(OG_ERR_LAUNCH, "the forward product writes 16-bit values");
   const bool gather = g.tokens != nullptr;
-  if (gather && mode == MODE_DX) return experts_fail(OG_ERR_LAUNCH, "the rows' gradient gathers nothing");
+  if (gather && mode != MODE_FORWARD) return experts_fail(OG_ERR_LAUNCH, "only the forward product gathers its rows");
   if (device < 0 || device >= XP_DEVICES) return experts_fail(OG_ERR_LAUNCH, "device %d is out of range: this library serves devices 0..%d", device, XP_DEVICES - 1);
   int current = -1;
   if (cudaGetDevice(&current) != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaGetDevice failed");
@@ -185,7 +185,6 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
   if (mode == MODE_DW) {  // dz [rows, n] against x [rows, k], both along their rows
     map(&p.map_x, g.x, n, uint64_t(g.rows), 64, "the output's gradient");
     map(&p.map_y, g.w, k, x_rows, 64, "the rows");
-    if (gather) map(&p.map_x32, g.w, k, x_rows, 1, "the gathered rows");
   } else {
     const uint64_t inner = mode == MODE_FORWARD ? k : n;
     map(&p.map_x, g.x, inner, x_rows, 128, "the rows");

@@ -41,7 +41,7 @@ __host__ __device__ constexpr int xp_threads(int mode) { return mode == MODE_DW 
 
 struct alignas(64) ExpertParams {
   CUtensorMap map_x;    // MMA-M side, boxes of 128 rows (64 x 64 in MODE_DW)
-  CUtensorMap map_x32;  // the same in boxes of 32 rows, for a group's last, short tile; gathered: one row
+  CUtensorMap map_x32;  // the same in boxes of 32 rows, for a group's last, short tile; gathered: of one row
   CUtensorMap map_y;    // MMA-N side
   const int* offsets;   // [groups + 1] first row of each group; null: one group of all rows
   const int* tokens;    // gathered operand: its row for each sorted row
@@ -110,6 +110,7 @@ __device__ __forceinline__ uint64_t column_operand_desc(uint32_t smem_addr) {
   return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(8192 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// GATHER and GLU: MODE_FORWARD only.
 template <int KIND, int CTA_GROUP, int MODE, bool GATHER, bool GLU, int OUT_BYTES>
 __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __grid_constant__ ExpertParams p) {
   constexpr int TILE_M = 128 * CTA_GROUP;
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
   if (threadIdx.x == 0) {
     prefetch_tmap(&p.map_x);
     prefetch_tmap(&p.map_y);
-    if (MODE == MODE_FORWARD || GATHER) prefetch_tmap(&p.map_x32);
+    if (MODE == MODE_FORWARD) prefetch_tmap(&p.map_x32);
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
@@ -250,18 +251,11 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
         }
         const uint32_t tx = uint32_t(whole) * 128 + CTA_GROUP * y_bytes;
         int token[4];
-        if constexpr (GATHER && MODE == MODE_FORWARD) {
+        if constexpr (GATHER) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)  // rows past the group's end repeat its last row
             token[i] = 4 * lane < mine ? p.tokens[min(x_row + 4 * lane + i, w.first_row + w.rows - 1)] : 0;
         }
-        auto tokens_of = [&](int kb) {
-          if constexpr (GATHER && MODE == MODE_DW) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) token[i] = p.tokens[w.first_row + min(kb * 64 + 4 * (lane & 15) + i, w.rows - 1)];
-          }
-        };
-        if (blocks > 0) tokens_of(0);
         for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(bar_empty + 8 * stage, phase ^ 1, ctx, SITE_PRODUCER_EMPTY)) {
             ok = false;
@@ -291,10 +285,8 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
               const int r = w.first_row + kb * 64, m0 = w.mi * TILE_M + int(rank) * 128;
               tma_load_2d<CTA_GROUP>(sx, &p.map_x, m0, r, full);
               tma_load_2d<CTA_GROUP>(sx + 8192, &p.map_x, m0 + 64, r, full);
-              if constexpr (!GATHER) {
-                const int c0 = w.ni * tile_n + int(rank) * y_rows;
-                for (int b = 0; b < y_boxes; ++b) tma_load_2d<CTA_GROUP>(sy + b * 8192, &p.map_y, c0 + 64 * b, r, full);
-              }
+              const int c0 = w.ni * tile_n + int(rank) * y_rows;
+              for (int b = 0; b < y_boxes; ++b) tma_load_2d<CTA_GROUP>(sy + b * 8192, &p.map_y, c0 + 64 * b, r, full);
             }
             if constexpr (MODE != MODE_DW && !GATHER) {
               if (mine == 128) tma_load_2d<CTA_GROUP>(sx, &p.map_x, kb * block_k, x_row, full);
@@ -302,15 +294,9 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
                 for (int r = 0; r < mine; r += 32) tma_load_2d<CTA_GROUP>(sx + r * 128, &p.map_x32, kb * block_k, x_row + r, full);
             }
           }
-          if constexpr (GATHER && MODE == MODE_FORWARD) {
+          if constexpr (GATHER) {
             if (4 * lane < mine)
               tma_gather4<CTA_GROUP>(sx + lane * 512, &p.map_x32, kb * block_k, token[0], token[1], token[2], token[3], full);
-          }
-          if constexpr (GATHER && MODE == MODE_DW) {
-            const int c0 = w.ni * tile_n + int(rank) * y_rows;
-            for (int b = lane >> 4; b < y_boxes; b += 2)
-              tma_gather4<CTA_GROUP>(sy + b * 8192 + (lane & 15) * 512, &p.map_x32, c0 + 64 * b, token[0], token[1], token[2], token[3], full);
-            if (kb + 1 < blocks) tokens_of(kb + 1);
           }
           if constexpr (MODE == MODE_DW) {  // a short block is on its way: warp 6 may look for it
             if (leads && rank == 0 && kb == blocks - 1 && (w.rows & 63)) mbar_arrive(bar_go + 8 * stage);

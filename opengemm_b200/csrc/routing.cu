@@ -129,11 +129,46 @@ __device__ __forceinline__ float score_of(float l, const RowScale& r, bool sigmo
 
 constexpr int ROUTE_WARPS = 4;
 
-// One warp per token; lane `lane` holds the experts lane, lane + 32, ...  A
-// choice is one warp-wide maximum of the keys and one minimum of the indices
-// that reach it, and only the winning lane rescans its values: top_k * 2
-// reductions a token.  Without a bias the order of the scores is that of the
+// The VALUES consecutive logits of a lane, -infinity past the last expert; one
+// vector load (or a few) where rows divide into such pieces.
+template <int VALUES, typename T>
+__device__ __forceinline__ void load_logits(const T* row, int lane, int experts, float (&l)[VALUES]) {
+  constexpr int BYTES = VALUES * int(sizeof(T)), WIDE = BYTES < 16 ? BYTES : 16;
+  if (experts % VALUES == 0 && reinterpret_cast<uintptr_t>(row) % WIDE == 0) {
+    alignas(16) T v[VALUES];
+    if (lane * VALUES < experts) {
+      if constexpr (WIDE == 16) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(row + lane * VALUES)[i];
+      } else if constexpr (WIDE == 8) {
+        *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(row + lane * VALUES);
+      } else if constexpr (WIDE == 4) {
+        *reinterpret_cast<uint32_t*>(v) = *reinterpret_cast<const uint32_t*>(row + lane * VALUES);
+      } else {
+        v[0] = row[lane];
+      }
+#pragma unroll
+      for (int j = 0; j < VALUES; ++j) l[j] = to_float(v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VALUES; ++j) l[j] = -INFINITY;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) l[j] = lane * VALUES + j < experts ? to_float(row[lane * VALUES + j]) : -INFINITY;
+}
+
+// One warp per token; lane `lane` holds VALUES consecutive experts, so that the
+// first lane that reaches a maximum also holds the lowest such index, and a
+// choice is one warp-wide maximum, a ballot and a shuffle; only the winning
+// lane rescans its values.  16-bit logits that are compared themselves leave
+// the low bits of their key free: with the (inverted) index in there a choice
+// is the maximum alone.  Without a bias the order of the scores is that of the
 // logits, which no rounding blurs, so those are compared.
+//
+// Bound by instruction issue: 16384 tokens of 128 experts, top 8, move 4 MB
+// but execute some 300 instructions a warp.
 template <int VALUES, typename T>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RouteParams p) {
   pdl_wait_prior_grids();
@@ -142,43 +177,38 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RoutePara
   const long long token = (long long)blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5);
   if (token >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + token * p.experts;
+  const int id0 = lane * VALUES;
   float l[VALUES];
-#pragma unroll
-  for (int j = 0; j < VALUES; ++j) l[j] = j * 32 + lane < p.experts ? to_float(row[j * 32 + lane]) : -INFINITY;
+  load_logits(row, lane, p.experts, l);
   const bool sigmoid = p.sigmoid != 0;
   const RowScale r = row_scale(l, sigmoid);
   uint32_t key[VALUES];
   const bool by_score = p.bias != nullptr || p.groups > 1;
 #pragma unroll
   for (int j = 0; j < VALUES; ++j) {
-    const int id = j * 32 + lane;
     float c = l[j];
-    if (by_score && c != -INFINITY) c = score_of(l[j], r, sigmoid) + (p.bias && id < p.experts ? p.bias[id] : 0.0f);
+    if (by_score && c != -INFINITY) c = score_of(l[j], r, sigmoid) + (p.bias && id0 + j < p.experts ? p.bias[id0 + j] : 0.0f);
     key[j] = score_key(c, l[j] != -INFINITY);
   }
   if (p.groups > 1) {
     uint32_t group_key = 0;  // of group `lane`
     for (int g = 0; g < p.groups; ++g) {
-      const int first = g * p.each, last = first + p.each;
-      uint32_t best = 0;
-      int at = 0x7FFFFFFF;
+      const int first = g * p.each - id0, last = first + p.each;  // in this lane's values
+      uint32_t best = 0, second = 0;
+      if (first < VALUES && last > 0) {
 #pragma unroll
-      for (int j = 0; j < VALUES; ++j) {
-        const int id = j * 32 + lane;
-        if (id >= first && id < last && key[j] > best) best = key[j], at = id;
+        for (int j = 0; j < VALUES; ++j) {
+          const uint32_t k = j >= first && j < last ? key[j] : 0u;
+          second = max(second, min(best, k));
+          best = max(best, k);
+        }
       }
       const uint32_t one = __reduce_max_sync(ALL, best);
       float score = key_score(one);
       if (p.group_top == 2 && one) {
-        const int winner = int(__reduce_min_sync(ALL, unsigned(best == one ? at : 0x7FFFFFFF)));
-        uint32_t second = 0;
-#pragma unroll
-        for (int j = 0; j < VALUES; ++j) {
-          const int id = j * 32 + lane;
-          if (id >= first && id < last && id != winner) second = max(second, key[j]);
-        }
-        second = __reduce_max_sync(ALL, second);
-        if (second) score += key_score(second);
+        const int holder = __ffs(__ballot_sync(ALL, best == one)) - 1;
+        const uint32_t two = __reduce_max_sync(ALL, lane == holder ? second : best);
+        if (two) score += key_score(two);
       }
       if (lane == g) group_key = one ? score_key(score, true) : 0u;
     }
@@ -190,32 +220,40 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RoutePara
       open |= 1u << winner;
       if (lane == winner) group_key = 0;
     }
+    int g = id0 / p.each, left = p.each - (id0 - g * p.each);
 #pragma unroll
     for (int j = 0; j < VALUES; ++j) {
-      const int id = j * 32 + lane;
-      if (id < p.experts && !(open >> (id / p.each) & 1)) key[j] = 0;
+      if (left == 0) ++g, left = p.each;
+      --left;
+      if (g >= p.groups || !(open >> g & 1)) key[j] = 0;
       if (!p.bias && key[j]) key[j] = score_key(l[j], true);  // inside the open groups the logits decide
     }
   }
-  uint32_t best = 0;
-  int at = 0x7FFFFFFF;
-  auto rescan = [&] {
-    best = 0, at = 0x7FFFFFFF;
+  int mine = -1;  // choice number `lane`
+  const bool packed = sizeof(T) == 2 && !p.bias;
+  if (packed) {
+    constexpr uint32_t LOW = 0x3FFu;  // a 16-bit float's key has at least 13 zeros (or, negative, ones) below
 #pragma unroll
-    for (int j = 0; j < VALUES; ++j)
-      if (key[j] > best) best = key[j], at = j * 32 + lane;
+    for (int j = 0; j < VALUES; ++j) key[j] = key[j] ? (key[j] & ~LOW) | (LOW - uint32_t(id0 + j)) : 0u;
+  }
+  uint32_t best = 0;
+  int at = 0;
+  auto rescan = [&] {
+    best = key[0], at = id0;
+#pragma unroll
+    for (int j = 1; j < VALUES; ++j)
+      if (key[j] > best) best = key[j], at = id0 + j;
   };
   rescan();
-  int mine = -1;  // choice number `lane`
   for (int i = 0; i < p.top_k; ++i) {
     const uint32_t top = __reduce_max_sync(ALL, best);
     if (!top) break;
-    const int winner = int(__reduce_min_sync(ALL, unsigned(best == top ? at : 0x7FFFFFFF)));
+    const bool won = packed ? best == top : __ffs(__ballot_sync(ALL, best == top)) - 1 == lane;
+    const int winner = packed ? int(0x3FFu - (top & 0x3FFu)) : __shfl_sync(ALL, at, __ffs(__ballot_sync(ALL, won)) - 1);
     if (lane == i) mine = winner;
-    if (at == winner) {
+    if (won) {
 #pragma unroll
-      for (int j = 0; j < VALUES; ++j)
-        if (j * 32 + lane == winner) key[j] = 0;
+      for (int j = 0; j < VALUES; ++j) key[j] = id0 + j == at ? 0u : key[j];
       rescan();
     }
   }
@@ -233,50 +271,70 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RoutePara
 // d weights -> d logits.  q: the chosen scores, S their sum, g' the incoming
 // gradient times the factor:  dq = (g' - sum(g' q) / S) / S when renormalised,
 // else g'.  Softmax: dl = s (ds - sum(ds s)), where the sum vanishes after a
-// renormalisation; logistic: dl = ds s (1 - s).
+// renormalisation; logistic: dl = ds s (1 - s).  The few ds are scattered
+// through shared memory (an index may be there twice).
 template <int VALUES, typename T>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const RouteParams p) {
+  __shared__ float scattered[ROUTE_WARPS][32 * VALUES];
+  float* const ds = scattered[threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31, id0 = lane * VALUES;
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j) ds[j * 32 + lane] = 0.0f;
   pdl_wait_prior_grids();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
   const long long token = (long long)blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5);
   if (token >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + token * p.experts;
-  float l[VALUES];
-#pragma unroll
-  for (int j = 0; j < VALUES; ++j) l[j] = j * 32 + lane < p.experts ? to_float(row[j * 32 + lane]) : -INFINITY;
-  const bool sigmoid = p.sigmoid != 0;
-  const RowScale r = row_scale(l, sigmoid);
   int mine = lane < p.top_k ? p.indices[token * p.top_k + lane] : -1;
   if (mine >= p.experts) mine = -1;
-  const float q = mine >= 0 ? score_of(to_float(row[mine]), r, sigmoid) : 0.0f;
   float g = mine >= 0 ? p.grad_weights[token * p.top_k + lane] * p.scale : 0.0f;
+  const float chosen = mine >= 0 ? to_float(row[mine]) : -INFINITY;
+  float l[VALUES];
+  load_logits(row, lane, p.experts, l);
+  const bool sigmoid = p.sigmoid != 0;
+  const RowScale r = row_scale(l, sigmoid);
+  const float q = score_of(chosen, r, sigmoid);
   if (p.renormalise) {
     const float total = warp_sum(q), dot = warp_sum(g * q);
     g = mine >= 0 && total != 0.0f ? (g - dot / total) / total : 0.0f;
   }
   const float through = sigmoid || p.renormalise ? 0.0f : warp_sum(g * q);
-  float ds[VALUES];
-#pragma unroll
-  for (int j = 0; j < VALUES; ++j) ds[j] = 0.0f;
-  for (int i = 0; i < p.top_k; ++i) {
-    const int id = __shfl_sync(ALL, mine, i);
-    const float add = __shfl_sync(ALL, g, i);
-    if (id >= 0 && (id & 31) == lane) {
-#pragma unroll
-      for (int j = 0; j < VALUES; ++j)
-        if (j == id >> 5) ds[j] += add;
-    }
+  __syncwarp();
+  // One after another where an index is repeated, in the order of the choices.
+  unsigned todo = __ballot_sync(ALL, mine >= 0);
+  const unsigned same = __match_any_sync(ALL, mine);
+  while (todo) {
+    const bool turn = (todo >> lane & 1) && !(same & todo & ((1u << lane) - 1));
+    if (turn) ds[mine] += g;
+    todo &= ~__ballot_sync(ALL, turn);
+    __syncwarp();
   }
   T* out = static_cast<T*>(p.grad_logits) + token * p.experts;
+  alignas(16) T v[VALUES];
 #pragma unroll
   for (int j = 0; j < VALUES; ++j) {
-    const int id = j * 32 + lane;
-    if (id < p.experts) {
-      const float s = score_of(l[j], r, sigmoid);
-      out[id] = from_float<T>(sigmoid ? ds[j] * s * (1.0f - s) : s * (ds[j] - through));
-    }
+    const float s = score_of(l[j], r, sigmoid);
+    v[j] = from_float<T>(sigmoid ? ds[id0 + j] * s * (1.0f - s) : s * (ds[id0 + j] - through));
   }
+  constexpr int BYTES = VALUES * int(sizeof(T)), WIDE = BYTES < 16 ? BYTES : 16;
+  if (p.experts % VALUES == 0 && reinterpret_cast<uintptr_t>(out) % WIDE == 0) {
+    if (id0 < p.experts) {
+      if constexpr (WIDE == 16) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(out + id0)[i] = reinterpret_cast<const uint4*>(v)[i];
+      } else if constexpr (WIDE == 8) {
+        *reinterpret_cast<uint2*>(out + id0) = *reinterpret_cast<const uint2*>(v);
+      } else if constexpr (WIDE == 4) {
+        *reinterpret_cast<uint32_t*>(out + id0) = *reinterpret_cast<const uint32_t*>(v);
+      } else {
+        out[id0] = v[0];
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < VALUES; ++j)
+    if (id0 + j < p.experts) out[id0 + j] = v[j];
 }
 
 // -------------------------------------------------------------------- plan
@@ -287,8 +345,11 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const 
 // (histograms of a first kernel), before the warp's part (counts in shared
 // memory), inside it (lanes with the same expert, match_any).  No atomics
 // decide an order, so the plan is the same every time.
-constexpr int PLAN_WARPS = 16;
-constexpr int PLAN_CHUNK = 4096;  // pairs per block; fewer pairs than this need no histogram
+// A lane reads its PLAN_EACH pairs at once and keeps them: with a load per step
+// the chain of trips to L2 was most of the time (4096 pairs: 6.9 us).
+constexpr int PLAN_WARPS = 32;
+constexpr int PLAN_CHUNK = 8192;  // pairs per block; up to this many need no histogram
+constexpr int PLAN_EACH = PLAN_CHUNK / (PLAN_WARPS * 32);
 
 struct PlanParams {
   const int* indices;
@@ -325,13 +386,23 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams 
   pdl_wait_prior_grids();
   pdl_launch_dependents();
   const int first = blockIdx.x * PLAN_CHUNK, size = min(PLAN_CHUNK, p.pairs - first);
-  const int part = (size + PLAN_WARPS * 32 - 1) / (PLAN_WARPS * 32) * 32;
+  const int part = (size + PLAN_WARPS * 32 - 1) / (PLAN_WARPS * 32) * 32;  // at most PLAN_EACH * 32
   const int begin = first + min(warp * part, size), end = first + min((warp + 1) * part, size);
   int* const own = counts + warp * p.experts;
-  for (int i = begin + lane; i - lane < end; i += 32) {
-    const int e = i < end ? p.indices[i] : -1;
-    const unsigned same = __match_any_sync(ALL, e);
-    if (e >= 0 && e < p.experts && lane == __ffs(same) - 1) own[e] += __popc(same);
+  int expert[PLAN_EACH];
+  unsigned same[PLAN_EACH];
+#pragma unroll
+  for (int s = 0; s < PLAN_EACH; ++s) {
+    const int i = begin + s * 32 + lane;
+    expert[s] = i < end ? p.indices[i] : -1;
+    if (expert[s] >= p.experts || expert[s] < 0) expert[s] = -1;
+  }
+#pragma unroll
+  for (int s = 0; s < PLAN_EACH; ++s) {
+    if (begin + s * 32 >= end) break;
+    const int e = expert[s];
+    same[s] = __match_any_sync(ALL, e);
+    if (e >= 0 && lane == __ffs(same[s]) - 1) own[e] += __popc(same[s]);
     __syncwarp();
   }
   __syncthreads();
@@ -377,19 +448,43 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams 
     if (blockIdx.x == 0 && lane == 31) p.offsets[p.experts] = run;
   }
   __syncthreads();
-  for (int i = begin + lane; i - lane < end; i += 32) {
-    const int e = i < end ? p.indices[i] : -1;
-    const unsigned same = __match_any_sync(ALL, e);
-    const bool goes = e >= 0 && e < p.experts;
-    const int row = goes ? base[e] + own[e] + __popc(same & ((1u << lane) - 1)) : -1;
+#pragma unroll
+  for (int s = 0; s < PLAN_EACH; ++s) {
+    const int i = begin + s * 32 + lane;
+    if (i - lane >= end) break;
+    const int e = expert[s];
+    const int row = e >= 0 ? base[e] + own[e] + __popc(same[s] & ((1u << lane) - 1)) : -1;
     __syncwarp();
-    if (goes && lane == __ffs(same) - 1) own[e] += __popc(same);
+    if (e >= 0 && lane == __ffs(same[s]) - 1) own[e] += __popc(same[s]);
     __syncwarp();
     if (i < end) {
       p.positions[i] = row;
-      if (goes) p.tokens[row] = i / p.top_k;
+      if (e >= 0) p.tokens[row] = i / p.top_k;
     }
   }
+}
+
+// ------------------------------------------------------------------ gather
+
+// out[r] = x[tokens[r]] for the plan's rows, 16 bytes a lane, a warp per row: two
+// passes over the rows (67 MB each for 8192 rows of 4096 bf16 values) against
+// fetching them row by row inside the product, where the copy engine takes some
+// 50 cycles for four rows of 128 bytes and a tile of 128 rows then waits for it
+// (8 experts, 4096 x 4096, 7675 rows: 660 us gathered there, 199 us on sorted rows).
+__global__ void __launch_bounds__(256) gather_kernel(const uint4* x, const int* tokens, const int* limit, uint4* out, int vectors, int rows) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= min(rows, *limit)) return;
+  const uint4* src = x + (long long)tokens[row] * vectors;
+  uint4* dst = out + (long long)row * vectors;
+  int i = lane;
+  for (; i + 96 < vectors; i += 128) {
+    const uint4 a = src[i], b = src[i + 32], c = src[i + 64], d = src[i + 96];
+    dst[i] = a, dst[i + 32] = b, dst[i + 64] = c, dst[i + 96] = d;
+  }
+  for (; i < vectors; i += 32) dst[i] = src[i];
 }
 
 // ----------------------------------------------------------------- combine
@@ -708,7 +803,7 @@ OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32
     if (const int bad = dependent_launch(plan_histogram_kernel, dim3(p.chunks), PLAN_WARPS * 32, experts * sizeof(int), stream, p)) return bad;
   }
   const size_t smem = size_t(PLAN_WARPS + 2) * experts * sizeof(int);
-  if (smem > 48 * 1024) {
+  if (smem > 48 * 1024) {  // up to 136 KiB for 1024 experts
     const cudaError_t status = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (PLAN_WARPS + 2) * 1024 * int(sizeof(int)));
     if (status != cudaSuccess) return routing_fail("cudaFuncSetAttribute: %s", cudaGetErrorString(status));
   }
@@ -716,6 +811,17 @@ OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32
 }
 
 static bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
+
+OG_API int32_t og_b200_expert_gather(const void* x, const int32_t* token_of_row, const int32_t* row_limit, void* out, int64_t row_bytes,
+                                     int32_t rows, int32_t device, void* stream) {
+  if (rows < 0 || row_bytes < 16 || row_bytes % 16 || row_bytes / 16 > 0x7FFFFFFF) return routing_fail("rows of %lld bytes: a multiple of 16", (long long)row_bytes);
+  if (!rows) return OG_OK;
+  if (!x || !token_of_row || !row_limit || !out) return routing_fail("x, the plan and out must be device pointers, got null");
+  if (!aligned16(x) || !aligned16(out)) return routing_fail("rows must start on 16-byte boundaries");
+  if (const int bad = use_device(device)) return bad;
+  return dependent_launch(gather_kernel, dim3(unsigned((rows + 7) / 8)), 256, 0, stream, static_cast<const uint4*>(x), token_of_row, row_limit,
+                          static_cast<uint4*>(out), int(row_bytes / 16), int(rows));
+}
 
 OG_API int32_t og_b200_expert_combine(int32_t dtype, int32_t y_is_f32, const void* y, const float* weights, const int32_t* positions, const void* residual,
                                       void* out, int64_t tokens, int32_t top_k, int32_t n, int32_t device, void* stream) {
