@@ -414,7 +414,7 @@ int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* str
     if (ready != OG_OK) return ready;
   }
   const cudaError_t launched =
-      fixed >= 0 ? fixed_kernel(fixed).launch(params, grid, p.smem_bytes, s, params.pdl != 0)
+      fixed >= 0 ? fixed_kernel(fixed).launch(params, grid, launch_smem_bytes(p, params, fused), s, params.pdl != 0)
                  : launch_variant(p.variant, params, grid, p.smem_bytes, s, params.pdl != 0);
   if (workspace_slot >= 0) release_workspace(device, workspace_slot, s);
   if (launched != cudaSuccess)

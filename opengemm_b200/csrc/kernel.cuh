@@ -35,6 +35,14 @@ namespace og {
 
 constexpr int MAX_STAGES = 16;
 constexpr int THREADS = 192;
+// The fused epilogue has twice the warps: two per quarter of the accumulator's
+// rows, taking turns at its columns.  One warp per scheduler cannot hide the
+// trips to memory and the special functions behind one another (e4m3 4096^3
+// with bias, gelu_tanh and residual: 75 us with four warps).
+__host__ __device__ constexpr int epilogue_warps(bool fused) { return fused ? 8 : 4; }
+__host__ __device__ constexpr int kernel_threads(bool fused) { return 64 + 32 * epilogue_warps(fused); }
+constexpr int FUSED_CHUNK = 32;  // columns a warp of the fused epilogue works on at a time
+constexpr int fused_staging_bytes(int out_bytes) { return epilogue_warps(true) * 32 * FUSED_CHUNK * out_bytes; }
 constexpr int SWIZZLE_ALIGN = 1024;
 constexpr int EPI_BUF_BYTES = 32 * 128;  // 32 rows of one 128-byte swizzle row
 constexpr int CLC_SLOTS = 3;             // answers in flight between the fastest and the slowest role
@@ -312,6 +320,262 @@ __device__ __forceinline__ void fold_schedules_off(GemmParams& p) {
 }
 #endif
 
+// The quantised bytes and scales of COLUMNS (32 or 64) values of row `row` from
+// column gc on (a multiple of COLUMNS), as the quantisation of a bfloat16 C
+// would make them.
+template <int FORMAT, int COLUMNS>
+__device__ __forceinline__ void store_quantized(const GemmParams& p, const float* x, int row, int gc) {
+  constexpr int BLOCK = FORMAT == Q_NVFP4 ? 16 : 32, BLOCKS = COLUMNS / BLOCK;
+  constexpr int WORDS = FORMAT == Q_MXFP8 ? BLOCK / 4 : BLOCK / 8;  // per block
+  uint32_t words[WORDS * BLOCKS], scales = 0;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    uint32_t stored;
+    quantize_block<FORMAT>(x + BLOCK * b, words + WORDS * b, stored);
+    scales |= (stored & 0xFFu) << (8 * b);
+  }
+  const size_t row_bytes = FORMAT == Q_MXFP8 ? size_t(p.rows_n) : size_t(p.rows_n >> 1);
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.d) + row * row_bytes + (FORMAT == Q_MXFP8 ? gc : gc >> 1));
+#pragma unroll
+  for (int u = 0; u < WORDS * BLOCKS / 4; ++u) dst[u] = make_uint4(words[4 * u], words[4 * u + 1], words[4 * u + 2], words[4 * u + 3]);
+  const int group = gc / BLOCK;  // this row's scale block
+  uint8_t* at = p.out_scales + (size_t(row >> 7) * p.out_k_groups + (group >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (group & 3);
+  if constexpr (BLOCKS == 4) *reinterpret_cast<uint32_t*>(at) = scales;
+  else if constexpr (BLOCKS == 2) *reinterpret_cast<uint16_t*>(at) = uint16_t(scales);
+  else *at = uint8_t(scales);
+}
+
+// The fused epilogue's warps (2 .. 9) of one CTA:
+//   z = alpha * acc + bias,  preact = z,  C = act(z) + residual
+// in float32, each tensor rounded once.  A warp works on 32 rows x 32 columns
+// at a time.  The residual comes in as whole row segments (64 or 128 bytes a
+// row, asked for one chunk ahead and before the accumulator is waited for) and
+// reaches the lane of its row through the warp's staging buffer, the way C goes
+// out; rows that are not whole 16-byte units pass through the buffer element by
+// element.  Two accumulator slots let the next tile's MMAs run meanwhile.
+template <int CTA_GROUP, int OUT_BYTES>
+__device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCtx& ctx, uint32_t staging, uint32_t bar_acc_full,
+                                               uint32_t bar_acc_empty, uint32_t tmem_base, uint32_t rank, int cluster_id, int num_clusters,
+                                               bool allocated) {
+  constexpr int TILE_M = 128 * CTA_GROUP, CHUNK = FUSED_CHUNK;
+  constexpr int ROW_BYTES = CHUNK * OUT_BYTES, UNITS = ROW_BYTES / 16;  // of a staging row: 4 or 8
+  constexpr int ROWS_AT_ONCE = 32 / UNITS, STEPS = 32 / ROWS_AT_ONCE, UNIT = 16 / OUT_BYTES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
+  const int chunk0 = ((warp - 2) >> 2) * CHUNK;
+  const uint32_t buf = staging + (warp - 2) * 32 * ROW_BYTES;
+  const int sub_row = lane / UNITS, unit = lane % UNITS;
+  // 16-byte unit u of row r sits swizzled, so that eight lanes on eight rows, or on
+  // the units of one row, touch all banks.
+  auto at_unit = [&](int r, int u) { return buf + r * ROW_BYTES + ((u ^ (UNITS == 8 ? r & 7 : (r >> 1) & 3)) << 4); };
+  auto at_element = [&](int r, int e) { return at_unit(r, e / UNIT) + (e % UNIT) * OUT_BYTES; };
+  const int tile_n = p.tile_n, rows_m = p.rows_m, rows_n = p.rows_n, ldd = p.ldd;
+  const bool transposed = p.transpose_out != 0, vec_ok = p.vec_ok != 0, out_f16 = p.out_f16 != 0;
+  const uint8_t* const residual = static_cast<const uint8_t*>(p.residual);
+  const bool residual_vec = residual && p.residual_vec && !transposed;
+  const float* const bias = p.bias;
+  const bool bias_vec = bias && (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
+  const float alpha = p.scale_out ? p.alpha : 1.0f;
+  const uint32_t acc_empty_leader = CTA_GROUP == 2 ? map_to_cta(bar_acc_empty, 0) : bar_acc_empty;
+  auto pack2 = [&](float lo, float hi) { return out_f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
+  auto widen = [&](uint32_t bits) { return out_f16 ? half_bits_to_float(bits) : __uint_as_float(bits << 16); };
+  if (p.pdl) pdl_wait_prior_grids();
+  int tile_idx = 0;
+  for (int tile = cluster_id; __all_sync(0xFFFFFFFFu, allocated) && tile < p.num_tiles; tile += num_clusters, ++tile_idx) {
+    const TileCoord t = tile_coord(p, tile);
+    const int row0 = t.mi * TILE_M + int(rank) * 128 + quarter * 32, row = row0 + lane;
+    const int col0 = t.ni * tile_n;
+    const int rows = min(32, rows_m - row0);  // of this warp, none or fewer at C's edge
+    uint4 res[STEPS];
+    auto whole = [&](int c) { return c + CHUNK <= tile_n && col0 + c + CHUNK <= rows_n; };
+    auto ask_residual = [&](int c) {
+      if (!residual_vec || !whole(c)) return;
+      const uint8_t* src = residual + (size_t(row0 + sub_row) * ldd + col0 + c) * OUT_BYTES + unit * 16;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i)
+        if (i * ROWS_AT_ONCE + sub_row < rows) res[i] = *reinterpret_cast<const uint4*>(src + size_t(i * ROWS_AT_ONCE) * ldd * OUT_BYTES);
+    };
+    ask_residual(chunk0);
+    if (transposed && row < rows_m) {  // few rows of C, this lane's column of each
+      if (bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + row));
+      if (residual)
+        for (int j = chunk0; j < min(chunk0 + CHUNK, min(tile_n, rows_n - col0)); ++j)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(residual + (size_t(col0 + j) * ldd + row) * OUT_BYTES));
+    } else if (bias) {
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + min(col0 + lane * 8, rows_n - 1)));
+    }
+    const int slot = (p.acc_slots == 2) ? (tile_idx & 1) : 0;
+    const uint32_t use = (p.acc_slots == 2) ? (tile_idx >> 1) : tile_idx;
+    const bool ready = mbar_wait(bar_acc_full + 8 * slot, use & 1, ctx, SITE_EPI_ACC_FULL);
+    if (!__all_sync(0xFFFFFFFFu, ready)) break;
+    tc_fence_after_sync();
+    const uint32_t acc = tmem_base + (uint32_t(quarter * 32) << 16) + slot * p.acc_stride;
+    auto hand_back = [&] {
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CTA_GROUP == 2) mbar_arrive_cluster(acc_empty_leader + 8 * slot);
+        else mbar_arrive(bar_acc_empty + 8 * slot);
+      }
+    };
+    // A chunk of this warp's rows, as rounded words or values in each lane, to `base`.
+    auto store = [&](const float* v, uint8_t* base, int c, int width) {
+      const int gc = col0 + c;
+      if (transposed) {  // this lane's MMA row is a column of C: a warp writes consecutive elements
+        if (row < rows_m) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            if (j < width && gc + j < rows_n) {
+              const size_t at = size_t(gc + j) * ldd + row;
+              if constexpr (OUT_BYTES == 4) reinterpret_cast<float*>(base)[at] = v[j];
+              else reinterpret_cast<uint16_t*>(base)[at] = uint16_t(pack2(v[j], 0.0f) & 0xFFFFu);
+            }
+          }
+        }
+        return;
+      }
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        uint32_t q[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          q[h] = OUT_BYTES == 4 ? __float_as_uint(v[(4 * u + h) % CHUNK]) : pack2(v[(8 * u + 2 * h) % CHUNK], v[(8 * u + 2 * h + 1) % CHUNK]);
+        st_shared_v4(at_unit(lane, u), q[0], q[1], q[2], q[3]);
+      }
+      __syncwarp();
+      if (vec_ok) {
+        const int gcol = gc + unit * UNIT;
+        if (unit * UNIT < width && gcol < rows_n) {
+          uint8_t* dst = base + (size_t(row0 + sub_row) * ldd + gcol) * OUT_BYTES;
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) {
+            const int r = i * ROWS_AT_ONCE + sub_row;
+            if (r < rows) *reinterpret_cast<uint4*>(dst + size_t(i * ROWS_AT_ONCE) * ldd * OUT_BYTES) = ld_shared_v4(at_unit(r, unit));
+          }
+        }
+      } else if (lane < min(width, rows_n - gc)) {
+        uint8_t* dst = base + (size_t(row0) * ldd + gc + lane) * OUT_BYTES;
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r, dst += size_t(ldd) * OUT_BYTES) {
+          if constexpr (OUT_BYTES == 4) *reinterpret_cast<uint32_t*>(dst) = ld_shared_u32(at_element(r, lane));
+          else *reinterpret_cast<uint16_t*>(dst) = ld_shared_u16(at_element(r, lane));
+        }
+      }
+      __syncwarp();
+    };
+
+    bool handed_back = false;
+    for (int c = chunk0; c < tile_n && col0 + c < rows_n && rows > 0; c += 2 * CHUNK) {
+      const int width = min(CHUNK, tile_n - c), gc = col0 + c;
+      float v[CHUNK];
+      uint32_t* const raw = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+      for (int j = 16; j < CHUNK; ++j) raw[j] = 0u;
+      if (width == CHUNK) tmem_ld_32(acc + c, raw);
+      else tmem_ld_16(acc + c, raw);
+      tmem_ld_wait();
+      tmem_ld_settle_32(raw);
+      const int next = c + 2 * CHUNK;
+      if (!(next < tile_n && col0 + next < rows_n)) {
+        hand_back();
+        handed_back = true;
+      }
+      if (p.scale_out) {
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
+      }
+      if (bias) {
+        if (transposed) {
+          const float mine = __ldg(bias + min(row, rows_m - 1));
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) v[j] += mine;
+        } else if (bias_vec && gc + CHUNK <= rows_n) {
+#pragma unroll
+          for (int u = 0; u < CHUNK / 4; ++u) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(bias + gc) + u);
+            v[4 * u] += q.x, v[4 * u + 1] += q.y, v[4 * u + 2] += q.z, v[4 * u + 3] += q.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) v[j] += __ldg(bias + min(gc + j, rows_n - 1));
+        }
+      }
+      if (p.preact) store(v, static_cast<uint8_t*>(p.preact), c, width);
+      if (p.act_shape == SHAPE_SIGMOID) {
+        const float a = p.act_a, b = p.act_b;
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_SIGMOID>(v[j], a, b);
+      } else if (p.act_shape == SHAPE_PHI) {
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_PHI>(v[j], 0.f, 0.f);
+      } else if (p.act_shape == SHAPE_RELU) {
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_RELU>(v[j], 0.f, 0.f);
+      }
+      if (residual && transposed) {
+        if (row < rows_m) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            if (j < width && gc + j < rows_n) {
+              const size_t at = size_t(gc + j) * ldd + row;
+              if constexpr (OUT_BYTES == 4) v[j] += reinterpret_cast<const float*>(residual)[at];
+              else v[j] += widen(reinterpret_cast<const uint16_t*>(residual)[at]);
+            }
+          }
+        }
+      } else if (residual) {
+        if (residual_vec && whole(c)) {
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) st_shared_v4(at_unit(i * ROWS_AT_ONCE + sub_row, unit), res[i].x, res[i].y, res[i].z, res[i].w);
+        } else {
+          const bool live = lane < min(width, rows_n - gc);
+          const uint8_t* src = residual + (size_t(row0) * ldd + gc + lane) * OUT_BYTES;
+#pragma unroll 8
+          for (int r = 0; r < rows; ++r, src += size_t(ldd) * OUT_BYTES) {
+            if constexpr (OUT_BYTES == 4) st_shared_u32(at_element(r, lane), live ? *reinterpret_cast<const uint32_t*>(src) : 0u);
+            else st_shared_u16(at_element(r, lane), live ? *reinterpret_cast<const uint16_t*>(src) : uint16_t(0));
+          }
+        }
+        __syncwarp();
+        ask_residual(next);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          const uint4 q4 = ld_shared_v4(at_unit(lane, u));
+          const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            if constexpr (OUT_BYTES == 4) {
+              v[(4 * u + h) % CHUNK] += __uint_as_float(q[h]);
+            } else {
+              v[(8 * u + 2 * h) % CHUNK] += out_f16 ? half_bits_to_float(q[h]) : __uint_as_float(q[h] << 16);
+              v[(8 * u + 2 * h + 1) % CHUNK] += out_f16 ? half_bits_to_float(q[h] >> 16) : __uint_as_float(q[h] & 0xFFFF0000u);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if constexpr (OUT_BYTES == 2) {
+        if (p.out_quant) {
+          if (row < rows_m) {
+#pragma unroll
+            for (int u = 0; u < CHUNK / 2; ++u) {  // the bytes equal those of quantising a bfloat16 C
+              const uint32_t both = pack_bf16x2(v[2 * u], v[2 * u + 1]);
+              v[2 * u] = __uint_as_float(both << 16);
+              v[2 * u + 1] = __uint_as_float(both & 0xFFFF0000u);
+            }
+            if (p.out_quant == 1 + Q_NVFP4) store_quantized<Q_NVFP4, CHUNK>(p, v, row, gc);
+            else if (p.out_quant == 1 + Q_MXFP8) store_quantized<Q_MXFP8, CHUNK>(p, v, row, gc);
+            else store_quantized<Q_MXFP4, CHUNK>(p, v, row, gc);
+          }
+          continue;
+        }
+      }
+      store(v, static_cast<uint8_t*>(p.d), c, width);
+    }
+    if (!handed_back) hand_back();
+  }
+}
+
+
 // FIXED_N == 0: every tile-plan value is read from `params` at run time.
 // FIXED_N != 0: the kernel is compiled for tiles FIXED_N wide with epilogue
 // path FIXED_EPI (0 each thread its own row, 1 staged rows, 2 TMA stores).
@@ -321,10 +585,9 @@ __device__ __forceinline__ void fold_schedules_off(GemmParams& p) {
 // the path it takes: bf16 128^3 spends 2.2 us between the previous grid's
 // completion and its own in the full kernel, 1.5 us in the plain one and
 // 1.0 us in one compiled for its tile shape.
-// FUSED: the static schedule with the activation, residual and pre-activation
-// of the fused epilogue (which the other builds do not carry).
+// FUSED: the static schedule with fused_epilogue, which the other builds do not carry.
 template <int KIND, int CTA_GROUP, int OUT_BYTES, int FIXED_N = 0, int FIXED_EPI = 0, bool PLAIN = false, bool FUSED = false>
-__global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant__ GemmParams params, const LaunchPad) {
+__global__ void __launch_bounds__(kernel_threads(FUSED), 1) gemm_kernel(const __grid_constant__ GemmParams params, const LaunchPad) {
   // `p` is the scalar view of the launch parameters.  A standalone kernel
   // emitted for one shape defines OG_FIXED_PLAN to overwrite the plan fields
   // of a local copy with literals, which lets the compiler fold them; tensor
@@ -402,7 +665,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar_acc_full + 8 * s, 1);
-      mbar_init(bar_acc_empty + 8 * s, 4 * CTA_GROUP);
+      mbar_init(bar_acc_empty + 8 * s, epilogue_warps(FUSED) * CTA_GROUP);
     }
     if (p.use_clc) {
       for (int s = 0; s < CLC_SLOTS; ++s) {
@@ -612,6 +875,10 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
         if (ok) mma_commit<CTA_GROUP>(bar_acc_full + 8 * slot);
       }
     }
+  } else if constexpr (FUSED) {
+    const bool allocated = mbar_wait(bar_tmem, 0, ctx, SITE_TMEM_READY);
+    tc_fence_after_sync();
+    fused_epilogue<CTA_GROUP, OUT_BYTES>(p, ctx, epi_base, bar_acc_full, bar_acc_empty, tmem_slot, rank, cluster_id, num_clusters, allocated);
   } else {
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;  // the 32 tensor-memory lanes this warp may read
@@ -651,29 +918,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
     WorkIter work(p, cluster_id, num_clusters, k_rank);
     if (p.use_clc) work.enable_clc(clc_state(false, lane == 0), CTA_GROUP);
     Work w;
-    // Fused epilogue: this thread's 128 bytes of the residual's next chunk.  They
-    // are requested before the accumulator is waited for, and the following
-    // chunk's as soon as these are used, so that the stores and the next
-    // tensor-memory load hide the trip to memory.  Each lane reads its own row:
-    // eight 16-byte loads of one line, which L1 serves after the first.  (Plain
-    // loads, not read-only ones: the residual may be C itself.)
-    uint4 res[FUSED ? 8 : 1];
-    const uint8_t* const residual = FUSED ? static_cast<const uint8_t*>(p.residual) : nullptr;
-    const bool residual_vec = FUSED && p.residual_vec && !transpose_out;
     for (; __all_sync(0xFFFFFFFFu, allocated) && work.next(w); ++tile_idx) {
       const TileCoord t = tile_coord(p, w.tile);
-      if constexpr (FUSED) {
-        if (residual_vec) {
-          if (p.pdl && !touched_memory) pdl_wait_prior_grids();
-          touched_memory = true;
-          const int r = t.mi * TILE_M + int(rank) * 128 + quarter * 32 + lane, c = t.ni * tile_n;
-          if (r < rows_m && c + CHUNK <= rows_n && CHUNK <= tile_n) {
-            const uint4* src = reinterpret_cast<const uint4*>(residual + (size_t(r) * ldd + c) * OUT_BYTES);
-#pragma unroll
-            for (int u = 0; u < 8; ++u) res[FUSED ? u : 0] = src[u];
-          }
-        }
-      }
       // Stream-K roles (a cluster-K rank also holds a K slice, but exchanges it through shared memory below).
       const bool contributes = p.stream_k && w.kb0 > 0;          // publish partial sums instead of output
       const bool finishes = p.stream_k && w.kb0 == 0 && w.kb1 < p.k_blocks;  // add the sharers' partials before storing
@@ -701,7 +947,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
       // rows at a time and stores whole 128-byte segments, clipped at the
       // edges of D.  Plain st.global: nothing to wait for before the buffer
       // is reused but the warp's own reads.
-      auto store_staged = [&](const uint32_t* w, int c, int width, uint8_t* base) {
+      auto store_staged = [&](const uint32_t* w, int c, int width) {
         const uint32_t rowaddr = my_buf + lane * 128;
 #pragma unroll
         for (int u = 0; u < 8; ++u)
@@ -710,7 +956,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
         __syncwarp();
         const int gcol = col0 + c + unit * UNIT;
         if (unit * UNIT < width && gcol < rows_n) {
-          uint8_t* dst = base + (size_t(row0 + sub_row) * ldd + gcol) * OUT_BYTES;
+          uint8_t* dst = out + (size_t(row0 + sub_row) * ldd + gcol) * OUT_BYTES;
           const size_t step = size_t(4) * ldd * OUT_BYTES;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -733,7 +979,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
             if (lane == 0) tma_store_wait_read<0>();
             __syncwarp();
           }
-          store_staged(w, c, width, out);
+          store_staged(w, c, width);
           return;
         }
         const uint32_t buf = my_buf + (buf_use & 1) * EPI_BUF_BYTES;
@@ -762,7 +1008,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
       // released, and only then are the held chunks stored.
       bool handed_back = false, handed_back_late = false;
       if constexpr (OUT_BYTES == 2) {
-        if (!FUSED && p.acc_slots == 1 && staged && tile_n == 256 && !contributes && !finishes && !scale_out && !bias && !out_f16 &&
+        if (p.acc_slots == 1 && staged && tile_n == 256 && !contributes && !finishes && !scale_out && !bias && !out_f16 &&
             !p.out_quant && cluster_k == 1 && row0 < rows_m) {
           auto pack64 = [](const uint32_t* f, uint32_t* w) {
 #pragma unroll
@@ -970,82 +1216,6 @@ __global__ void __launch_bounds__(THREADS, 1) gemm_kernel(const __grid_constant_
             const float mine = __ldg(bias + min(row, rows_m - 1));
 #pragma unroll
             for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + mine);
-          }
-        }
-        if constexpr (FUSED) {
-          const int gc = col0 + c;
-          auto value_bits = [&](uint32_t x) { return OUT_BYTES == 4 ? x : pack2(x, 0u) & 0xFFFFu; };
-          if (p.preact) {
-            // The pre-activation leaves by the same paths as C itself below (never by TMA store).
-            uint8_t* const pre = static_cast<uint8_t*>(p.preact);
-            if (staged && row0 < rows_m) {
-              uint32_t w[32];
-#pragma unroll
-              for (int u = 0; u < 32; ++u) w[u] = OUT_BYTES == 4 ? v[u] : pack2(v[(2 * u) % CHUNK], v[(2 * u + 1) % CHUNK]);
-              store_staged(w, c, width, pre);
-            } else if (row < rows_m) {
-#pragma unroll
-              for (int j = 0; j < CHUNK; ++j) {
-                if (j < width && gc + j < rows_n) {
-                  const size_t at = transpose_out ? size_t(gc + j) * ldd + row : size_t(row) * ldd + gc + j;
-                  if constexpr (OUT_BYTES == 4) reinterpret_cast<uint32_t*>(pre)[at] = v[j];
-                  else reinterpret_cast<uint16_t*>(pre)[at] = uint16_t(value_bits(v[j]));
-                }
-              }
-            }
-          }
-          if (p.act_shape == SHAPE_SIGMOID) {
-            const float a = p.act_a, b = p.act_b;
-#pragma unroll
-            for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(act_value<SHAPE_SIGMOID>(__uint_as_float(v[j]), a, b));
-          } else if (p.act_shape == SHAPE_PHI) {
-#pragma unroll
-            for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(act_value<SHAPE_PHI>(__uint_as_float(v[j]), 0.f, 0.f));
-          } else if (p.act_shape == SHAPE_RELU) {
-#pragma unroll
-            for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(act_value<SHAPE_RELU>(__uint_as_float(v[j]), 0.f, 0.f));
-          }
-          if (residual && row < rows_m) {
-            if (residual_vec && gc + CHUNK <= rows_n && width == CHUNK) {
-#pragma unroll
-              for (int u = 0; u < 8; ++u) {
-                const uint32_t q[4] = {res[FUSED ? u : 0].x, res[FUSED ? u : 0].y, res[FUSED ? u : 0].z, res[FUSED ? u : 0].w};
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                  if constexpr (OUT_BYTES == 4) {
-                    v[4 * u + h] = __float_as_uint(__uint_as_float(v[4 * u + h]) + __uint_as_float(q[h]));
-                  } else {
-                    const int j = (8 * u + 2 * h) % CHUNK;
-                    const float lo = out_f16 ? half_bits_to_float(q[h]) : __uint_as_float(q[h] << 16);
-                    const float hi = out_f16 ? half_bits_to_float(q[h] >> 16) : __uint_as_float(q[h] & 0xFFFF0000u);
-                    v[j] = __float_as_uint(__uint_as_float(v[j]) + lo);
-                    v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + hi);
-                  }
-                }
-              }
-              const int next = c + CHUNK;
-              if (next + CHUNK <= tile_n && col0 + next + CHUNK <= rows_n) {
-                const uint4* src = reinterpret_cast<const uint4*>(residual + (size_t(row) * ldd + col0 + next) * OUT_BYTES);
-#pragma unroll
-                for (int u = 0; u < 8; ++u) res[FUSED ? u : 0] = src[u];
-              }
-            } else {
-              before_global_memory();
-#pragma unroll
-              for (int j = 0; j < CHUNK; ++j) {
-                if (j < width && gc + j < rows_n) {
-                  const size_t at = transpose_out ? size_t(gc + j) * ldd + row : size_t(row) * ldd + gc + j;
-                  float add;
-                  if constexpr (OUT_BYTES == 4) {
-                    add = reinterpret_cast<const float*>(residual)[at];
-                  } else {
-                    const uint32_t bits = reinterpret_cast<const uint16_t*>(residual)[at];
-                    add = out_f16 ? half_bits_to_float(bits) : __uint_as_float(bits << 16);
-                  }
-                  v[j] = __float_as_uint(__uint_as_float(v[j]) + add);
-                }
-              }
-            }
           }
         }
         if constexpr (OUT_BYTES == 2) {

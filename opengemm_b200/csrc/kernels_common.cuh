@@ -12,7 +12,7 @@ cudaError_t launch_one(const GemmParams& params, int grid, int smem_bytes, cudaS
                        bool pdl) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(grid, 1, 1);
-  config.blockDim = dim3(THREADS, 1, 1);
+  config.blockDim = dim3(kernel_threads(FUSED), 1, 1);
   config.dynamicSmemBytes = size_t(smem_bytes);
   config.stream = stream;
   cudaLaunchAttribute attrs[2];

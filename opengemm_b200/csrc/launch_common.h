@@ -11,6 +11,7 @@
 // keyed by pointer and geometry.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -233,8 +234,7 @@ inline int fill_params(const Plan& p, const OgGemm& g, const LaunchPointers& io,
   if (rc != OG_OK) return rc;
   const bool c_aligned = (reinterpret_cast<uintptr_t>(io.c) & 15) == 0;
   const int epi_staged = p.epi_staged && c_aligned;
-  const int epi_tma = p.epi_tma && c_aligned && !io.out_quant &&  // block-scaled C is stored by its own path,
-                      !io.preact;  // and a kept pre-activation shares C's staging buffer
+  const int epi_tma = p.epi_tma && c_aligned && !io.out_quant && !io.fused();  // block-scaled and fused C have stores of their own
   if (epi_tma) {
     const int type = p.format->out == OUT_S32    ? int(CU_TENSOR_MAP_DATA_TYPE_INT32)
                      : p.format->out == OUT_BF16 ? int(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16)
@@ -297,6 +297,12 @@ inline int fill_params(const Plan& p, const OgGemm& g, const LaunchPointers& io,
     params.scale_out = 1;
     params.alpha = *alpha;
   }
+  if (io.fused()) {
+    // Eight epilogue warps with a staging buffer each; the ring gives up what that takes.
+    params.epi_staged = 1;
+    params.epi_tma = 0;
+    params.stages = std::min(p.stages, (SMEM_LIMIT - SMEM_RESERVE - fused_staging_bytes(p.out_bytes)) / p.stage_bytes);
+  }
   params.residual = io.residual;
   params.preact = io.preact;
   act_constants(io.activation, &params.act_shape, &params.act_a, &params.act_b);
@@ -307,6 +313,11 @@ inline int fill_params(const Plan& p, const OgGemm& g, const LaunchPointers& io,
     params.out_k_groups = ceil_div(g.n, io.out_quant == 1 ? 64 : 128);
   }
   return OG_OK;
+}
+
+// Shared memory of a launch whose parameters fill_params has filled.
+inline int launch_smem_bytes(const Plan& p, const GemmParams& params, bool fused) {
+  return fused ? params.stages * params.stage_bytes + fused_staging_bytes(p.out_bytes) + 1024 : p.smem_bytes;
 }
 
 // The limit of device-side waits set by og_b200_set_wait_limit_ms (host.cu).

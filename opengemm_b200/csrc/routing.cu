@@ -159,18 +159,31 @@ __device__ __forceinline__ void load_logits(const T* row, int lane, int experts,
   for (int j = 0; j < VALUES; ++j) l[j] = lane * VALUES + j < experts ? to_float(row[lane * VALUES + j]) : -INFINITY;
 }
 
+// One step of a sorting network, larger key first.
+__device__ __forceinline__ void order_keys(uint32_t& a, uint32_t& b) {
+  const uint32_t hi = max(a, b);
+  b = min(a, b);
+  a = hi;
+}
+
 // One warp per token; lane `lane` holds VALUES consecutive experts, so that the
 // first lane that reaches a maximum also holds the lowest such index, and a
 // choice is one warp-wide maximum, a ballot and a shuffle; only the winning
-// lane rescans its values.  16-bit logits that are compared themselves leave
-// the low bits of their key free: with the (inverted) index in there a choice
-// is the maximum alone.  Without a bias the order of the scores is that of the
-// logits, which no rounding blurs, so those are compared.
+// lane looks for its next best.
 //
-// Bound by instruction issue: 16384 tokens of 128 experts, top 8, move 4 MB
-// but execute some 300 instructions a warp.
-template <int VALUES, typename T>
+// SIMPLE: neither bias nor groups.  The order of the scores is then that of the
+// logits, which no rounding blurs, so those are compared, and renormalised
+// softmax weights need neither the row's sum nor the other experts' exponentials.
+// The key of a 16-bit logit leaves its low bits free: with the (inverted) index
+// in there a choice is the maximum alone, and each lane keeps its few keys
+// sorted so that the next best moves up.
+//
+// Bound by instruction issue (16384 tokens of 128 experts, top 8, are 4 MB):
+// 690 instructions a warp and 13.2 us before the two shortcuts.
+template <int VALUES, typename T, bool SIMPLE>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RouteParams p) {
+  constexpr bool PACKED = SIMPLE && sizeof(T) == 2;
+  constexpr bool SORTED = PACKED && VALUES <= 8;
   pdl_wait_prior_grids();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
@@ -181,16 +194,17 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RoutePara
   float l[VALUES];
   load_logits(row, lane, p.experts, l);
   const bool sigmoid = p.sigmoid != 0;
-  const RowScale r = row_scale(l, sigmoid);
+  RowScale r{0.0f, 1.0f};
+  const bool by_chosen = SIMPLE && p.renormalise;  // scores relative to the largest chosen one
+  if (!by_chosen) r = row_scale(l, sigmoid);
   uint32_t key[VALUES];
-  const bool by_score = p.bias != nullptr || p.groups > 1;
 #pragma unroll
   for (int j = 0; j < VALUES; ++j) {
     float c = l[j];
-    if (by_score && c != -INFINITY) c = score_of(l[j], r, sigmoid) + (p.bias && id0 + j < p.experts ? p.bias[id0 + j] : 0.0f);
+    if (!SIMPLE && c != -INFINITY) c = score_of(l[j], r, sigmoid) + (p.bias && id0 + j < p.experts ? p.bias[id0 + j] : 0.0f);
     key[j] = score_key(c, l[j] != -INFINITY);
   }
-  if (p.groups > 1) {
+  if (!SIMPLE && p.groups > 1) {
     uint32_t group_key = 0;  // of group `lane`
     for (int g = 0; g < p.groups; ++g) {
       const int first = g * p.each - id0, last = first + p.each;  // in this lane's values
@@ -230,34 +244,67 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RoutePara
     }
   }
   int mine = -1;  // choice number `lane`
-  const bool packed = sizeof(T) == 2 && !p.bias;
-  if (packed) {
+  if constexpr (PACKED) {
     constexpr uint32_t LOW = 0x3FFu;  // a 16-bit float's key has at least 13 zeros (or, negative, ones) below
 #pragma unroll
     for (int j = 0; j < VALUES; ++j) key[j] = key[j] ? (key[j] & ~LOW) | (LOW - uint32_t(id0 + j)) : 0u;
-  }
-  uint32_t best = 0;
-  int at = 0;
-  auto rescan = [&] {
-    best = key[0], at = id0;
+    if constexpr (SORTED) {
 #pragma unroll
-    for (int j = 1; j < VALUES; ++j)
-      if (key[j] > best) best = key[j], at = id0 + j;
-  };
-  rescan();
-  for (int i = 0; i < p.top_k; ++i) {
-    const uint32_t top = __reduce_max_sync(ALL, best);
-    if (!top) break;
-    const bool won = packed ? best == top : __ffs(__ballot_sync(ALL, best == top)) - 1 == lane;
-    const int winner = packed ? int(0x3FFu - (top & 0x3FFu)) : __shfl_sync(ALL, at, __ffs(__ballot_sync(ALL, won)) - 1);
-    if (lane == i) mine = winner;
-    if (won) {
+      for (int step = 0; step < VALUES; ++step)  // odd-even transposition: neighbours only
 #pragma unroll
-      for (int j = 0; j < VALUES; ++j) key[j] = id0 + j == at ? 0u : key[j];
-      rescan();
+        for (int j = step & 1; j + 1 < VALUES; j += 2) order_keys(key[j], key[j + 1]);
+    }
+    uint32_t best = key[0];
+    if constexpr (!SORTED) {
+#pragma unroll
+      for (int j = 1; j < VALUES; ++j) best = max(best, key[j]);
+    }
+    for (int i = 0; i < p.top_k; ++i) {
+      const uint32_t top = __reduce_max_sync(ALL, best);
+      if (!top) break;
+      if (lane == i) mine = int(LOW - (top & LOW));
+      if (best == top) {
+        if constexpr (SORTED) {
+#pragma unroll
+          for (int j = 0; j + 1 < VALUES; ++j) key[j] = key[j + 1];
+          key[VALUES - 1] = 0;
+          best = key[0];
+        } else {
+          best = 0;
+#pragma unroll
+          for (int j = 0; j < VALUES; ++j) {
+            key[j] = key[j] == top ? 0u : key[j];
+            best = max(best, key[j]);
+          }
+        }
+      }
+    }
+  } else {
+    uint32_t best = 0;
+    int at = 0;
+    auto rescan = [&] {
+      best = key[0], at = id0;
+#pragma unroll
+      for (int j = 1; j < VALUES; ++j)
+        if (key[j] > best) best = key[j], at = id0 + j;
+    };
+    rescan();
+    for (int i = 0; i < p.top_k; ++i) {
+      const uint32_t top = __reduce_max_sync(ALL, best);
+      if (!top) break;
+      const int holder = __ffs(__ballot_sync(ALL, best == top)) - 1;
+      const int winner = __shfl_sync(ALL, at, holder);
+      if (lane == i) mine = winner;
+      if (lane == holder) {
+#pragma unroll
+        for (int j = 0; j < VALUES; ++j) key[j] = id0 + j == at ? 0u : key[j];
+        rescan();
+      }
     }
   }
-  float w = mine >= 0 ? score_of(to_float(row[mine]), r, sigmoid) : 0.0f;
+  const float chosen = mine >= 0 ? to_float(row[mine]) : -INFINITY;
+  if (by_chosen) r.top = __shfl_sync(ALL, chosen, 0);
+  float w = score_of(chosen, r, sigmoid);
   if (p.renormalise) {
     const float total = warp_sum(w);
     w = total == 0.0f ? 0.0f : w / total;
@@ -343,8 +390,8 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const 
 // stable counting sort.  A block takes a chunk of pairs and each of its warps a
 // contiguous part, so ranks follow from counts in order: before the chunk
 // (histograms of a first kernel), before the warp's part (counts in shared
-// memory), inside it (lanes with the same expert, match_any).  No atomics
-// decide an order, so the plan is the same every time.
+// memory), inside it (lanes with the same expert).  Atomics only count, they
+// decide no order, so the plan is the same every time.
 // A lane reads its PLAN_EACH pairs at once and keeps them: with a load per step
 // the chain of trips to L2 was most of the time (4096 pairs: 6.9 us).
 constexpr int PLAN_WARPS = 32;
@@ -390,7 +437,6 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams 
   const int begin = first + min(warp * part, size), end = first + min((warp + 1) * part, size);
   int* const own = counts + warp * p.experts;
   int expert[PLAN_EACH];
-  unsigned same[PLAN_EACH];
 #pragma unroll
   for (int s = 0; s < PLAN_EACH; ++s) {
     const int i = begin + s * 32 + lane;
@@ -398,21 +444,21 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams 
     if (expert[s] >= p.experts || expert[s] < 0) expert[s] = -1;
   }
 #pragma unroll
-  for (int s = 0; s < PLAN_EACH; ++s) {
-    if (begin + s * 32 >= end) break;
-    const int e = expert[s];
-    same[s] = __match_any_sync(ALL, e);
-    if (e >= 0 && lane == __ffs(same[s]) - 1) own[e] += __popc(same[s]);
-    __syncwarp();
-  }
+  for (int s = 0; s < PLAN_EACH; ++s)
+    if (expert[s] >= 0) atomicAdd(&own[expert[s]], 1);  // a count, whatever the order
   __syncthreads();
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
     int run = 0;
+#pragma unroll 1
+    for (int w0 = 0; w0 < PLAN_WARPS; w0 += 16) {  // sixteen loads in flight, not one
+      int part_of[16];
 #pragma unroll
-    for (int w = 0; w < PLAN_WARPS; ++w) {
-      const int c = counts[w * p.experts + e];
-      counts[w * p.experts + e] = run;
-      run += c;
+      for (int w = 0; w < 16; ++w) part_of[w] = counts[(w0 + w) * p.experts + e];
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        counts[(w0 + w) * p.experts + e] = run;
+        run += part_of[w];
+      }
     }
     int before = 0, total = run;
     if (p.chunks > 1) {
@@ -453,9 +499,14 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams 
     const int i = begin + s * 32 + lane;
     if (i - lane >= end) break;
     const int e = expert[s];
-    const int row = e >= 0 ? base[e] + own[e] + __popc(same[s] & ((1u << lane) - 1)) : -1;
+    unsigned same = __ballot_sync(ALL, e >= 0);  // lanes with the same expert: one ballot per bit of its number
+    for (int bit = 1; bit < p.experts; bit *= 2) {
+      const unsigned set = __ballot_sync(ALL, (e & bit) != 0);
+      same &= (e & bit) ? set : ~set;
+    }
+    const int row = e >= 0 ? base[e] + own[e] + __popc(same & ((1u << lane) - 1)) : -1;
     __syncwarp();
-    if (e >= 0 && lane == __ffs(same[s]) - 1) own[e] += __popc(same[s]);
+    if (e >= 0 && lane == __ffs(same) - 1) own[e] += __popc(same);
     __syncwarp();
     if (i < end) {
       p.positions[i] = row;
@@ -674,15 +725,24 @@ __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientPara
   if (at < p.n) p.partial[(long long)blockIdx.x * p.n + at] = total;
 }
 
-__global__ void __launch_bounds__(128) column_sum_kernel(const float* partial, float* out, int blocks, int n) {
+// Sums over the row blocks: eight lanes take every eighth block, added in order.
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* partial, float* out, int blocks, int n) {
   pdl_wait_prior_grids();
   pdl_launch_dependents();
-  const int col = blockIdx.x * 128 + threadIdx.x;
-  if (col >= n) return;
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float sum = 0.0f;
+  if (col < n) {
 #pragma unroll 8
-  for (int b = 0; b < blocks; ++b) sum += partial[(long long)b * n + col];
-  out[col] = sum;
+    for (int b = part; b < blocks; b += 8) sum += partial[(long long)b * n + col];
+  }
+  __shared__ float parts[8][32];
+  parts[part][lane] = sum;
+  __syncthreads();
+  if (part || col >= n) return;
+  float total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) total += parts[i][lane];
+  out[col] = total;
 }
 
 // -------------------------------------------------------------------- host
@@ -729,7 +789,8 @@ auto pick_values(int experts) {
   return values <= 1 ? Picker<1, T>::kernel : values <= 2 ? Picker<2, T>::kernel : values <= 4 ? Picker<4, T>::kernel
          : values <= 8 ? Picker<8, T>::kernel : values <= 16 ? Picker<16, T>::kernel : Picker<32, T>::kernel;
 }
-template <int VALUES, typename T> struct RouteForward { static constexpr void (*kernel)(RouteParams) = route_kernel<VALUES, T>; };
+template <int VALUES, typename T> struct RouteSimple { static constexpr void (*kernel)(RouteParams) = route_kernel<VALUES, T, true>; };
+template <int VALUES, typename T> struct RouteForward { static constexpr void (*kernel)(RouteParams) = route_kernel<VALUES, T, false>; };
 template <int VALUES, typename T> struct RouteGradient { static constexpr void (*kernel)(RouteParams) = route_gradient_kernel<VALUES, T>; };
 
 int check_route(const OgRoute& r) {
@@ -765,9 +826,10 @@ OG_API int32_t og_b200_route(const OgRoute* route, const void* logits, const flo
   p.logits = logits, p.bias = bias, p.weights = weights, p.indices = indices, p.tokens = r.tokens, p.experts = r.experts;
   p.top_k = r.top_k, p.sigmoid = r.sigmoid, p.groups = r.groups, p.each = r.experts / r.groups, p.top_groups = r.top_groups;
   p.group_top = r.group_top, p.renormalise = r.renormalise, p.scale = r.scale;
-  const auto kernel = r.dtype == TYPE_F32    ? pick_values<RouteForward, float>(r.experts)
-                      : r.dtype == TYPE_BF16 ? pick_values<RouteForward, __nv_bfloat16>(r.experts)
-                                             : pick_values<RouteForward, __half>(r.experts);
+  const bool simple = !bias && r.groups == 1;
+#define OG_ROUTE(T) (simple ? pick_values<RouteSimple, T>(r.experts) : pick_values<RouteForward, T>(r.experts))
+  const auto kernel = r.dtype == TYPE_F32 ? OG_ROUTE(float) : r.dtype == TYPE_BF16 ? OG_ROUTE(__nv_bfloat16) : OG_ROUTE(__half);
+#undef OG_ROUTE
   return dependent_launch(kernel, dim3(unsigned((r.tokens + ROUTE_WARPS - 1) / ROUTE_WARPS)), ROUTE_WARPS * 32, 0, stream, p);
 }
 
@@ -884,7 +946,7 @@ OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, co
     if (const int bad = dependent_launch(kernel, grid, 256, 0, stream, p)) return bad;
   }
   if (!bias_gradient) return OG_OK;
-  return dependent_launch(column_sum_kernel, dim3(unsigned((n + 127) / 128)), 128, 0, stream, (const float*)workspace, bias_gradient, blocks, int(n));
+  return dependent_launch(column_sum_kernel, dim3(unsigned((n + 31) / 32)), 256, 0, stream, (const float*)workspace, bias_gradient, blocks, int(n));
 }
 
 }  // extern "C"
