@@ -366,6 +366,22 @@ OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, co
                                            int64_t rows, int32_t n, int32_t device, void* stream);
 OG_API const char* og_b200_routing_error(void);
 
+/* Gradients of C = act(factor * A . B^T + bias): with dz = grad * act'(z),
+ *   grad_a = factor * dz . B,  grad_b = factor * dz^T . A,  grad_bias = column sums of dz.
+ * grad, z and dz (scratch, not used without an activation) [m, n], a [m, k], b [n, k], all of
+ * `dtype` ("bf16" or "f16"), n and k multiples of 8, on 16-byte boundaries; grad_a and grad_b
+ * of `dtype` or float32 (out_f32), grad_bias float32 [n] through `partial`, ceil(m / 64) * n
+ * floats.  A gradient whose pointer is null is not computed.  Errors: og_b200_experts_error(). */
+typedef struct OgGemmGradients {
+  const void *grad, *a, *b, *z;
+  void *dz, *grad_a, *grad_b;
+  float *grad_bias, *partial;
+  int32_t m, n, k, activation, out_f32;
+  float factor;
+  char dtype[16];
+} OgGemmGradients;
+OG_API int32_t og_b200_gemm_gradients(const OgGemmGradients* g, int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

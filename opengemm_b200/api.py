@@ -214,6 +214,7 @@ def gemm_backward(grad, a, b, activation=None, preactivation=None, alpha=None, w
         raise TypeError(f"gradients are served for bfloat16 and float16 CUDA operands, got {a.dtype} on {a.device}")
     name = "bf16" if a.dtype is torch.bfloat16 else "f16"
     d = DTYPES[name]
+    out_dtype = out_dtype or a.dtype
     if a.dim() != 2 or b.dim() != 2:
         raise TypeError("a and b must be contiguous 2-D CUDA tensors")
     m, n, k = a.size(0), b.size(0), a.size(1)
@@ -230,28 +231,30 @@ def gemm_backward(grad, a, b, activation=None, preactivation=None, alpha=None, w
         if t is not None and not (t.is_cuda and t.device == a.device and t.dtype is a.dtype and t.is_contiguous()
                                   and t.shape == (m, n)):
             raise TypeError(f"{label} must be a contiguous {a.dtype} [{m}, {n}] on {a.device}")
-    if out_dtype not in (None, a.dtype, torch.float32):
+    if out_dtype is not a.dtype and out_dtype is not torch.float32:
         raise TypeError(f"gradients leave as {a.dtype} or torch.float32, not {out_dtype}")
     for label, t in (("grad", grad), ("preactivation", preactivation), ("a", a), ("b", b)):
         if t is not None and t.data_ptr() % 16:
             raise ValueError(f"{label} must start on a 16-byte boundary")
-    out_dtype = out_dtype or a.dtype
-    lib = capi.library("mm")
-    dz, grad_a, grad_b, grad_bias, workspace = grad, None, None, None, None
-    if activation is not None:
-        dz = torch.empty_like(grad)
+    grad_a = grad_b = grad_bias = scratch = None
+    if "a" in want:
+        grad_a = torch.empty_like(a, dtype=out_dtype)
+    if "b" in want:
+        grad_b = torch.empty_like(b, dtype=out_dtype)
+    dz_bytes = 0 if activation is None else -(-m * n // 8) * 16
     if "bias" in want:
         grad_bias = torch.empty(n, device=a.device, dtype=torch.float32)
-        workspace = torch.empty((-(-m // 64), n), device=a.device, dtype=torch.float32)
-    if activation is not None or grad_bias is not None:
-        lib.activation_gradient(capi.ACTIVATIONS[activation], grad, preactivation, None if dz is grad else dz, n, grad_bias, workspace)
-    alpha = 1.0 if alpha is None else float(alpha)
-    if "a" in want:
-        grad_a = torch.empty((m, k), device=a.device, dtype=out_dtype)
-        lib.expert_product(capi.ROWS_GRADIENT, name.encode(), dz, b, grad_a, 1, m, n, k, factor=alpha)
-    if "b" in want:
-        grad_b = torch.empty((n, k), device=a.device, dtype=out_dtype)
-        lib.expert_product(capi.WEIGHTS_GRADIENT, name.encode(), dz, a, grad_b, 1, m, n, k, factor=alpha)
+        scratch = torch.empty(dz_bytes + -(-m // 64) * n * 4, device=a.device, dtype=torch.uint8)
+    elif dz_bytes:
+        scratch = torch.empty(dz_bytes, device=a.device, dtype=torch.uint8)
+    dz = 0 if scratch is None else scratch.data_ptr()
+    capi.library("mm").gemm_gradients(
+        capi.OgGemmGradients(
+            grad.data_ptr(), a.data_ptr(), b.data_ptr(), 0 if preactivation is None else preactivation.data_ptr(), dz,
+            0 if grad_a is None else grad_a.data_ptr(), 0 if grad_b is None else grad_b.data_ptr(),
+            0 if grad_bias is None else grad_bias.data_ptr(), dz + dz_bytes, m, n, k, capi.ACTIVATIONS[activation],
+            out_dtype is torch.float32, 1.0 if alpha is None else alpha, name.encode()),
+        a.get_device())
     return grad_a, grad_b, grad_bias
 
 

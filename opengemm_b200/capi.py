@@ -59,6 +59,14 @@ class OgExpertProduct(ctypes.Structure):
                 + [("factor", ctypes.c_float), ("dtype", c_char * 16)])
 
 
+class OgGemmGradients(ctypes.Structure):
+    """The gradients of one product (include/opengemm_b200.h)."""
+
+    _fields_ = ([(f, c_void_p) for f in ("grad", "a", "b", "z", "dz", "grad_a", "grad_b", "grad_bias", "partial")]
+                + [(f, c_int32) for f in ("m", "n", "k", "activation", "out_f32")]
+                + [("factor", ctypes.c_float), ("dtype", c_char * 16)])
+
+
 class OgRoute(ctypes.Structure):
     """How experts are chosen (include/opengemm_b200.h)."""
 
@@ -201,6 +209,7 @@ class Library:
             self._fused.argtypes = [POINTER(OgGemm)] + [c_void_p] * 5 + [c_int32, c_void_p, POINTER(OgEpilogue)]
             for name, argtypes in {
                 "expert_product": [POINTER(OgExpertProduct), c_int32, c_void_p],
+                "gemm_gradients": [POINTER(OgGemmGradients), c_int32, c_void_p],
                 "route": [POINTER(OgRoute)] + [c_void_p] * 4 + [c_int32, c_void_p],
                 "route_gradient": [POINTER(OgRoute)] + [c_void_p] * 4 + [c_int32, c_void_p],
                 "expert_plan": [c_void_p, ctypes.c_int64, c_int32, c_int32] + [c_void_p] * 4 + [c_int32, c_void_p],
@@ -352,66 +361,27 @@ class Library:
         if status != OG_OK:
             raise RuntimeError(self.error())
 
-    def expert_product(self, mode, dtype, x, w, out, groups, rows, n, k, offsets=None, tokens=None, x_rows=0, alpha=None,
-                       activation=0, preactivation=None, factor=1.0):
-        """One launch of og_b200_expert_product on CUDA tensors, on the current stream of `out`'s device."""
+    def expert_product(self, mode, dtype, x, w, out, groups, rows, n, k, offsets=0, tokens=0, x_rows=0, alpha=None,
+                       activation=0, preactivation=None):
+        """One launch of og_b200_expert_product on CUDA tensors, on the current stream of `out`'s
+        device; `offsets` and `tokens` are addresses."""
         device = out.get_device()
         product = OgExpertProduct(
-            x.data_ptr(), w.data_ptr(), 0 if offsets is None else offsets.data_ptr(), 0 if tokens is None else tokens.data_ptr(),
-            0 if alpha is None else alpha.data_ptr(), out.data_ptr(), 0 if preactivation is None else preactivation.data_ptr(),
-            mode, groups, rows, x_rows, n, k, activation, out.dtype is torch.float32, factor, dtype,
+            x.data_ptr(), w.data_ptr(), offsets, tokens, 0 if alpha is None else alpha.data_ptr(), out.data_ptr(),
+            0 if preactivation is None else preactivation.data_ptr(), mode, groups, rows, x_rows, n, k, activation,
+            out.dtype is torch.float32, 1.0, dtype,
         )
         if self._expert_product(byref(product), device, raw_stream(device)) != OG_OK:
             raise RuntimeError(self._experts_error().decode())
 
-    def route(self, how, logits, bias, weights, indices):
-        device = logits.get_device()
-        if self._route(byref(how), logits.data_ptr(), 0 if bias is None else bias.data_ptr(), weights.data_ptr(),
-                       indices.data_ptr(), device, raw_stream(device)) != OG_OK:
-            raise RuntimeError(self._routing_error().decode())
+    def gemm_gradients(self, gradients, device):
+        """The launches of an OgGemmGradients on the current stream of device index `device`."""
+        if self._gemm_gradients(byref(gradients), device, raw_stream(device)) != OG_OK:
+            raise RuntimeError(self._experts_error().decode())
 
-    def route_gradient(self, how, grad_weights, logits, indices, grad_logits):
-        device = logits.get_device()
-        if self._route_gradient(byref(how), grad_weights.data_ptr(), logits.data_ptr(), indices.data_ptr(),
-                                grad_logits.data_ptr(), device, raw_stream(device)) != OG_OK:
-            raise RuntimeError(self._routing_error().decode())
-
-    def expert_plan(self, indices, experts, offsets, tokens, positions, workspace):
-        device = indices.get_device()
-        if self._expert_plan(indices.data_ptr(), indices.size(0), indices.size(1), experts, offsets.data_ptr(),
-                             tokens.data_ptr(), positions.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
-                             device, raw_stream(device)) != OG_OK:
-            raise RuntimeError(self._routing_error().decode())
-
-    def expert_gather(self, x, tokens, row_limit, out):
-        """out[r] = x[tokens[r]] for the rows below the device integer at address `row_limit`."""
-        device = out.get_device()
-        if self._expert_gather(x.data_ptr(), tokens.data_ptr(), row_limit, out.data_ptr(), x.size(1) * x.element_size(),
-                               out.size(0), device, raw_stream(device)) != OG_OK:
-            raise RuntimeError(self._routing_error().decode())
-
-    def expert_combine(self, y, weights, positions, residual, out):
-        device = out.get_device()
-        if self._expert_combine(ELEMENT_TYPES[out.dtype], y.dtype is torch.float32, y.data_ptr(), 0 if weights is None else weights.data_ptr(),
-                                positions.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(),
-                                out.size(0), positions.size(1), out.size(1), device, raw_stream(device)) != OG_OK:
-            raise RuntimeError(self._routing_error().decode())
-
-    def expert_combine_gradient(self, grad, y, weights, positions, grad_y, grad_weights):
-        device = grad.get_device()
-        if self._expert_combine_gradient(ELEMENT_TYPES[grad.dtype], grad.data_ptr(), y.data_ptr(), weights.data_ptr(),
-                                         positions.data_ptr(), grad_y.data_ptr(), grad_weights.data_ptr(), grad.size(0),
-                                         positions.size(1), grad.size(1), device, raw_stream(device)) != OG_OK:
-            raise RuntimeError(self._routing_error().decode())
-
-    def activation_gradient(self, activation, grad, z, dz, n, bias_gradient=None, workspace=None, row_limit=None):
-        """dz = grad * act'(z) (and its column sums); `activation` is a code of the C ABI."""
-        device = grad.get_device()
-        if self._activation_gradient(ELEMENT_TYPES[grad.dtype], activation, grad.data_ptr(), 0 if z is None else z.data_ptr(),
-                                     0 if dz is None else dz.data_ptr(),
-                                     0 if bias_gradient is None else bias_gradient.data_ptr(),
-                                     0 if workspace is None else workspace.data_ptr(),
-                                     0 if row_limit is None else row_limit, grad.size(0), n, device, raw_stream(device)) != OG_OK:
+    def routing(self, call, *args):
+        """One of the routing entry points: `args` up to the device index, then its current stream."""
+        if call(*args, raw_stream(args[-1])) != OG_OK:
             raise RuntimeError(self._routing_error().decode())
 
     def status(self, word):
@@ -493,6 +463,9 @@ def independent_inputs():
 
 def library(impl):
     """The loaded library for `impl`, loading it on first use."""
+    loaded = _libraries.get(impl)
+    if loaded is not None:
+        return loaded
     with _lock:
         if impl not in _libraries:
             _libraries[impl] = Library(impl)

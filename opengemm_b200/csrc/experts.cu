@@ -222,6 +222,34 @@ extern "C" {
 
 OG_API const char* og_b200_experts_error(void) { return experts_error; }
 
+OG_API int32_t og_b200_gemm_gradients(const OgGemmGradients* g, int32_t device, void* stream) {
+  if (!g) return experts_fail(OG_ERR_LAUNCH, "null OgGemmGradients");
+  const bool bf16 = !std::strncmp(g->dtype, "bf16", 16);
+  if (!bf16 && std::strncmp(g->dtype, "f16", 16)) return experts_fail(OG_ERR_LAUNCH, "dtype %.16s is not served: bf16 and f16", g->dtype);
+  if (g->activation < ACT_NONE || g->activation > ACT_SILU) return experts_fail(OG_ERR_LAUNCH, "activation %d is none of 0..%d", g->activation, int(ACT_SILU));
+  if (g->m < 0 || g->n <= 0 || g->k <= 0 || g->n % 8 || g->k % 8) return experts_fail(OG_ERR_LAUNCH, "m = %d, n = %d, k = %d: n and k come in eights", g->m, g->n, g->k);
+  if (g->activation || g->grad_bias) {
+    const int rc = og_b200_activation_gradient(bf16 ? 1 : 2, g->activation, g->grad, g->z, g->dz, g->grad_bias, g->partial, nullptr, g->m, g->n, device, stream);
+    if (rc != OG_OK) return experts_fail(rc, "%s", og_b200_routing_error());
+  }
+  OgExpertProduct product;
+  std::memset(&product, 0, sizeof product);
+  product.x = g->activation ? g->dz : g->grad;
+  product.groups = 1, product.rows = g->m, product.n = g->n, product.k = g->k;
+  product.out_f32 = g->out_f32, product.factor = g->factor;
+  std::memcpy(product.dtype, g->dtype, sizeof product.dtype);
+  if (g->grad_a) {
+    product.mode = MODE_DX, product.w = g->b, product.out = g->grad_a;
+    const int rc = launch_product(product, device, stream);
+    if (rc != OG_OK) return rc;
+  }
+  if (g->grad_b) {
+    product.mode = MODE_DW, product.w = g->a, product.out = g->grad_b;
+    return launch_product(product, device, stream);
+  }
+  return OG_OK;
+}
+
 OG_API int32_t og_b200_expert_product(const OgExpertProduct* product, int32_t device, void* stream) {
   if (!product) return experts_fail(OG_ERR_LAUNCH, "null OgExpertProduct");
   return launch_product(*product, device, stream);

@@ -13,14 +13,15 @@ device.  How many rows each expert gets is known on the device only: nothing
 here synchronises, and all calls can be captured into a CUDA graph.
 """
 
-from dataclasses import dataclass
+from ctypes import byref
 
 import torch
 
 from . import capi
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
-_PRODUCT_TYPES = {torch.bfloat16: b"bf16", torch.float16: b"f16", torch.float8_e4m3fn: b"e4m3"}
+_GRADIENT_TYPES = {torch.bfloat16: b"bf16", torch.float16: b"f16"}
+_PRODUCT_TYPES = {**_GRADIENT_TYPES, torch.float8_e4m3fn: b"e4m3"}
 _ACTIVATIONS = {**capi.ACTIVATIONS, **capi.GATED_ACTIVATIONS}
 _PLAN_CHUNK = 8192  # pairs that a plan takes without a workspace
 # Up to this many rows per expert the forward product gathers tokens itself; with more, the copy
@@ -31,20 +32,20 @@ _GATHER_IN_PRODUCT = 16
 
 
 def _expect(label, t, dtype, shape, device):
-    """Raise unless `t` is a contiguous CUDA tensor of this dtype and shape (None: any extent)."""
-    if not (t.is_cuda and t.device == device and t.dtype is dtype and t.is_contiguous() and t.dim() == len(shape)
-            and all(want is None or want == have for want, have in zip(shape, t.shape))):
-        raise TypeError(f"{label} must be a contiguous {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}"
-                        .replace("None", "any"))
+    """Raise unless `t` is a contiguous CUDA tensor of this dtype and shape."""
+    if not (t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous() and t.is_cuda):
+        raise TypeError(f"{label} must be a contiguous {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _how(logits, top_k, scores, groups, top_groups, group_top, renormalise, scale):
-    if scores not in _SCORES:
+    sigmoid = _SCORES.get(scores)
+    if sigmoid is None:
         raise TypeError(f"scores must be one of {list(_SCORES)}, got {scores!r}")
-    if not (logits.is_cuda and logits.dim() == 2 and logits.is_contiguous() and logits.dtype in capi.ELEMENT_TYPES):
+    dtype = capi.ELEMENT_TYPES.get(logits.dtype)
+    if dtype is None or not (logits.is_cuda and logits.dim() == 2 and logits.is_contiguous()):
         raise TypeError("logits must be a contiguous 2-D CUDA tensor of float32, bfloat16 or float16")
-    return capi.OgRoute(logits.size(0), capi.ELEMENT_TYPES[logits.dtype], logits.size(1), top_k, _SCORES[scores], groups,
-                        top_groups, group_top, bool(renormalise), scale)
+    tokens, experts = logits.shape
+    return capi.OgRoute(tokens, dtype, experts, top_k, sigmoid, groups, top_groups, group_top, bool(renormalise), scale)
 
 
 def route(logits, top_k, scores="softmax", bias=None, groups=1, top_groups=1, group_top=2, renormalise=True, scale=1.0):
@@ -71,10 +72,12 @@ def route(logits, top_k, scores="softmax", bias=None, groups=1, top_groups=1, gr
     """
     how = _how(logits, top_k, scores, groups, top_groups, group_top, renormalise, scale)
     if bias is not None:
-        _expect("bias", bias, torch.float32, (logits.size(1),), logits.device)
-    weights = torch.empty((logits.size(0), top_k), device=logits.device, dtype=torch.float32)
-    indices = torch.empty((logits.size(0), top_k), device=logits.device, dtype=torch.int32)
-    capi.library("mm").route(how, logits, bias, weights, indices)
+        _expect("bias", bias, torch.float32, (how.experts,), logits.device)
+    weights = logits.new_empty((how.tokens, max(top_k, 0)), dtype=torch.float32)
+    indices = torch.empty_like(weights, dtype=torch.int32)
+    lib = capi.library("mm")
+    lib.routing(lib._route, byref(how), logits.data_ptr(), 0 if bias is None else bias.data_ptr(), weights.data_ptr(),
+                indices.data_ptr(), logits.get_device())
     return weights, indices
 
 
@@ -85,14 +88,15 @@ def route_backward(grad_weights, logits, indices, scores="softmax", renormalise=
     `scores`, `renormalise` and `scale` those it was called with.
     """
     how = _how(logits, indices.size(1) if indices.dim() == 2 else 0, scores, 1, 1, 1, renormalise, scale)
-    _expect("indices", indices, torch.int32, (logits.size(0), None), logits.device)
-    _expect("grad_weights", grad_weights, torch.float32, tuple(indices.shape), logits.device)
+    _expect("indices", indices, torch.int32, (how.tokens, how.top_k), logits.device)
+    _expect("grad_weights", grad_weights, torch.float32, (how.tokens, how.top_k), logits.device)
     grad = torch.empty_like(logits)
-    capi.library("mm").route_gradient(how, grad_weights, logits, indices, grad)
+    lib = capi.library("mm")
+    lib.routing(lib._route_gradient, byref(how), grad_weights.data_ptr(), logits.data_ptr(), indices.data_ptr(),
+                grad.data_ptr(), logits.get_device())
     return grad
 
 
-@dataclass(frozen=True)
 class ExpertPlan:
     """Where every (token, choice) pair's row is, in order of the experts.
 
@@ -100,18 +104,33 @@ class ExpertPlan:
     tokens; `tokens[row]` is a row's token and `positions[t, j]` the row of token
     t's choice j, or -1 for an index outside 0 .. experts - 1.  With such
     indices there are fewer than `rows` rows; what lies behind the last one is
-    neither read nor written.
+    neither read nor written.  The three int32 tensors are views of one buffer.
     """
 
-    offsets: torch.Tensor
-    tokens: torch.Tensor
-    positions: torch.Tensor
-    experts: int
+    __slots__ = ("experts", "token_count", "top_k", "rows", "device", "_store", "_offsets", "_tokens", "_positions", "_limit")
+
+    def __init__(self, indices, experts):
+        self.experts, self.device = experts, indices.device
+        self.token_count, self.top_k = indices.shape
+        rows = self.rows = self.token_count * self.top_k  # of the tensors in the plan's order
+        self._store = torch.empty(experts + 1 + 2 * rows, device=indices.device, dtype=torch.int32)
+        # addresses that the launches take: the first rows (and, behind the last of them, how many rows there are) ...
+        self._offsets = self._store.data_ptr()
+        self._limit = self._offsets + 4 * experts
+        self._tokens = self._limit + 4
+        self._positions = self._tokens + 4 * rows
 
     @property
-    def rows(self):
-        """Rows of the tensors in the plan's order: tokens x top_k."""
-        return self.tokens.size(0)
+    def offsets(self):
+        return self._store[:self.experts + 1]
+
+    @property
+    def tokens(self):
+        return self._store[self.experts + 1:self.experts + 1 + self.rows]
+
+    @property
+    def positions(self):
+        return self._store[self.experts + 1 + self.rows:].view(self.token_count, self.top_k)
 
 
 def expert_plan(indices, experts):
@@ -125,34 +144,34 @@ def expert_plan(indices, experts):
     Returns:
         An `ExpertPlan`; the same indices always give the same plan.
     """
-    if not (indices.is_cuda and indices.dim() == 2 and indices.is_contiguous() and indices.dtype is torch.int32):
+    if not (indices.dtype is torch.int32 and indices.is_cuda and indices.dim() == 2 and indices.is_contiguous()):
         raise TypeError("indices must be a contiguous 2-D int32 CUDA tensor")
     if indices.size(1) < 1:
         raise ValueError("indices must name at least one expert per token")
-    pairs, device = indices.numel(), indices.device
-    offsets = torch.empty(experts + 1, device=device, dtype=torch.int32)
-    tokens = torch.empty(pairs, device=device, dtype=torch.int32)
-    positions = torch.empty(indices.shape, device=device, dtype=torch.int32)
+    if not 1 <= experts <= 1024:
+        raise ValueError(f"{experts} experts: 1 to 1024 are served")
+    plan = ExpertPlan(indices, experts)
     workspace = None
-    if pairs > _PLAN_CHUNK:
-        workspace = torch.empty(-(-pairs // _PLAN_CHUNK) * experts, device=device, dtype=torch.int32)
-    capi.library("mm").expert_plan(indices, experts, offsets, tokens, positions, workspace)
-    return ExpertPlan(offsets, tokens, positions, experts)
+    if plan.rows > _PLAN_CHUNK:
+        workspace = torch.empty(-(-plan.rows // _PLAN_CHUNK) * experts, device=indices.device, dtype=torch.int32)
+    lib = capi.library("mm")
+    lib.routing(lib._expert_plan, indices.data_ptr(), plan.token_count, plan.top_k, experts, plan._offsets, plan._tokens,
+                plan._positions, 0 if workspace is None else workspace.data_ptr(), indices.get_device())
+    return plan
 
 
 def _check_product(x, w, plan, gather, activation, types):
     """The checks that a product and its gradients share; returns (name, n, k, gated)."""
-    name = _PRODUCT_TYPES.get(x.dtype)
-    if name is None or x.dtype not in types:
+    name = types.get(x.dtype)
+    if name is None:
         raise TypeError(f"x is {x.dtype}: served are {[str(t) for t in types]}")
     if w.dim() != 3:
         raise TypeError(f"w must be [experts, N, K], got {list(w.shape)}")
     experts, n, k = w.shape
-    device = plan.offsets.device
     if experts != plan.experts:
         raise ValueError(f"w has {experts} experts and the plan {plan.experts}")
-    _expect("x", x, x.dtype, (plan.positions.size(0) if gather else plan.rows, k), device)
-    _expect("w", w, x.dtype, (experts, n, k), device)
+    _expect("x", x, x.dtype, (plan.token_count if gather else plan.rows, k), plan.device)
+    _expect("w", w, x.dtype, (experts, n, k), plan.device)
     if activation not in _ACTIVATIONS:
         raise TypeError(f"activation must be one of {[a for a in _ACTIVATIONS if a]}, got {activation!r}")
     gated = activation in capi.GATED_ACTIVATIONS
@@ -160,9 +179,8 @@ def _check_product(x, w, plan, gather, activation, types):
     if not n or not k or k % multiple or (gated and n % 16):
         raise ValueError(f"K must be a positive multiple of {multiple} (got {k}) and N positive, a multiple of 16 "
                          f"with a gated activation (got {n})")
-    for label, t in (("x", x), ("w", w)):
-        if t.data_ptr() % 16:
-            raise ValueError(f"{label} must start on a 16-byte boundary")
+    if (x.data_ptr() | w.data_ptr()) % 16:
+        raise ValueError("x and w must start on 16-byte boundaries")
     return name, n, k, gated
 
 
@@ -190,8 +208,8 @@ def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None,
         `(plan.rows, N or N / 2)` rows in the plan's order.  Rows behind the plan's
         last are left as they were.
     """
-    name, n, k, gated = _check_product(x, w, plan, gather, activation, tuple(_PRODUCT_TYPES))
-    device, rows = x.device, plan.rows
+    name, n, k, gated = _check_product(x, w, plan, gather, activation, _PRODUCT_TYPES)
+    device, rows = plan.device, plan.rows
     width = n // 2 if gated else n
     own = torch.bfloat16 if x.dtype is torch.float8_e4m3fn else x.dtype
     if out_dtype not in (None, own):
@@ -205,18 +223,28 @@ def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None,
     if alpha is not None:
         _expect("alpha", alpha, torch.float32, (plan.experts,), device)
     if gather and rows > _GATHER_IN_PRODUCT * min(plan.experts, rows):
-        x, gather = _sorted_rows(x, plan), False
+        x, gather = _sorted_rows(x, plan, k), False
     capi.library("mm").expert_product(
-        capi.FORWARD, name, x, w, out, plan.experts, rows, n, k, plan.offsets, plan.tokens if gather else None,
-        x.size(0), alpha, _ACTIVATIONS[activation], preactivation)
+        capi.FORWARD, name, x, w, out, plan.experts, rows, n, k, plan._offsets, plan._tokens if gather else 0,
+        plan.token_count, alpha, _ACTIVATIONS[activation], preactivation)
     return out
 
 
-def _sorted_rows(x, plan):
+def _sorted_rows(x, plan, k):
     """The tokens' rows in the plan's order."""
-    rows = torch.empty((plan.rows, x.size(1)), device=x.device, dtype=x.dtype)
-    capi.library("mm").expert_gather(x, plan.tokens, plan.offsets.data_ptr() + 4 * plan.experts, rows)
+    rows = x.new_empty((plan.rows, k))
+    lib = capi.library("mm")
+    lib.routing(lib._expert_gather, x.data_ptr(), plan._tokens, plan._limit, rows.data_ptr(), k * x.element_size(), plan.rows,
+                x.get_device())
     return rows
+
+
+def _combine(y, weights, plan, residual, out, n):
+    """The launch of `expert_combine`; `weights` None: ones; `y` may be float32."""
+    lib = capi.library("mm")
+    lib.routing(lib._expert_combine, capi.ELEMENT_TYPES[out.dtype], y.dtype is torch.float32, y.data_ptr(),
+                0 if weights is None else weights.data_ptr(), plan._positions, 0 if residual is None else residual.data_ptr(),
+                out.data_ptr(), plan.token_count, plan.top_k, n, out.get_device())
 
 
 def expert_gemm_backward(grad, x, w, plan, gather=False, activation=None, preactivation=None, want=("x", "w"), out_dtype=None):
@@ -240,7 +268,7 @@ def expert_gemm_backward(grad, x, w, plan, gather=False, activation=None, preact
     Returns:
         `(grad_x, grad_w)`, None in the place of what is not wanted.
     """
-    name, n, k, gated = _check_product(x, w, plan, gather, activation, (torch.bfloat16, torch.float16))
+    name, n, k, gated = _check_product(x, w, plan, gather, activation, _GRADIENT_TYPES)
     if n % 8:
         raise ValueError(f"N must be a multiple of 8, got {n}")
     if not set(want) <= {"x", "w"}:
@@ -249,7 +277,7 @@ def expert_gemm_backward(grad, x, w, plan, gather=False, activation=None, preact
         raise TypeError("an activation and its preactivation come together")
     if out_dtype not in (None, x.dtype, torch.float32):
         raise TypeError(f"gradients leave as {x.dtype} or torch.float32, not {out_dtype}")
-    device, rows = x.device, plan.rows
+    device, rows = plan.device, plan.rows
     _expect("grad", grad, x.dtype, (rows, n // 2 if gated else n), device)
     if preactivation is not None:
         _expect("preactivation", preactivation, x.dtype, (rows, n), device)
@@ -260,20 +288,20 @@ def expert_gemm_backward(grad, x, w, plan, gather=False, activation=None, preact
     dz = grad
     if activation is not None:
         dz = torch.empty_like(preactivation)
-        lib.activation_gradient(_ACTIVATIONS[activation], grad, preactivation, dz, n,
-                                row_limit=plan.offsets.data_ptr() + 4 * plan.experts)
+        lib.routing(lib._activation_gradient, capi.ELEMENT_TYPES[x.dtype], _ACTIVATIONS[activation], grad.data_ptr(),
+                    preactivation.data_ptr(), dz.data_ptr(), 0, 0, plan._limit, rows, n, x.get_device())
     grad_x = grad_w = None
     if "x" in want:
         # a token's rows are added before anything is rounded
         grad_x = torch.empty((rows, k), device=device, dtype=torch.float32 if gather else out_dtype or x.dtype)
-        lib.expert_product(capi.ROWS_GRADIENT, name, dz, w, grad_x, plan.experts, rows, n, k, plan.offsets)
+        lib.expert_product(capi.ROWS_GRADIENT, name, dz, w, grad_x, plan.experts, rows, n, k, plan._offsets)
         if gather:
             by_row, grad_x = grad_x, torch.empty_like(x)
-            lib.expert_combine(by_row, None, plan.positions, None, grad_x)
+            _combine(by_row, None, plan, None, grad_x, k)
     if "w" in want:
-        grad_w = torch.empty(w.shape, device=device, dtype=out_dtype or x.dtype)
-        sorted_x = _sorted_rows(x, plan) if gather else x
-        lib.expert_product(capi.WEIGHTS_GRADIENT, name, dz, sorted_x, grad_w, plan.experts, rows, n, k, plan.offsets)
+        grad_w = torch.empty_like(w, dtype=out_dtype or x.dtype)
+        sorted_x = _sorted_rows(x, plan, k) if gather else x
+        lib.expert_product(capi.WEIGHTS_GRADIENT, name, dz, sorted_x, grad_w, plan.experts, rows, n, k, plan._offsets)
     return grad_x, grad_w
 
 
@@ -290,20 +318,28 @@ def expert_combine(y, weights, plan, residual=None, out=None):
     Returns:
         `(tokens, N)` of y's dtype, summed in float32 in the order of the choices.
     """
-    device = plan.offsets.device
-    if y.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"y is {y.dtype}: bfloat16 and float16 are served")
-    _expect("y", y, y.dtype, (plan.rows, None), device)
-    _expect("weights", weights, torch.float32, tuple(plan.positions.shape), device)
-    shape = (plan.positions.size(0), y.size(1))
+    n = _check_combine(y, weights, plan)
+    shape = (plan.token_count, n)
     if residual is not None:
-        _expect("residual", residual, y.dtype, shape, device)
+        _expect("residual", residual, y.dtype, shape, plan.device)
     if out is None:
-        out = torch.empty(shape, device=device, dtype=y.dtype)
+        out = y.new_empty(shape)
     else:
-        _expect("out", out, y.dtype, shape, device)
-    capi.library("mm").expert_combine(y, weights, plan.positions, residual, out)
+        _expect("out", out, y.dtype, shape, plan.device)
+    _combine(y, weights, plan, residual, out, n)
     return out
+
+
+def _check_combine(y, weights, plan):
+    """The checks that the combination and its gradient share; returns its columns."""
+    if y.dtype not in _GRADIENT_TYPES:
+        raise TypeError(f"y is {y.dtype}: bfloat16 and float16 are served")
+    if y.dim() != 2 or y.size(1) < 1:
+        raise TypeError(f"y must be [rows, N], got {list(y.shape)}")
+    n = y.size(1)
+    _expect("y", y, y.dtype, (plan.rows, n), plan.device)
+    _expect("weights", weights, torch.float32, (plan.token_count, plan.top_k), plan.device)
+    return n
 
 
 def expert_combine_backward(grad, y, weights, plan):
@@ -314,12 +350,10 @@ def expert_combine_backward(grad, y, weights, plan):
     holds `<grad[t], y[row of (t, j)]>`, 0 for a pair that goes nowhere.  The
     residual's gradient is `grad` itself.
     """
-    device = plan.offsets.device
-    if y.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"y is {y.dtype}: bfloat16 and float16 are served")
-    _expect("y", y, y.dtype, (plan.rows, None), device)
-    _expect("weights", weights, torch.float32, tuple(plan.positions.shape), device)
-    _expect("grad", grad, y.dtype, (plan.positions.size(0), y.size(1)), device)
+    n = _check_combine(y, weights, plan)
+    _expect("grad", grad, y.dtype, (plan.token_count, n), plan.device)
     grad_y, grad_weights = torch.empty_like(y), torch.empty_like(weights)
-    capi.library("mm").expert_combine_gradient(grad, y, weights, plan.positions, grad_y, grad_weights)
+    lib = capi.library("mm")
+    lib.routing(lib._expert_combine_gradient, capi.ELEMENT_TYPES[y.dtype], grad.data_ptr(), y.data_ptr(), weights.data_ptr(),
+                plan._positions, grad_y.data_ptr(), grad_weights.data_ptr(), plan.token_count, plan.top_k, n, y.get_device())
     return grad_y, grad_weights

@@ -258,7 +258,7 @@ def test_refusals():
         og.route(torch.zeros(1, 1025, device="cuda"), 2)
     with pytest.raises(TypeError, match="indices"):
         og.expert_plan(torch.zeros(4, 2, device="cuda", dtype=torch.int64), 4)
-    with pytest.raises(RuntimeError, match="1024"):
+    with pytest.raises(ValueError, match="1024"):
         og.expert_plan(torch.zeros(4, 2, device="cuda", dtype=torch.int32), 1025)
     weights, indices = og.route(x, 2)
     plan = og.expert_plan(indices, 16)
