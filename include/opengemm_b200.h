@@ -189,7 +189,8 @@ OG_API int32_t og_b200_launch_quantized(const OgGemm* g, const void* a, const vo
  * may be C itself, `preactivation` starts on a 16-byte boundary.  Float formats only.
  * With `out_format` the activation's value leaves block-scaled as in
  * og_b200_launch_quantized (no residual or pre-activation then).  Launches run the
- * static schedule: split_k, cluster_k, use_clc and walk of `g` are not followed. */
+ * static schedule without an operand swap: split_k, cluster_k, use_clc, walk and swap_ab
+ * of `g` are not followed.  Up to four rows of 16-bit operands take a kernel of their own. */
 typedef struct OgEpilogue {
   const void* bias;     /* float32 [n], or null */
   const void* residual; /* or null */

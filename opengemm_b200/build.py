@@ -33,7 +33,7 @@ LIB_DIR = PACKAGE / "lib"
 LIB_NAME = "libopengemm_b200.so"
 UNITS = ("host", "kernels_dense", "kernels_scaled", "kernels_fixed_dense", "kernels_fixed_scaled",
          "kernels_plain_dense", "kernels_plain_scaled", "kernels_fused_dense", "kernels_fused_scaled", "no_alloc",
-         "quantize", "experts", "experts_forward16", "experts_forward8", "experts_gradient", "routing")
+         "quantize", "experts", "experts_forward16", "experts_forward8", "experts_gradient", "routing", "skinny")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", *ARCH, "-Xcompiler", "-fPIC,-fvisibility=hidden"]

@@ -3,12 +3,12 @@
 // silu and the tanh form of gelu are one expression, x * sigmoid(a x + b x^3):
 // (a, b) = (1, 0) and 2 sqrt(2/pi) (1, 0.044715), since (1 + tanh u) / 2 =
 // sigmoid(2u).  The epilogues therefore carry the two coefficients at run time
-// and compile one code path for both.  gelu itself is x * Phi(x); Phi(-|x|)
-// comes from Abramowitz and Stegun, Handbook of Mathematical Functions,
-// 7.1.26 (|error| <= 1.5e-7 in erf), whose exponential the derivative shares.
-// Both need two special-function instructions a value; a call of erff or tanhf
-// would be two to three times the instructions, and the four epilogue warps
-// have to keep up with the tensor pipe.
+// (times -log2(e), for the base-2 exponential) and compile one code path for
+// both.  gelu itself is x * Phi(x); Phi(-|x|) comes from Abramowitz and Stegun,
+// Handbook of Mathematical Functions, 7.1.26 (|error| <= 1.5e-7 in erf), whose
+// exponential the derivative shares.  Each needs two special-function
+// instructions and 6 to 12 others a value: the epilogue's warps have to keep up
+// with the tensor pipe, and a call of erff or tanhf is two to three times that.
 #pragma once
 
 #include <cstdint>
@@ -26,45 +26,58 @@ enum Activation : int {
   ACT_GEGLU = 6,   // gelu(gate) * up, likewise
 };
 
-constexpr float SIGMOID_TANH_A = 1.5957691216057308f;   // 2 sqrt(2 / pi)
-constexpr float SIGMOID_TANH_B = 0.07135481282553488f;  // 2 sqrt(2 / pi) * 0.044715
+constexpr double LOG2_E = 1.4426950408889634;
+constexpr double TANH_A = 1.5957691216057308;  // 2 sqrt(2 / pi)
 
 #ifdef __CUDACC__
 
 // Shape of the code an activation runs: none, relu, x * Phi(x), x * sigmoid(a x + b x^3).
 enum ActShape : int { SHAPE_NONE = 0, SHAPE_RELU = 1, SHAPE_PHI = 2, SHAPE_SIGMOID = 3 };
 
-__device__ __forceinline__ float sigmoid_of(float t) { return __fdividef(1.0f, 1.0f + __expf(-t)); }
+// 2^x and 1 / x to within 2 units and 1 unit of the last place; results and
+// arguments below the normal range are zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float reciprocal_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
-// Phi(-|x|) and, through `density`, exp(-x^2 / 2).
+// sigmoid(t) for the coefficients of -log2(e) t = a x + b x^3.  The square is capped
+// far past saturation, so that an infinite x times b = 0 makes no NaN.
+__device__ __forceinline__ float gate_of(float x, float a, float b) {
+  return reciprocal_fast(1.0f + exp2_fast(x * fmaf(b, fminf(x * x, 1e8f), a)));
+}
+
+// Phi(-|x|), and exp(-x^2 / 2) through `density`.
 __device__ __forceinline__ float lower_tail(float x, float* density) {
-  const float y = fabsf(x) * 0.7071067811865476f;
-  const float t = __fdividef(1.0f, fmaf(0.3275911f, y, 1.0f));
-  const float e = __expf(-0.5f * x * x);
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
+  const float t = reciprocal_fast(fmaf(0.3275911f * 0.7071067811865476f, fabsf(x), 1.0f));
+  const float e = exp2_fast(x * x * -0.7213475204444817f);  // -log2(e) / 2
+  float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  p = fmaf(p, t, 0.5f * 1.421413741f);
+  p = fmaf(p, t, 0.5f * -0.284496736f);
+  p = fmaf(p, t, 0.5f * 0.254829592f);
   *density = e;
-  return 0.5f * p * t * e;
+  return p * t * e;
 }
-
-__device__ __forceinline__ float act_phi(float x) {
-  float e;
-  const float tail = lower_tail(x, &e);
-  return x * (x > 0.0f ? 1.0f - tail : tail);
-}
-
-// sigmoid(a x + b x^3).  The square is capped far past saturation, so that an infinite x
-// times b = 0 makes no NaN.
-__device__ __forceinline__ float gate_of(float x, float a, float b) { return sigmoid_of(x * fmaf(b, fminf(x * x, 1e8f), a)); }
 
 template <int SHAPE>
 __device__ __forceinline__ float act_value(float x, float a, float b) {
-  if constexpr (SHAPE == SHAPE_RELU) return x < 0.0f ? 0.0f : x;  // keeps a NaN
-  else if constexpr (SHAPE == SHAPE_PHI) return act_phi(x);
-  else if constexpr (SHAPE == SHAPE_SIGMOID) return x * gate_of(x, a, b);
-  else return x;
+  if constexpr (SHAPE == SHAPE_RELU) {
+    return x < 0.0f ? 0.0f : x;  // keeps a NaN
+  } else if constexpr (SHAPE == SHAPE_PHI) {
+    // x Phi(x) = max(x, 0) - |x| Phi(-|x|); the cap keeps infinity times zero out
+    float e;
+    return fmaf(-fminf(fabsf(x), 1e4f), lower_tail(x, &e), fmaxf(x, 0.0f));
+  } else if constexpr (SHAPE == SHAPE_SIGMOID) {
+    return x * gate_of(x, a, b);
+  } else {
+    return x;
+  }
 }
 
 // The activation and its derivative at x.
@@ -80,9 +93,11 @@ __device__ __forceinline__ void act_both(float x, float a, float b, float* value
     *value = x * cdf;
     *slope = fmaf(x * 0.3989422804014327f, e, cdf);
   } else if constexpr (SHAPE == SHAPE_SIGMOID) {
-    const float p = gate_of(x, a, b);
+    // p' = p (1 - p) t' with t' = -ln(2) (a + 3 b x^2)
+    const float q = fminf(x * x, 1e8f);
+    const float p = reciprocal_fast(1.0f + exp2_fast(x * fmaf(b, q, a)));
     *value = x * p;
-    *slope = fmaf(x * p * (1.0f - p), fmaf(3.0f * b, fminf(x * x, 1e8f), a), p);
+    *slope = fmaf(x * p * (1.0f - p), -0.6931471805599453f * fmaf(3.0f * b, q, a), p);
   } else {
     *value = x;
     *slope = 1.0f;
@@ -97,8 +112,8 @@ inline void act_constants(int activation, int* shape, float* a, float* b) {
   switch (activation) {
     case ACT_RELU: *shape = 1; break;
     case ACT_GELU: case ACT_GEGLU: *shape = 2; break;
-    case ACT_GELU_TANH: *shape = 3, *a = SIGMOID_TANH_A, *b = SIGMOID_TANH_B; break;
-    case ACT_SILU: case ACT_SWIGLU: *shape = 3, *a = 1.0f; break;
+    case ACT_GELU_TANH: *shape = 3, *a = float(-LOG2_E * TANH_A), *b = float(-LOG2_E * TANH_A * 0.044715); break;
+    case ACT_SILU: case ACT_SWIGLU: *shape = 3, *a = float(-LOG2_E); break;
     default: *shape = 0;
   }
 }

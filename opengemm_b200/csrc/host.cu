@@ -24,6 +24,7 @@
 #include "kernels_fixed.cuh"
 #include "launch_common.h"
 #include "plan.h"
+#include "skinny.h"
 
 namespace og {
 
@@ -338,6 +339,13 @@ int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* str
     on_static_schedule = *g;
     on_static_schedule.cluster_k = 1, on_static_schedule.split_k = 1, on_static_schedule.use_clc = 0;
     on_static_schedule.walk = 0;
+    if (g->swap_ab) {
+      // A's few rows are the MMA's 128 (what is past them is not fetched), B's rows
+      // its N side, in tiles just wide enough that one wave of CTAs covers them.
+      on_static_schedule.swap_ab = 0, on_static_schedule.use_2cta = 0, on_static_schedule.cluster_m = 1;
+      on_static_schedule.row = g->row & ~1;  // variants come in pairs: one CTA, two
+      on_static_schedule.output_n = std::min(256, std::max(32, round_up(ceil_div(g->n, 148), 16)));
+    }
     g = &on_static_schedule;
   }
   if (!plan_memo.valid || std::memcmp(&plan_memo.key, g, sizeof(OgGemm)) != 0) {
@@ -353,6 +361,16 @@ int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* str
   char why[320];
   if (want_scaled >= 0 && int(p.format->scaled) != want_scaled)
     return fail(OG_ERR_LAUNCH, "dtype %.16s does not belong to this library", g->dtype);
+  static const bool pdl_enabled = [] { const char* e = getenv("OPENGEMM_PDL"); return !(e && e[0] == '0'); }();
+  if (fused && skinny_serves(*g, *p.format, io)) {
+    const int rc = check_pointers(*g, p, io, alpha, why, sizeof why);
+    if (rc != OG_OK) return fail(rc, "%s", why);
+    const int followed = follow_device(device);
+    if (followed != OG_OK) return followed;
+    const cudaError_t launched = launch_skinny(*g, *p.format, io, alpha, pdl_enabled, sm_count_of(device), static_cast<cudaStream_t>(stream));
+    if (launched != cudaSuccess) return fail(OG_ERR_LAUNCH, "kernel launch failed: %s", cudaGetErrorString(launched));
+    return OG_OK;
+  }
   const unsigned long long wait_limit = current_wait_limit_ns();
   if (!params_memo) params_memo.reset(new ParamsMemo[1u << PARAMS_MEMO_BITS]());
   ParamsMemo& memo =
@@ -381,7 +399,6 @@ int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* str
     params.tx_bytes += overcredit_next;
     overcredit_next = 0;
   }
-  static const bool pdl_enabled = [] { const char* e = getenv("OPENGEMM_PDL"); return !(e && e[0] == '0'); }();
   params.pdl = pdl_enabled ? (independent_inputs.load(std::memory_order_relaxed) ? 2 : 1) : 0;
 
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -316,7 +316,7 @@ __device__ __forceinline__ void fold_features_off(GemmParams& p) {
 
 // A fused launch runs the static schedule in the default walk: what its kernel leaves out.
 __device__ __forceinline__ void fold_schedules_off(GemmParams& p) {
-  p.walk = 0, p.use_clc = 0, p.stream_k = 0, p.cluster_k = 1;
+  p.walk = 0, p.use_clc = 0, p.stream_k = 0, p.cluster_k = 1, p.transpose_out = 0;
 }
 #endif
 
@@ -348,11 +348,13 @@ __device__ __forceinline__ void store_quantized(const GemmParams& p, const float
 // The fused epilogue's warps (2 .. 9) of one CTA:
 //   z = alpha * acc + bias,  preact = z,  C = act(z) + residual
 // in float32, each tensor rounded once.  A warp works on 32 rows x 32 columns
-// at a time.  The residual comes in as whole row segments (64 or 128 bytes a
-// row, asked for one chunk ahead and before the accumulator is waited for) and
-// reaches the lane of its row through the warp's staging buffer, the way C goes
-// out; rows that are not whole 16-byte units pass through the buffer element by
-// element.  Two accumulator slots let the next tile's MMAs run meanwhile.
+// at a time.  The next chunk's accumulators and residual (each lane its own
+// row's 64 or 128 bytes) are asked for while the current one is worked on, the
+// first residual before the accumulator is waited for.  C leaves as whole row
+// segments through the warp's staging buffer; rows that are not whole 16-byte
+// units pass through it element by element, both ways.  Two accumulator slots
+// let the next tile's MMAs run meanwhile, and a slot is handed back as soon as
+// its last columns are in registers.
 template <int CTA_GROUP, int OUT_BYTES>
 __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCtx& ctx, uint32_t staging, uint32_t bar_acc_full,
                                                uint32_t bar_acc_empty, uint32_t tmem_base, uint32_t rank, int cluster_id, int num_clusters,
@@ -360,6 +362,7 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
   constexpr int TILE_M = 128 * CTA_GROUP, CHUNK = FUSED_CHUNK;
   constexpr int ROW_BYTES = CHUNK * OUT_BYTES, UNITS = ROW_BYTES / 16;  // of a staging row: 4 or 8
   constexpr int ROWS_AT_ONCE = 32 / UNITS, STEPS = 32 / ROWS_AT_ONCE, UNIT = 16 / OUT_BYTES;
+  constexpr int STRIDE = epilogue_warps(true) / 4 * CHUNK;  // from one of a warp's chunks to its next
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
   const int chunk0 = ((warp - 2) >> 2) * CHUNK;
   const uint32_t buf = staging + (warp - 2) * 32 * ROW_BYTES;
@@ -369,15 +372,14 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
   auto at_unit = [&](int r, int u) { return buf + r * ROW_BYTES + ((u ^ (UNITS == 8 ? r & 7 : (r >> 1) & 3)) << 4); };
   auto at_element = [&](int r, int e) { return at_unit(r, e / UNIT) + (e % UNIT) * OUT_BYTES; };
   const int tile_n = p.tile_n, rows_m = p.rows_m, rows_n = p.rows_n, ldd = p.ldd;
-  const bool transposed = p.transpose_out != 0, vec_ok = p.vec_ok != 0, out_f16 = p.out_f16 != 0;
+  const bool vec_ok = p.vec_ok != 0, out_f16 = p.out_f16 != 0;
   const uint8_t* const residual = static_cast<const uint8_t*>(p.residual);
-  const bool residual_vec = residual && p.residual_vec && !transposed;
+  const bool residual_vec = residual && p.residual_vec;
   const float* const bias = p.bias;
   const bool bias_vec = bias && (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
   const float alpha = p.scale_out ? p.alpha : 1.0f;
   const uint32_t acc_empty_leader = CTA_GROUP == 2 ? map_to_cta(bar_acc_empty, 0) : bar_acc_empty;
   auto pack2 = [&](float lo, float hi) { return out_f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
-  auto widen = [&](uint32_t bits) { return out_f16 ? half_bits_to_float(bits) : __uint_as_float(bits << 16); };
   if (p.pdl) pdl_wait_prior_grids();
   int tile_idx = 0;
   for (int tile = cluster_id; __all_sync(0xFFFFFFFFu, allocated) && tile < p.num_tiles; tile += num_clusters, ++tile_idx) {
@@ -385,24 +387,17 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
     const int row0 = t.mi * TILE_M + int(rank) * 128 + quarter * 32, row = row0 + lane;
     const int col0 = t.ni * tile_n;
     const int rows = min(32, rows_m - row0);  // of this warp, none or fewer at C's edge
-    uint4 res[STEPS];
+    uint4 res[UNITS];
+    auto live = [&](int c) { return c < tile_n && col0 + c < rows_n && rows > 0; };
     auto whole = [&](int c) { return c + CHUNK <= tile_n && col0 + c + CHUNK <= rows_n; };
     auto ask_residual = [&](int c) {
-      if (!residual_vec || !whole(c)) return;
-      const uint8_t* src = residual + (size_t(row0 + sub_row) * ldd + col0 + c) * OUT_BYTES + unit * 16;
+      if (!residual_vec || !whole(c) || lane >= rows) return;
+      const uint4* src = reinterpret_cast<const uint4*>(residual + (size_t(row) * ldd + col0 + c) * OUT_BYTES);
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i)
-        if (i * ROWS_AT_ONCE + sub_row < rows) res[i] = *reinterpret_cast<const uint4*>(src + size_t(i * ROWS_AT_ONCE) * ldd * OUT_BYTES);
+      for (int u = 0; u < UNITS; ++u) res[u] = src[u];
     };
     ask_residual(chunk0);
-    if (transposed && row < rows_m) {  // few rows of C, this lane's column of each
-      if (bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + row));
-      if (residual)
-        for (int j = chunk0; j < min(chunk0 + CHUNK, min(tile_n, rows_n - col0)); ++j)
-          asm volatile("prefetch.global.L1 [%0];" ::"l"(residual + (size_t(col0 + j) * ldd + row) * OUT_BYTES));
-    } else if (bias) {
-      asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + min(col0 + lane * 8, rows_n - 1)));
-    }
+    if (bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + min(col0 + lane * 8, rows_n - 1)));
     const int slot = (p.acc_slots == 2) ? (tile_idx & 1) : 0;
     const uint32_t use = (p.acc_slots == 2) ? (tile_idx >> 1) : tile_idx;
     const bool ready = mbar_wait(bar_acc_full + 8 * slot, use & 1, ctx, SITE_EPI_ACC_FULL);
@@ -413,26 +408,15 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CTA_GROUP == 2) mbar_arrive_cluster(acc_empty_leader + 8 * slot);
+        // Relaxed: what is handed back is tensor memory, whose loads have completed;
+        // a release would wait for this warp's stores of C as well.
+        if constexpr (CTA_GROUP == 2) mbar_arrive_cluster_relaxed(acc_empty_leader + 8 * slot);
         else mbar_arrive(bar_acc_empty + 8 * slot);
       }
     };
     // A chunk of this warp's rows, as rounded words or values in each lane, to `base`.
     auto store = [&](const float* v, uint8_t* base, int c, int width) {
       const int gc = col0 + c;
-      if (transposed) {  // this lane's MMA row is a column of C: a warp writes consecutive elements
-        if (row < rows_m) {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) {
-            if (j < width && gc + j < rows_n) {
-              const size_t at = size_t(gc + j) * ldd + row;
-              if constexpr (OUT_BYTES == 4) reinterpret_cast<float*>(base)[at] = v[j];
-              else reinterpret_cast<uint16_t*>(base)[at] = uint16_t(pack2(v[j], 0.0f) & 0xFFFFu);
-            }
-          }
-        }
-        return;
-      }
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
         uint32_t q[4];
@@ -463,41 +447,42 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
       __syncwarp();
     };
 
-    bool handed_back = false;
-    for (int c = chunk0; c < tile_n && col0 + c < rows_n && rows > 0; c += 2 * CHUNK) {
-      const int width = min(CHUNK, tile_n - c), gc = col0 + c;
+    uint32_t coming[CHUNK];
+    auto ask_accumulators = [&](int c) {
+      if (tile_n - c >= CHUNK) {
+        tmem_ld_32(acc + c, coming);
+      } else {
+#pragma unroll
+        for (int j = 16; j < CHUNK; ++j) coming[j] = 0u;
+        tmem_ld_16(acc + c, coming);
+      }
+    };
+    if (live(chunk0)) ask_accumulators(chunk0);
+    else hand_back();
+    for (int c = chunk0; live(c); c += STRIDE) {
+      const int width = min(CHUNK, tile_n - c), gc = col0 + c, next = c + STRIDE;
       float v[CHUNK];
-      uint32_t* const raw = reinterpret_cast<uint32_t*>(v);
-#pragma unroll
-      for (int j = 16; j < CHUNK; ++j) raw[j] = 0u;
-      if (width == CHUNK) tmem_ld_32(acc + c, raw);
-      else tmem_ld_16(acc + c, raw);
       tmem_ld_wait();
-      tmem_ld_settle_32(raw);
-      const int next = c + 2 * CHUNK;
-      if (!(next < tile_n && col0 + next < rows_n)) {
-        hand_back();
-        handed_back = true;
-      }
-      if (p.scale_out) {
+      tmem_ld_settle_32(coming);
 #pragma unroll
-        for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
-      }
-      if (bias) {
-        if (transposed) {
-          const float mine = __ldg(bias + min(row, rows_m - 1));
+      for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(coming[j]);
+      if (live(next)) ask_accumulators(next);
+      else hand_back();
+      if (!bias) {
+        if (p.scale_out) {
 #pragma unroll
-          for (int j = 0; j < CHUNK; ++j) v[j] += mine;
-        } else if (bias_vec && gc + CHUNK <= rows_n) {
-#pragma unroll
-          for (int u = 0; u < CHUNK / 4; ++u) {
-            const float4 q = __ldg(reinterpret_cast<const float4*>(bias + gc) + u);
-            v[4 * u] += q.x, v[4 * u + 1] += q.y, v[4 * u + 2] += q.z, v[4 * u + 3] += q.w;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) v[j] += __ldg(bias + min(gc + j, rows_n - 1));
+          for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
         }
+      } else if (bias_vec && gc + CHUNK <= rows_n) {
+#pragma unroll
+        for (int u = 0; u < CHUNK / 4; ++u) {
+          const float4 q = __ldg(reinterpret_cast<const float4*>(bias + gc) + u);
+          v[4 * u] = fmaf(v[4 * u], alpha, q.x), v[4 * u + 1] = fmaf(v[4 * u + 1], alpha, q.y);
+          v[4 * u + 2] = fmaf(v[4 * u + 2], alpha, q.z), v[4 * u + 3] = fmaf(v[4 * u + 3], alpha, q.w);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) v[j] = fmaf(v[j], alpha, __ldg(bias + min(gc + j, rows_n - 1)));
       }
       if (p.preact) store(v, static_cast<uint8_t*>(p.preact), c, width);
       if (p.act_shape == SHAPE_SIGMOID) {
@@ -511,36 +496,23 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
 #pragma unroll
         for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_RELU>(v[j], 0.f, 0.f);
       }
-      if (residual && transposed) {
-        if (row < rows_m) {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) {
-            if (j < width && gc + j < rows_n) {
-              const size_t at = size_t(gc + j) * ldd + row;
-              if constexpr (OUT_BYTES == 4) v[j] += reinterpret_cast<const float*>(residual)[at];
-              else v[j] += widen(reinterpret_cast<const uint16_t*>(residual)[at]);
-            }
-          }
-        }
-      } else if (residual) {
-        if (residual_vec && whole(c)) {
-#pragma unroll
-          for (int i = 0; i < STEPS; ++i) st_shared_v4(at_unit(i * ROWS_AT_ONCE + sub_row, unit), res[i].x, res[i].y, res[i].z, res[i].w);
-        } else {
-          const bool live = lane < min(width, rows_n - gc);
+      if (residual) {
+        if (!(residual_vec && whole(c))) {
+          const bool mine = lane < min(width, rows_n - gc);
           const uint8_t* src = residual + (size_t(row0) * ldd + gc + lane) * OUT_BYTES;
 #pragma unroll 8
           for (int r = 0; r < rows; ++r, src += size_t(ldd) * OUT_BYTES) {
-            if constexpr (OUT_BYTES == 4) st_shared_u32(at_element(r, lane), live ? *reinterpret_cast<const uint32_t*>(src) : 0u);
-            else st_shared_u16(at_element(r, lane), live ? *reinterpret_cast<const uint16_t*>(src) : uint16_t(0));
+            if constexpr (OUT_BYTES == 4) st_shared_u32(at_element(r, lane), mine ? *reinterpret_cast<const uint32_t*>(src) : 0u);
+            else st_shared_u16(at_element(r, lane), mine ? *reinterpret_cast<const uint16_t*>(src) : uint16_t(0));
           }
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < UNITS; ++u) res[u] = ld_shared_v4(at_unit(lane, u));
+          __syncwarp();
         }
-        __syncwarp();
-        ask_residual(next);
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-          const uint4 q4 = ld_shared_v4(at_unit(lane, u));
-          const uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+          const uint32_t q[4] = {res[u].x, res[u].y, res[u].z, res[u].w};
 #pragma unroll
           for (int h = 0; h < 4; ++h) {
             if constexpr (OUT_BYTES == 4) {
@@ -551,7 +523,7 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
             }
           }
         }
-        __syncwarp();
+        ask_residual(next);
       }
       if constexpr (OUT_BYTES == 2) {
         if (p.out_quant) {
@@ -571,7 +543,6 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
       }
       store(v, static_cast<uint8_t*>(p.d), c, width);
     }
-    if (!handed_back) hand_back();
   }
 }
 

@@ -108,6 +108,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
                : "memory");
 }
 
+// The same without ordering the thread's earlier memory accesses before it.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // One attempt: the hardware parks the thread until the phase completes or the
 // hint (nanoseconds) runs out, so a waiting role does not burn issue slots and
 // power spinning - on a power-capped part that is tensor-core clock.

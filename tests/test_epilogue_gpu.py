@@ -103,6 +103,16 @@ def test_every_plan(name, out_dtype, plan):
     check(name, 600, 776, 512, out_dtype, "gelu_tanh", plan=PLANS[plan])
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+@pytest.mark.parametrize("n,k", [(1, 8), (53, 3616), (4735, 264), (4741, 72), (9001, 1032)])
+def test_a_few_rows(m, name, n, k):
+    """Up to four rows take another kernel than the tiled one."""
+    check(name, m, n, k, torch.bfloat16 if name == "bf16" else torch.float16, "gelu")
+    check(name, m, n, k, torch.float32, "silu", bias=False, save=False, alpha=None)
+    check(name, m, n, k, torch.bfloat16, None, residual=True, save=False)
+
+
 @pytest.mark.parametrize("parts", [dict(bias=False), dict(residual=False), dict(save=False), dict(bias=False, residual=False, save=False),
                                    dict(alpha=None, bias=False, save=False)], ids=str)
 @pytest.mark.parametrize("shape", [(2304, 2560, 256), (64, 4096, 256)], ids=lambda s: "x".join(map(str, s)))
