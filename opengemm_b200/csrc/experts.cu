@@ -1,6 +1,7 @@
 // Host side of the experts' products and of the gradients of products: tile
 // choice, tensor maps and the launch (experts.cuh has the kernel).
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -42,35 +43,39 @@ struct ExpertPlan {
   int cta_group, tile_n;
 };
 
-// The tile of a launch.  Only bounds of the groups' sizes are known here (the
-// table of offsets is on the device), so they are taken as equal.
+// The tile of a launch: the cheapest of a short menu by an estimate.
 //
-// A tile costs its K blocks plus about 2500 cycles outside them.  A K block
-// costs the larger of the MMAs (half the tile width per instruction, 8192
-// multiply-adds a cycle and SM for 16 bits) and, where a group has no more rows
-// than one tile and its weights are therefore read from memory exactly once,
-// the SM's share of the memory bandwidth (24 bytes a cycle).  Pairs of CTAs
-// share the N-side operand, which is what lets wide tiles run at the tensor
-// pipe's rate; narrow tiles exist to give every SM work when there are few.
+// With several groups only their number and the number of all rows are known
+// here (the table of offsets is on the device): they are taken as equal, a
+// group's last tile as half full, and the last wave of tiles as half idle.
+// A tile costs its K blocks and some 300 cycles between two tiles (loads run
+// ahead into the next one, and its accumulator is a second one).  A K block
+// costs what full waves of such tiles measured: pairs of CTAs share the N-side
+// operand, which lets wide tiles run nearest the tensor pipe's rate (bf16
+// 4096 x 8192 x 4096, rows' gradient: 190 us in pairs, 217 / 237 / 364 us in
+// single CTAs 256 / 128 / 64 wide).  Where a group's rows fit one tile its
+// weights are read from memory once and nothing else is: the block then costs
+// the SM's share of the memory bandwidth, best used by tiles of 128 (16 tokens x
+// 8 of 64 experts, 2048 x 2048 weights: 59 us; 65 us in pairs, 63 us 256 wide,
+// 66 us 64 wide).  Narrow tiles give every SM work when there are few.
 ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count) {
   const int busy = std::max(1, std::min(groups, rows));
-  const int rows_each = ceil_div(std::max(rows, 1), busy);
-  static const ExpertPlan menu[] = {{2, 256}, {2, 128}, {1, 256}, {1, 128}, {1, 64}};
-  static const int mma_cycles[] = {560, 340, 620, 340, 220};
+  const double rows_each = double(std::max(rows, 1)) / busy;
+  static const ExpertPlan menu[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
+  static const int multiply_cycles[] = {560, 640, 350, 268}, stream_cycles[] = {775, 1250, 683, 430};
   ExpertPlan best = menu[0];
   double best_cost = 0;
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const ExpertPlan& c = menu[i];
-    if (glu && c.tile_n < 128) continue;
-    const int out_n = glu ? c.tile_n / 2 : c.tile_n;
-    const int m_tiles = mode == MODE_DW ? ceil_div(m_out, 128 * c.cta_group) : ceil_div(rows_each, 128 * c.cta_group);
-    const double tiles = double(mode == MODE_DW ? groups : busy) * m_tiles * ceil_div(cols, out_n);
-    const int blocks = mode == MODE_DW ? ceil_div(rows_each, 64) : blocks_fixed;
-    double block = mma_cycles[i];
-    if (mode != MODE_DW && m_tiles == 1) block = std::max(block, c.tile_n / c.cta_group * 128 / 24.0);
-    const double slots = sm_count / c.cta_group;
-    const double waves = std::max(1.0, double(int64_t((tiles + slots - 1) / slots)));
-    const double cost = waves * (blocks * block + 2500);
+    const int out_n = glu ? c.tile_n / 2 : c.tile_n, tile_m = 128 * c.cta_group;
+    const double m_tiles = mode == MODE_DW   ? ceil_div(m_out, tile_m)
+                           : groups == 1     ? ceil_div(std::max(rows, 1), tile_m)
+                                             : std::max(1.0, rows_each / tile_m + 0.5);
+    const double tiles = (mode == MODE_DW ? groups : busy) * m_tiles * ceil_div(cols, out_n);
+    const double blocks = mode == MODE_DW ? std::max(1.0, rows_each / 64) : blocks_fixed;
+    const int block = mode != MODE_DW && rows_each <= tile_m ? stream_cycles[i] : multiply_cycles[i];
+    const double waves = tiles / (sm_count / c.cta_group);
+    const double cost = (groups == 1 ? std::ceil(waves) : std::max(1.0, waves + 0.5)) * (blocks * block + 300);
     if (i == 0 || cost < best_cost) best = c, best_cost = cost;
   }
   return best;

@@ -35,7 +35,8 @@ enum ExpertMode : int { MODE_FORWARD = 0, MODE_DX = 1, MODE_DW = 2 };
 
 constexpr int XP_MAX_STAGES = 12;
 constexpr int XP_MAX_GROUPS = 1024;
-constexpr int XP_STAGING = 32 * 128;  // per epilogue warp: 32 rows of one 128-byte line
+constexpr int XP_CHUNK = 32;  // columns an epilogue warp works on at a time
+constexpr int XP_STAGING = 32 * XP_CHUNK * 4;  // per epilogue warp: its 32 rows of a chunk
 
 __host__ __device__ constexpr int xp_threads(int mode) { return mode == MODE_DW ? 224 : 192; }
 
@@ -115,8 +116,8 @@ template <int KIND, int CTA_GROUP, int MODE, bool GATHER, bool GLU, int OUT_BYTE
 __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __grid_constant__ ExpertParams p) {
   constexpr int TILE_M = 128 * CTA_GROUP;
   constexpr bool X_COLUMNS = MODE == MODE_DW, Y_COLUMNS = MODE != MODE_FORWARD;
-  constexpr int CHUNK = OUT_BYTES == 2 ? 64 : 32;  // columns of a 128-byte staging row
-  constexpr int UNIT = 16 / OUT_BYTES;
+  constexpr int CHUNK = XP_CHUNK, ROW_BYTES = CHUNK * OUT_BYTES, UNITS = ROW_BYTES / 16, UNIT = 16 / OUT_BYTES;
+  constexpr int ROWS_AT_ONCE = 32 / UNITS, STEPS = 32 / ROWS_AT_ONCE;
 
   extern __shared__ uint8_t dyn_smem[];
   __shared__ __align__(8) uint64_t bars[4 * XP_MAX_STAGES + 5];
@@ -417,7 +418,10 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     const uint32_t lane_base = uint32_t(quarter * 32) << 16;
     const uint32_t acc_empty_leader = CTA_GROUP == 2 ? map_to_cta(bar_acc_empty, 0) : bar_acc_empty;
     const uint32_t my_buf = staging + (warp - 2) * XP_STAGING;
-    const int sub_row = lane >> 3, unit = lane & 7;
+    const int sub_row = lane / UNITS, unit = lane % UNITS;
+    // 16-byte unit u of staging row r, swizzled so that eight lanes on eight rows,
+    // or on the units of one row, touch all banks.
+    auto at_unit = [&](int r, int u) { return my_buf + r * ROW_BYTES + ((u ^ (UNITS == 8 ? r & 7 : (r >> 1) & 3)) << 4); };
     const int out_tile_n = p.out_tile_n, cols = p.cols;
     const bool out_f16 = p.out_f16 != 0, vec_ok = p.vec_ok != 0;
     auto pack2 = [&](float lo, float hi) { return out_f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
@@ -442,51 +446,41 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
       const float alpha = MODE == MODE_FORWARD && p.alpha ? p.alpha[w.group] * p.factor : p.factor;
 
       // CHUNK columns of this lane's row, through the warp's swizzled buffer, as
-      // whole 128-byte segments of four rows an instruction; unaligned rows
-      // element by element.
+      // whole row segments; unaligned rows element by element, side by side.
       auto store = [&](const float* v, uint8_t* base, int ld, int col, int limit) {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+          uint32_t q[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+            q[h] = OUT_BYTES == 4 ? __float_as_uint(v[(4 * u + h) % CHUNK]) : pack2(v[(8 * u + 2 * h) % CHUNK], v[(8 * u + 2 * h + 1) % CHUNK]);
+          st_shared_v4(at_unit(lane, u), q[0], q[1], q[2], q[3]);
+        }
+        __syncwarp();
         if (vec_ok) {
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            uint32_t q[4];
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-              q[h] = OUT_BYTES == 4 ? __float_as_uint(v[(4 * u + h) % CHUNK]) : pack2(v[(8 * u + 2 * h) % CHUNK], v[(8 * u + 2 * h + 1) % CHUNK]);
-            st_shared_v4(my_buf + lane * 128 + ((u ^ (lane & 7)) << 4), q[0], q[1], q[2], q[3]);
-          }
-          __syncwarp();
           const int gcol = col + unit * UNIT;
           if (gcol < limit) {
             uint8_t* dst = base + ((row0 + sub_row) * ld + gcol) * OUT_BYTES;
-            const size_t step = size_t(4) * ld * OUT_BYTES;
+            const size_t step = size_t(ROWS_AT_ONCE) * ld * OUT_BYTES;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 4 * i + sub_row;
-              if (r < valid) *reinterpret_cast<uint4*>(dst + i * step) = ld_shared_v4(my_buf + r * 128 + ((unit ^ (r & 7)) << 4));
+            for (int i = 0; i < STEPS; ++i) {
+              const int r = i * ROWS_AT_ONCE + sub_row;
+              if (r < valid) *reinterpret_cast<uint4*>(dst + i * step) = ld_shared_v4(at_unit(r, unit));
             }
           }
-          __syncwarp();
-        } else if (lane < valid) {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) {
-            if (col + j < limit) {
-              const size_t at = (row0 + lane) * ld + col + j;
-              if constexpr (OUT_BYTES == 4) reinterpret_cast<float*>(base)[at] = v[j];
-              else reinterpret_cast<uint16_t*>(base)[at] = uint16_t(pack2(v[j], 0.0f) & 0xFFFFu);
-            }
+        } else if (col + lane < limit) {
+          uint8_t* dst = base + (row0 * ld + col + lane) * OUT_BYTES;
+#pragma unroll 8
+          for (int r = 0; r < valid; ++r, dst += size_t(ld) * OUT_BYTES) {
+            const uint32_t from = at_unit(r, lane / UNIT) + (lane % UNIT) * OUT_BYTES;
+            if constexpr (OUT_BYTES == 4) *reinterpret_cast<uint32_t*>(dst) = ld_shared_u32(from);
+            else *reinterpret_cast<uint16_t*>(dst) = ld_shared_u16(from);
           }
         }
+        __syncwarp();
       };
-      auto load = [&](int c, float* v) {
-        uint32_t* raw = reinterpret_cast<uint32_t*>(v);
-        tmem_ld_32(acc + c, raw);
-        if constexpr (CHUNK == 64) tmem_ld_32(acc + c + 32, raw + 32);
-      };
-      auto settle = [&](float* v) {
-        uint32_t* raw = reinterpret_cast<uint32_t*>(v);
-        tmem_ld_settle_32(raw);
-        if constexpr (CHUNK == 64) tmem_ld_settle_32(raw + 32);
-      };
+      auto load = [&](int c, float* v) { tmem_ld_32(acc + c, reinterpret_cast<uint32_t*>(v)); };
+      auto settle = [&](float* v) { tmem_ld_settle_32(reinterpret_cast<uint32_t*>(v)); };
       auto activate = [&](float* v) {
         if (p.act_shape == SHAPE_SIGMOID) {
           const float a = p.act_a, b = p.act_b;
@@ -545,7 +539,9 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CTA_GROUP == 2) mbar_arrive_cluster(acc_empty_leader + 8 * slot);
+        // Relaxed: what is handed back is tensor memory, whose loads have completed;
+        // a release would wait for this warp's stores as well.
+        if constexpr (CTA_GROUP == 2) mbar_arrive_cluster_relaxed(acc_empty_leader + 8 * slot);
         else mbar_arrive(bar_acc_empty + 8 * slot);
       }
     }
