@@ -49,8 +49,10 @@ struct ExpertPlan {
 // here (the table of offsets is on the device): they are taken as equal, a
 // group's last tile as half full, and the last wave of tiles as half idle.
 // A tile costs its K blocks and some 300 cycles between two tiles (loads run
-// ahead into the next one, and its accumulator is a second one).  A K block
-// costs what full waves of such tiles measured: pairs of CTAs share the N-side
+// ahead into the next one, and its accumulator is a second one), but no less
+// than storing it takes (16 experts with eight rows each, weights' gradient of
+// 2608 x 2992: 71 us in tiles of 256, 86 us in pairs, 96 and 149 us in narrower
+// ones; clearing that memory takes 66 us).  A K block costs what full waves of such tiles measured: pairs of CTAs share the N-side
 // operand, which lets wide tiles run nearest the tensor pipe's rate (bf16
 // 4096 x 8192 x 4096, rows' gradient: 190 us in pairs, 217 / 237 / 364 us in
 // single CTAs 256 / 128 / 64 wide).  Where a group's rows fit one tile its
@@ -62,7 +64,8 @@ ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int 
   const int busy = std::max(1, std::min(groups, rows));
   const double rows_each = double(std::max(rows, 1)) / busy;
   static const ExpertPlan menu[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
-  static const int multiply_cycles[] = {560, 640, 350, 268}, stream_cycles[] = {775, 1250, 683, 430};
+  static const int multiply_cycles[] = {560, 640, 350, 268}, stream_cycles[] = {775, 1365, 683, 430};
+  static const int least_cycles[] = {5600, 4800, 3300, 2600};
   ExpertPlan best = menu[0];
   double best_cost = 0;
   for (int i = 0; i < 4; ++i) {
@@ -75,7 +78,7 @@ ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int 
     const double blocks = mode == MODE_DW ? std::max(1.0, rows_each / 64) : blocks_fixed;
     const int block = mode != MODE_DW && rows_each <= tile_m ? stream_cycles[i] : multiply_cycles[i];
     const double waves = tiles / (sm_count / c.cta_group);
-    const double cost = (groups == 1 ? std::ceil(waves) : std::max(1.0, waves + 0.5)) * (blocks * block + 300);
+    const double cost = (groups == 1 ? std::ceil(waves) : std::max(1.0, waves + 0.5)) * std::max(blocks * block + 300, double(least_cycles[i]));
     if (i == 0 || cost < best_cost) best = c, best_cost = cost;
   }
   return best;
@@ -160,7 +163,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
   p.band = 8;
   p.y_bytes = plan.tile_n / plan.cta_group * 128;
   p.stage_bytes = 16384 + p.y_bytes;
-  p.stages = std::min(XP_MAX_STAGES, (SMEM_LIMIT - XP_STATIC_SMEM - 1024 - 4 * XP_STAGING) / p.stage_bytes);
+  p.stages = std::min(XP_MAX_STAGES, (SMEM_LIMIT - XP_STATIC_SMEM - 1024 - XP_EPILOGUE_WARPS * XP_STAGING) / p.stage_bytes);
   p.tmem_cols = pow2_at_least(2 * plan.tile_n);
   const uint32_t x_columns = mode == MODE_DW, y_columns = mode != MODE_FORWARD;
   const uint32_t fmt = bf16 ? 1u : 0u;  // e4m3 is code 0 of its kind, f16 of its own
@@ -212,7 +215,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
   const int64_t m_tiles = mode == MODE_DW ? int64_t(g.groups) * p.tiles_m_fixed
                                           : int64_t(g.rows) / (128 * plan.cta_group) + std::min(g.groups, g.rows);
   const int clusters = int(std::min<int64_t>(sm_count / plan.cta_group, m_tiles * p.tiles_n));
-  const int smem = p.stages * p.stage_bytes + 4 * XP_STAGING + 1024;
+  const int smem = p.stages * p.stage_bytes + XP_EPILOGUE_WARPS * XP_STAGING + 1024;
   const cudaError_t launched = kernel->launch(p, std::max(1, clusters) * plan.cta_group, smem, s);
   if (launched != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "kernel launch failed: %s", cudaGetErrorString(launched));
   return OG_OK;

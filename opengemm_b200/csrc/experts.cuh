@@ -18,12 +18,12 @@
 // the host never sees them): tiles start at the group's first row, rows past
 // its end are computed from whatever lies there and not stored.  Only the
 // weight gradient, which sums over rows, has to cut its last block of 64 rows
-// short: warp 6 waits for that stage's data and clears the rows past the end
-// in shared memory before the MMA reads it.
+// short: a warp of its own waits for that stage's data and clears the rows past
+// the end in shared memory before the MMA reads it.
 //
 // Roles as in kernel.cuh: warp 0 loads (one thread; all lanes when rows are
 // gathered, four rows a lane and instruction), warp 1 issues the MMAs, warps
-// 2-5 store.  Every wait is bounded.
+// 2-9 store, warp 10 is the weight gradient's.  Every wait is bounded.
 #pragma once
 
 #include "activation.cuh"
@@ -38,7 +38,10 @@ constexpr int XP_MAX_GROUPS = 1024;
 constexpr int XP_CHUNK = 32;  // columns an epilogue warp works on at a time
 constexpr int XP_STAGING = 32 * XP_CHUNK * 4;  // per epilogue warp: its 32 rows of a chunk
 
-__host__ __device__ constexpr int xp_threads(int mode) { return mode == MODE_DW ? 224 : 192; }
+// Two epilogue warps per quarter of the accumulator's rows, taking turns at its
+// columns: a weight gradient over few rows is all stores.
+constexpr int XP_EPILOGUE_WARPS = 8;
+__host__ __device__ constexpr int xp_threads(int mode) { return 64 + 32 * XP_EPILOGUE_WARPS + (mode == MODE_DW ? 32 : 0); }
 
 struct alignas(64) ExpertParams {
   CUtensorMap map_x;    // MMA-M side, boxes of 128 rows (64 x 64 in MODE_DW)
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar_acc_full + 8 * s, 1);
-      mbar_init(bar_acc_empty + 8 * s, 4 * CTA_GROUP);
+      mbar_init(bar_acc_empty + 8 * s, XP_EPILOGUE_WARPS * CTA_GROUP);
     }
     mbar_init(bar_tmem, CTA_GROUP);
     abort_flag = 0;
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
             if (4 * lane < mine)
               tma_gather4<CTA_GROUP>(sx + lane * 512, &p.map_x32, kb * block_k, token[0], token[1], token[2], token[3], full);
           }
-          if constexpr (MODE == MODE_DW) {  // a short block is on its way: warp 6 may look for it
+          if constexpr (MODE == MODE_DW) {  // a short block is on its way: the clearing warp may look for it
             if (leads && rank == 0 && kb == blocks - 1 && (w.rows & 63)) mbar_arrive(bar_go + 8 * stage);
           }
           ++issued;
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
         if (ok) mma_commit<CTA_GROUP>(bar_acc_full + 8 * slot);
       }
     }
-  } else if (MODE == MODE_DW && warp == 6) {
+  } else if (MODE == MODE_DW && warp == 2 + XP_EPILOGUE_WARPS) {
     // ------------------------------------------------------- short blocks
     // Counts the stages as the producer does.  Once the producer has asked for
     // a short block, the leader waits for its data (its barrier counts both
@@ -495,54 +498,56 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
         }
       };
 
-      if (valid > 0) {
-        for (int c = 0; c < out_tile_n && col0 + c < cols; c += CHUNK) {
-          float v[CHUNK];
-          if (nothing) {
-#pragma unroll
-            for (int j = 0; j < CHUNK; ++j) v[j] = 0.0f;
-          } else {
-            load(c, v);
-            if constexpr (GLU) {
-              float up[CHUNK];
-              load(out_tile_n + c, up);
-              tmem_ld_wait();
-              settle(v);
-              settle(up);
-              if (alpha != 1.0f) {
-#pragma unroll
-                for (int j = 0; j < CHUNK; ++j) v[j] *= alpha, up[j] *= alpha;
-              }
-              if (p.preact) {
-                store(v, static_cast<uint8_t*>(p.preact), p.ldz, col0 + c, cols);
-                store(up, static_cast<uint8_t*>(p.preact), p.ldz, p.glu_offset + col0 + c, p.glu_offset + cols);
-              }
-              activate(v);
-#pragma unroll
-              for (int j = 0; j < CHUNK; ++j) v[j] *= up[j];
-            } else {
-              tmem_ld_wait();
-              settle(v);
-              if (alpha != 1.0f) {
-#pragma unroll
-                for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
-              }
-              if constexpr (MODE == MODE_FORWARD) {
-                if (p.preact) store(v, static_cast<uint8_t*>(p.preact), p.ldz, col0 + c, cols);
-                activate(v);
-              }
-            }
-          }
-          store(v, static_cast<uint8_t*>(p.d), p.ldd, col0 + c, cols);
+      auto hand_back = [&] {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          // Relaxed: what is handed back is tensor memory, whose loads have completed;
+          // a release would wait for this warp's stores as well.
+          if constexpr (CTA_GROUP == 2) mbar_arrive_cluster_relaxed(acc_empty_leader + 8 * slot);
+          else mbar_arrive(bar_acc_empty + 8 * slot);
         }
-      }
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        // Relaxed: what is handed back is tensor memory, whose loads have completed;
-        // a release would wait for this warp's stores as well.
-        if constexpr (CTA_GROUP == 2) mbar_arrive_cluster_relaxed(acc_empty_leader + 8 * slot);
-        else mbar_arrive(bar_acc_empty + 8 * slot);
+      };
+      // The next chunk's accumulators are on their way while a chunk is stored
+      // (not those of a gated pair, which would be 64 more registers), and the
+      // slot goes back once its last columns have arrived.
+      constexpr int STRIDE = XP_EPILOGUE_WARPS / 4 * CHUNK;
+      const int chunk0 = (warp - 2) / 4 * CHUNK;
+      auto live = [&](int c) { return valid > 0 && c < out_tile_n && col0 + c < cols; };
+      float coming[CHUNK];
+      if (live(chunk0)) load(chunk0, coming);
+      else hand_back();
+      for (int c = chunk0; live(c); c += STRIDE) {
+        const bool last = !live(c + STRIDE);
+        float v[CHUNK], up[GLU ? CHUNK : 1];
+        if constexpr (GLU) load(out_tile_n + c, up);
+        tmem_ld_wait();
+        settle(coming);
+        if constexpr (GLU) settle(up);
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) v[j] = nothing ? 0.0f : coming[j];
+        if (last) hand_back();
+        else if (!GLU) load(c + STRIDE, coming);
+        if (alpha != 1.0f) {
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j) {
+            v[j] *= alpha;
+            if constexpr (GLU) up[j] *= alpha;
+          }
+        }
+        if constexpr (MODE == MODE_FORWARD) {
+          if (p.preact) {
+            store(v, static_cast<uint8_t*>(p.preact), p.ldz, col0 + c, cols);
+            if constexpr (GLU) store(up, static_cast<uint8_t*>(p.preact), p.ldz, p.glu_offset + col0 + c, p.glu_offset + cols);
+          }
+          activate(v);
+          if constexpr (GLU) {
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) v[j] *= up[j];
+          }
+        }
+        store(v, static_cast<uint8_t*>(p.d), p.ldd, col0 + c, cols);
+        if (GLU && !last) load(c + STRIDE, coming);
       }
     }
   }
