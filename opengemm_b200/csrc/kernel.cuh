@@ -42,7 +42,8 @@ constexpr int THREADS = 192;
 __host__ __device__ constexpr int epilogue_warps(bool fused) { return fused ? 8 : 4; }
 __host__ __device__ constexpr int kernel_threads(bool fused) { return 64 + 32 * epilogue_warps(fused); }
 constexpr int FUSED_CHUNK = 32;  // columns a warp of the fused epilogue works on at a time
-constexpr int fused_staging_bytes(int out_bytes) { return epilogue_warps(true) * 32 * FUSED_CHUNK * out_bytes; }
+// Per warp 32 rows of a chunk on their way out, and the chunk's bias.
+constexpr int fused_staging_bytes(int out_bytes) { return epilogue_warps(true) * (32 * FUSED_CHUNK * out_bytes + FUSED_CHUNK * 4); }
 constexpr int SWIZZLE_ALIGN = 1024;
 constexpr int EPI_BUF_BYTES = 32 * 128;  // 32 rows of one 128-byte swizzle row
 constexpr int CLC_SLOTS = 3;             // answers in flight between the fastest and the slowest role
@@ -350,7 +351,10 @@ __device__ __forceinline__ void store_quantized(const GemmParams& p, const float
 // in float32, each tensor rounded once.  A warp works on 32 rows x 32 columns
 // at a time.  The next chunk's accumulators and residual (each lane its own
 // row's 64 or 128 bytes) are asked for while the current one is worked on, the
-// first residual before the accumulator is waited for.  C leaves as whole row
+// first residual before the accumulator is waited for; so is the next chunk's
+// bias, one value a lane, which all lanes then read from shared memory (from L1,
+// where the residual's lines keep pushing it out, it cost 8 us of the 64 that
+// e4m3 4096^3 takes with everything on).  C leaves as whole row
 // segments through the warp's staging buffer; rows that are not whole 16-byte
 // units pass through it element by element, both ways.  Two accumulator slots
 // let the next tile's MMAs run meanwhile, and a slot is handed back as soon as
@@ -366,6 +370,7 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3;
   const int chunk0 = ((warp - 2) >> 2) * CHUNK;
   const uint32_t buf = staging + (warp - 2) * 32 * ROW_BYTES;
+  const uint32_t bias_buf = staging + epilogue_warps(true) * 32 * ROW_BYTES + (warp - 2) * CHUNK * 4;
   const int sub_row = lane / UNITS, unit = lane % UNITS;
   // 16-byte unit u of row r sits swizzled, so that eight lanes on eight rows, or on
   // the units of one row, touch all banks.
@@ -376,7 +381,6 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
   const uint8_t* const residual = static_cast<const uint8_t*>(p.residual);
   const bool residual_vec = residual && p.residual_vec;
   const float* const bias = p.bias;
-  const bool bias_vec = bias && (reinterpret_cast<uintptr_t>(bias) & 15) == 0;
   const float alpha = p.scale_out ? p.alpha : 1.0f;
   const uint32_t acc_empty_leader = CTA_GROUP == 2 ? map_to_cta(bar_acc_empty, 0) : bar_acc_empty;
   auto pack2 = [&](float lo, float hi) { return out_f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); };
@@ -397,7 +401,7 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
       for (int u = 0; u < UNITS; ++u) res[u] = src[u];
     };
     ask_residual(chunk0);
-    if (bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(bias + min(col0 + lane * 8, rows_n - 1)));
+    float my_bias = bias ? __ldg(bias + min(col0 + chunk0 + lane, rows_n - 1)) : 0.0f;
     const int slot = (p.acc_slots == 2) ? (tile_idx & 1) : 0;
     const uint32_t use = (p.acc_slots == 2) ? (tile_idx >> 1) : tile_idx;
     const bool ready = mbar_wait(bar_acc_full + 8 * slot, use & 1, ctx, SITE_EPI_ACC_FULL);
@@ -468,21 +472,20 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
       for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(coming[j]);
       if (live(next)) ask_accumulators(next);
       else hand_back();
-      if (!bias) {
-        if (p.scale_out) {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
-        }
-      } else if (bias_vec && gc + CHUNK <= rows_n) {
+      if (bias) {
+        st_shared_u32(bias_buf + lane * 4, __float_as_uint(my_bias));
+        __syncwarp();
+        my_bias = __ldg(bias + min(col0 + next + lane, rows_n - 1));
 #pragma unroll
         for (int u = 0; u < CHUNK / 4; ++u) {
-          const float4 q = __ldg(reinterpret_cast<const float4*>(bias + gc) + u);
-          v[4 * u] = fmaf(v[4 * u], alpha, q.x), v[4 * u + 1] = fmaf(v[4 * u + 1], alpha, q.y);
-          v[4 * u + 2] = fmaf(v[4 * u + 2], alpha, q.z), v[4 * u + 3] = fmaf(v[4 * u + 3], alpha, q.w);
+          const uint4 q = ld_shared_v4(bias_buf + u * 16);
+          v[4 * u] = fmaf(v[4 * u], alpha, __uint_as_float(q.x)), v[4 * u + 1] = fmaf(v[4 * u + 1], alpha, __uint_as_float(q.y));
+          v[4 * u + 2] = fmaf(v[4 * u + 2], alpha, __uint_as_float(q.z)), v[4 * u + 3] = fmaf(v[4 * u + 3], alpha, __uint_as_float(q.w));
         }
-      } else {
+        __syncwarp();
+      } else if (p.scale_out) {
 #pragma unroll
-        for (int j = 0; j < CHUNK; ++j) v[j] = fmaf(v[j], alpha, __ldg(bias + min(gc + j, rows_n - 1)));
+        for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
       }
       if (p.preact) store(v, static_cast<uint8_t*>(p.preact), c, width);
       if (p.act_shape == SHAPE_SIGMOID) {
