@@ -853,15 +853,16 @@ OG_API int32_t og_b200_route_gradient(const OgRoute* route, const float* grad_we
 OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32_t top_k, int32_t experts, int32_t* offsets,
                                    int32_t* token_of_row, int32_t* positions, int32_t* workspace, int32_t device, void* stream) {
   if (experts < 1 || experts > 1024) return routing_fail("%d experts: 1 to 1024 are served", experts);
-  if (top_k < 1 || tokens < 0 || tokens * top_k >= 0x7FFFFFFFll) return routing_fail("%lld tokens with %d experts each are too many", (long long)tokens, top_k);
+  if (top_k < 1 || tokens < 0 || tokens > 0x40000000ll || tokens * top_k > 0x40000000ll) return routing_fail("%lld tokens with %d experts each are too many", (long long)tokens, top_k);
   if (!offsets || (tokens && (!indices || !token_of_row || !positions))) return routing_fail("indices and the plan's arrays must be device pointers, got null");
+  if (tokens * top_k > PLAN_CHUNK && !workspace)
+    return routing_fail("%lld pairs take a workspace of %lld integers", (long long)(tokens * top_k), (long long)((tokens * top_k + PLAN_CHUNK - 1) / PLAN_CHUNK * experts));
   if (const int bad = use_device(device)) return bad;
   PlanParams p{};
   p.indices = indices, p.offsets = offsets, p.tokens = token_of_row, p.positions = positions, p.histogram = workspace;
   p.pairs = int(tokens * top_k), p.top_k = top_k, p.experts = experts;
   p.chunks = std::max(1, (p.pairs + PLAN_CHUNK - 1) / PLAN_CHUNK);
   if (p.chunks > 1) {
-    if (!workspace) return routing_fail("%d pairs take a workspace of %lld integers", p.pairs, (long long)p.chunks * experts);
     if (const int bad = dependent_launch(plan_histogram_kernel, dim3(p.chunks), PLAN_WARPS * 32, experts * sizeof(int), stream, p)) return bad;
   }
   const size_t smem = size_t(PLAN_WARPS + 2) * experts * sizeof(int);
