@@ -80,6 +80,58 @@ __device__ __forceinline__ float act_value(float x, float a, float b) {
   }
 }
 
+// Two float32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// act_value of two values; the same operations, two at a time where there are such instructions.
+template <int SHAPE>
+__device__ __forceinline__ float2 act_value2(float2 x, float a, float b) {
+  if constexpr (SHAPE == SHAPE_SIGMOID) {
+    float2 q = mul2(x, x);
+    q = make_float2(fminf(q.x, 1e8f), fminf(q.y, 1e8f));
+    const float2 t = mul2(x, fma2(both(b), q, both(a)));
+    const float2 e = make_float2(1.0f + exp2_fast(t.x), 1.0f + exp2_fast(t.y));
+    return mul2(x, make_float2(reciprocal_fast(e.x), reciprocal_fast(e.y)));
+  } else if constexpr (SHAPE == SHAPE_PHI) {
+    const float2 m = make_float2(fabsf(x.x), fabsf(x.y));
+    const float2 d = fma2(both(0.3275911f * 0.7071067811865476f), m, both(1.0f));
+    const float2 t = make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
+    const float2 q = mul2(mul2(x, x), both(-0.7213475204444817f));
+    const float2 e = make_float2(exp2_fast(q.x), exp2_fast(q.y));
+    float2 p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+    p = fma2(p, t, both(0.5f * 1.421413741f));
+    p = fma2(p, t, both(0.5f * -0.284496736f));
+    p = fma2(p, t, both(0.5f * 0.254829592f));
+    return fma2(make_float2(-fminf(m.x, 1e4f), -fminf(m.y, 1e4f)), mul2(mul2(p, t), e), make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+  } else {
+    return make_float2(act_value<SHAPE>(x.x, a, b), act_value<SHAPE>(x.y, a, b));
+  }
+}
+
+template <int SHAPE, int COUNT>
+__device__ __forceinline__ void activate_all(float* v, float a, float b) {
+#pragma unroll
+  for (int j = 0; j < COUNT; j += 2) {
+    const float2 y = act_value2<SHAPE>(make_float2(v[j], v[j + 1]), a, b);
+    v[j] = y.x, v[j + 1] = y.y;
+  }
+}
+
 // The activation and its derivative at x.
 template <int SHAPE>
 __device__ __forceinline__ void act_both(float x, float a, float b, float* value, float* slope) {

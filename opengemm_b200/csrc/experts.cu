@@ -64,7 +64,7 @@ ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int 
   const int busy = std::max(1, std::min(groups, rows));
   const double rows_each = double(std::max(rows, 1)) / busy;
   static const ExpertPlan menu[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
-  static const int multiply_cycles[] = {560, 640, 350, 268}, stream_cycles[] = {775, 1365, 683, 430};
+  static const int multiply_cycles[] = {560, 640, 420, 325}, stream_cycles[] = {775, 1365, 683, 430};
   static const int least_cycles[] = {5600, 4800, 3300, 2600};
   ExpertPlan best = menu[0];
   double best_cost = 0;
@@ -161,7 +161,8 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
   p.tiles_n = ceil_div(p.cols, p.out_tile_n);
   p.tiles_m_fixed = ceil_div(p.m_out, 128 * plan.cta_group);
   p.band = 8;
-  p.y_bytes = plan.tile_n / plan.cta_group * 128;
+  const int y_rows = plan.tile_n / plan.cta_group;  // of the N side, per CTA: a multiple of 64
+  p.y_bytes = y_rows * 128;
   p.stage_bytes = 16384 + p.y_bytes;
   p.stages = std::min(XP_MAX_STAGES, (SMEM_LIMIT - XP_STATIC_SMEM - 1024 - XP_EPILOGUE_WARPS * XP_STAGING) / p.stage_bytes);
   p.tmem_cols = pow2_at_least(2 * plan.tile_n);
@@ -197,8 +198,8 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
     const uint64_t inner = mode == MODE_FORWARD ? k : n;
     map(&p.map_x, g.x, inner, x_rows, 128, "the rows");
     map(&p.map_x32, g.x, inner, x_rows, gather ? 1 : 32, "the rows");
-    const uint32_t y_rows = mode == MODE_DX ? 64 : uint32_t(glu ? plan.tile_n / 2 : plan.tile_n / plan.cta_group);
-    map(&p.map_y, g.w, k, n, y_rows, "the weights", uint64_t(g.groups));
+    const uint32_t box_rows = mode == MODE_DX ? 64 : uint32_t(glu ? plan.tile_n / 2 : y_rows);
+    map(&p.map_y, g.w, k, n, box_rows, "the weights", uint64_t(g.groups));
   }
   if (rc != OG_OK) return experts_fail(rc, "%s", why);
 

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
       const int stages = p.stages, block_k = p.block_k, tile_n = p.tile_n;
       const uint32_t stage_bytes = p.stage_bytes, y_bytes = p.y_bytes;
       const int y_rows = tile_n / CTA_GROUP;       // MMA-N rows this CTA loads
-      const int y_boxes = (y_rows + 63) / 64;      // column boxes of a Y_COLUMNS operand
+      const int y_boxes = y_rows / 64;             // column boxes of a Y_COLUMNS operand
       const bool leads = !GATHER || lane == 0;     // the one thread that credits bytes and loads whole boxes
       int stage = 0;
       uint32_t phase = 0, issued = 0;
@@ -485,17 +485,9 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
       auto load = [&](int c, float* v) { tmem_ld_32(acc + c, reinterpret_cast<uint32_t*>(v)); };
       auto settle = [&](float* v) { tmem_ld_settle_32(reinterpret_cast<uint32_t*>(v)); };
       auto activate = [&](float* v) {
-        if (p.act_shape == SHAPE_SIGMOID) {
-          const float a = p.act_a, b = p.act_b;
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_SIGMOID>(v[j], a, b);
-        } else if (p.act_shape == SHAPE_PHI) {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_PHI>(v[j], 0.f, 0.f);
-        } else if (p.act_shape == SHAPE_RELU) {
-#pragma unroll
-          for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_RELU>(v[j], 0.f, 0.f);
-        }
+        if (p.act_shape == SHAPE_SIGMOID) activate_all<SHAPE_SIGMOID, CHUNK>(v, p.act_a, p.act_b);
+        else if (p.act_shape == SHAPE_PHI) activate_all<SHAPE_PHI, CHUNK>(v, 0.f, 0.f);
+        else if (p.act_shape == SHAPE_RELU) activate_all<SHAPE_RELU, CHUNK>(v, 0.f, 0.f);
       };
 
       auto hand_back = [&] {

@@ -479,8 +479,9 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
 #pragma unroll
         for (int u = 0; u < CHUNK / 4; ++u) {
           const uint4 q = ld_shared_v4(bias_buf + u * 16);
-          v[4 * u] = fmaf(v[4 * u], alpha, __uint_as_float(q.x)), v[4 * u + 1] = fmaf(v[4 * u + 1], alpha, __uint_as_float(q.y));
-          v[4 * u + 2] = fmaf(v[4 * u + 2], alpha, __uint_as_float(q.z)), v[4 * u + 3] = fmaf(v[4 * u + 3], alpha, __uint_as_float(q.w));
+          const float2 lo = fma2(make_float2(v[4 * u], v[4 * u + 1]), make_float2(alpha, alpha), make_float2(__uint_as_float(q.x), __uint_as_float(q.y)));
+          const float2 hi = fma2(make_float2(v[4 * u + 2], v[4 * u + 3]), make_float2(alpha, alpha), make_float2(__uint_as_float(q.z), __uint_as_float(q.w)));
+          v[4 * u] = lo.x, v[4 * u + 1] = lo.y, v[4 * u + 2] = hi.x, v[4 * u + 3] = hi.y;
         }
         __syncwarp();
       } else if (p.scale_out) {
@@ -488,25 +489,26 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
         for (int j = 0; j < CHUNK; ++j) v[j] *= alpha;
       }
       if (p.preact) store(v, static_cast<uint8_t*>(p.preact), c, width);
-      if (p.act_shape == SHAPE_SIGMOID) {
-        const float a = p.act_a, b = p.act_b;
-#pragma unroll
-        for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_SIGMOID>(v[j], a, b);
-      } else if (p.act_shape == SHAPE_PHI) {
-#pragma unroll
-        for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_PHI>(v[j], 0.f, 0.f);
-      } else if (p.act_shape == SHAPE_RELU) {
-#pragma unroll
-        for (int j = 0; j < CHUNK; ++j) v[j] = act_value<SHAPE_RELU>(v[j], 0.f, 0.f);
-      }
+      if (p.act_shape == SHAPE_SIGMOID) activate_all<SHAPE_SIGMOID, CHUNK>(v, p.act_a, p.act_b);
+      else if (p.act_shape == SHAPE_PHI) activate_all<SHAPE_PHI, CHUNK>(v, 0.f, 0.f);
+      else if (p.act_shape == SHAPE_RELU) activate_all<SHAPE_RELU, CHUNK>(v, 0.f, 0.f);
       if (residual) {
         if (!(residual_vec && whole(c))) {
           const bool mine = lane < min(width, rows_n - gc);
           const uint8_t* src = residual + (size_t(row0) * ldd + gc + lane) * OUT_BYTES;
-#pragma unroll 8
-          for (int r = 0; r < rows; ++r, src += size_t(ldd) * OUT_BYTES) {
-            if constexpr (OUT_BYTES == 4) st_shared_u32(at_element(r, lane), mine ? *reinterpret_cast<const uint32_t*>(src) : 0u);
-            else st_shared_u16(at_element(r, lane), mine ? *reinterpret_cast<const uint16_t*>(src) : uint16_t(0));
+          uint32_t element[32];  // all rows in flight at once
+#pragma unroll
+          for (int r = 0; r < 32; ++r, src += size_t(ldd) * OUT_BYTES) {
+            element[r] = 0u;
+            if (mine && r < rows) {
+              if constexpr (OUT_BYTES == 4) element[r] = *reinterpret_cast<const uint32_t*>(src);
+              else element[r] = *reinterpret_cast<const uint16_t*>(src);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 32; ++r) {
+            if constexpr (OUT_BYTES == 4) st_shared_u32(at_element(r, lane), element[r]);
+            else st_shared_u16(at_element(r, lane), uint16_t(element[r]));
           }
           __syncwarp();
 #pragma unroll
