@@ -369,19 +369,25 @@ OG_API const char* og_b200_routing_error(void);
 
 /* Gradients of C = act(factor * A . B^T + bias): with dz = grad * act'(z),
  *   grad_a = factor * dz . B,  grad_b = factor * dz^T . A,  grad_bias = column sums of dz.
- * grad, z and dz (scratch, not used without an activation) [m, n], a [m, k], b [n, k], all of
- * `dtype` ("bf16" or "f16"), n and k multiples of 8, on 16-byte boundaries; grad_a and grad_b
- * of `dtype` or float32 (out_f32), grad_bias float32 [n] through `partial`, ceil(m / 64) * n
- * floats.  A gradient whose pointer is null is not computed.  Errors: og_b200_experts_error(). */
+ * grad and z [m, n] (z not used without an activation), a [m, k], b [n, k], all of `dtype`
+ * ("bf16" or "f16"), n and k multiples of 8, on 16-byte boundaries; grad_a and grad_b of
+ * `dtype` or float32 (out_f32), grad_bias float32 [n].  A gradient whose pointer is null is
+ * not computed.  The 16-byte aligned workspace (dz, partial sums) holds at least what
+ * og_b200_gemm_gradients_workspace answers for the same structure (workspace and
+ * workspace_bytes aside); a negative answer is an error code.  Errors:
+ * og_b200_experts_error(). */
 typedef struct OgGemmGradients {
   const void *grad, *a, *b, *z;
-  void *dz, *grad_a, *grad_b;
-  float *grad_bias, *partial;
+  void *grad_a, *grad_b;
+  float* grad_bias;
+  void* workspace;
+  int64_t workspace_bytes;
   int32_t m, n, k, activation, out_f32;
   float factor;
   char dtype[16];
 } OgGemmGradients;
 OG_API int32_t og_b200_gemm_gradients(const OgGemmGradients* g, int32_t device, void* stream);
+OG_API int64_t og_b200_gemm_gradients_workspace(const OgGemmGradients* g, int32_t device);
 
 #ifdef __cplusplus
 }

@@ -236,25 +236,20 @@ def gemm_backward(grad, a, b, activation=None, preactivation=None, alpha=None, w
     for label, t in (("grad", grad), ("preactivation", preactivation), ("a", a), ("b", b)):
         if t is not None and t.data_ptr() % 16:
             raise ValueError(f"{label} must start on a 16-byte boundary")
-    grad_a = grad_b = grad_bias = scratch = None
+    grad_a = grad_b = grad_bias = None
     if "a" in want:
         grad_a = torch.empty_like(a, dtype=out_dtype)
     if "b" in want:
         grad_b = torch.empty_like(b, dtype=out_dtype)
-    dz_bytes = 0 if activation is None else -(-m * n // 8) * 16
     if "bias" in want:
         grad_bias = torch.empty(n, device=a.device, dtype=torch.float32)
-        scratch = torch.empty(dz_bytes + -(-m // 64) * n * 4, device=a.device, dtype=torch.uint8)
-    elif dz_bytes:
-        scratch = torch.empty(dz_bytes, device=a.device, dtype=torch.uint8)
-    dz = 0 if scratch is None else scratch.data_ptr()
     capi.library("mm").gemm_gradients(
         capi.OgGemmGradients(
-            grad.data_ptr(), a.data_ptr(), b.data_ptr(), 0 if preactivation is None else preactivation.data_ptr(), dz,
+            grad.data_ptr(), a.data_ptr(), b.data_ptr(), 0 if preactivation is None else preactivation.data_ptr(),
             0 if grad_a is None else grad_a.data_ptr(), 0 if grad_b is None else grad_b.data_ptr(),
-            0 if grad_bias is None else grad_bias.data_ptr(), dz + dz_bytes, m, n, k, capi.ACTIVATIONS[activation],
+            0 if grad_bias is None else grad_bias.data_ptr(), 0, 0, m, n, k, capi.ACTIVATIONS[activation],
             out_dtype is torch.float32, 1.0 if alpha is None else alpha, name.encode()),
-        a.get_device())
+        a.device)
     return grad_a, grad_b, grad_bias
 
 

@@ -62,8 +62,8 @@ class OgExpertProduct(ctypes.Structure):
 class OgGemmGradients(ctypes.Structure):
     """The gradients of one product (include/opengemm_b200.h)."""
 
-    _fields_ = ([(f, c_void_p) for f in ("grad", "a", "b", "z", "dz", "grad_a", "grad_b", "grad_bias", "partial")]
-                + [(f, c_int32) for f in ("m", "n", "k", "activation", "out_f32")]
+    _fields_ = ([(f, c_void_p) for f in ("grad", "a", "b", "z", "grad_a", "grad_b", "grad_bias", "workspace")]
+                + [("workspace_bytes", ctypes.c_int64)] + [(f, c_int32) for f in ("m", "n", "k", "activation", "out_f32")]
                 + [("factor", ctypes.c_float), ("dtype", c_char * 16)])
 
 
@@ -221,6 +221,9 @@ class Library:
                 fn = getattr(lib, "og_b200_" + name)
                 fn.restype, fn.argtypes = c_int32, argtypes
                 setattr(self, "_" + name, fn)
+            self._gradients_workspace = lib.og_b200_gemm_gradients_workspace
+            self._gradients_workspace.restype = ctypes.c_int64
+            self._gradients_workspace.argtypes = [POINTER(OgGemmGradients), c_int32]
             for name in ("experts_error", "routing_error"):
                 fn = getattr(lib, "og_b200_" + name)
                 fn.restype, fn.argtypes = c_char_p, []
@@ -375,7 +378,13 @@ class Library:
             raise RuntimeError(self._experts_error().decode())
 
     def gemm_gradients(self, gradients, device):
-        """The launches of an OgGemmGradients on the current stream of device index `device`."""
+        """The launches of an OgGemmGradients on the current stream of `device`, in a workspace made here."""
+        size, index = self._gradients_workspace(byref(gradients), device.index), device.index
+        workspace = None
+        if size > 0:
+            workspace = torch.empty(size, device=device, dtype=torch.uint8)
+            gradients.workspace, gradients.workspace_bytes = workspace.data_ptr(), size
+        device = index
         if self._gemm_gradients(byref(gradients), device, raw_stream(device)) != OG_OK:
             raise RuntimeError(self._experts_error().decode())
 

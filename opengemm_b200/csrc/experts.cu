@@ -6,8 +6,11 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "../../include/opengemm_b200.h"
@@ -38,9 +41,10 @@ int experts_fail(int code, const char* format, ...) {
 constexpr int XP_DEVICES = 64;
 constexpr int XP_STATIC_SMEM = 9 * 1024;  // barriers and the group tables
 
-// What a launch runs with.
+// What a launch runs with, and its estimated cycles.
 struct ExpertPlan {
   int cta_group, tile_n;
+  double cost = 0;
 };
 
 // The tile of a launch: the cheapest of a short menu by an estimate.
@@ -60,7 +64,9 @@ struct ExpertPlan {
 // the SM's share of the memory bandwidth, best used by tiles of 128 (16 tokens x
 // 8 of 64 experts, 2048 x 2048 weights: 59 us; 65 us in pairs, 63 us 256 wide,
 // 66 us 64 wide).  Narrow tiles give every SM work when there are few.
-ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count) {
+// With `parts` > 1 a single group's work is cut along its reduction into that
+// many launches' worth of tiles.
+ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count, int parts = 1) {
   const int busy = std::max(1, std::min(groups, rows));
   const double rows_each = double(std::max(rows, 1)) / busy;
   static const ExpertPlan menu[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
@@ -74,13 +80,14 @@ ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int 
     const double m_tiles = mode == MODE_DW   ? ceil_div(m_out, tile_m)
                            : groups == 1     ? ceil_div(std::max(rows, 1), tile_m)
                                              : std::max(1.0, rows_each / tile_m + 0.5);
-    const double tiles = (mode == MODE_DW ? groups : busy) * m_tiles * ceil_div(cols, out_n);
-    const double blocks = mode == MODE_DW ? std::max(1.0, rows_each / 64) : blocks_fixed;
+    const double tiles = double(parts) * (mode == MODE_DW ? groups : busy) * m_tiles * ceil_div(cols, out_n);
+    const double blocks = (mode == MODE_DW ? std::max(1.0, rows_each / 64) : blocks_fixed) / parts;
     const int block = mode != MODE_DW && rows_each <= tile_m ? stream_cycles[i] : multiply_cycles[i];
     const double waves = tiles / (sm_count / c.cta_group);
     const double cost = (groups == 1 ? std::ceil(waves) : std::max(1.0, waves + 0.5)) * std::max(blocks * block + 300, double(least_cycles[i]));
     if (i == 0 || cost < best_cost) best = c, best_cost = cost;
   }
+  best.cost = best_cost;
   return best;
 }
 
@@ -109,7 +116,59 @@ const ExpertKernel* find_kernel(int kind, int cta_group, int mode, bool gather, 
   return nullptr;
 }
 
-int launch_product(const OgExpertProduct& g, int device, void* stream) {
+// Parts that a plain product's gradient is cut into along its reduction: few
+// tiles with many K blocks each leave most SMs idle, and a part more costs the
+// float32 sums it writes and one short kernel that adds them (some 6000 cycles
+// and the sums' bytes, twice, at 3400 a cycle).
+int choose_parts(int mode, int m, int n, int k, int sm_count) {
+  const int m_out = mode == MODE_DW ? n : m, blocks = ceil_div(mode == MODE_DW ? m : n, 64);
+  int best = 1;
+  double best_cost = 0;
+  for (int parts = 1; parts <= 16 && parts * 4 <= std::max(4, blocks); parts *= 2) {
+    const double sums = parts > 1 ? 6000 + double(parts) * m_out * k * 8 / 3400 : 0;
+    const double cost = choose_plan(mode, false, 1, m, n, k, blocks, sm_count, parts).cost + sums;
+    if (parts == 1 || cost < 0.9 * best_cost) best = parts, best_cost = cost;
+  }
+  return best;
+}
+
+// out = sum over `parts` of partial[part], rounded once; in the order of the parts.
+template <typename T>
+__global__ void __launch_bounds__(256) add_parts_kernel(const float4* partial, T* out, long long vectors, int parts) {
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= vectors) return;
+  float4 sum = partial[i];
+  for (int s = 1; s < parts; ++s) {
+    const float4 v = partial[s * vectors + i];
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(out)[i] = sum;
+  } else if constexpr (std::is_same<T, __half>::value) {
+    reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_f16x2(sum.x, sum.y), pack_f16x2(sum.z, sum.w));
+  } else {
+    reinterpret_cast<uint2*>(out)[i] = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+  }
+}
+
+template <typename T>
+cudaError_t add_parts(const void* partial, void* out, long long values, int parts, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned((values / 4 + 255) / 256), 1, 1);
+  config.blockDim = dim3(256, 1, 1);
+  config.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, add_parts_kernel<T>, static_cast<const float4*>(partial), static_cast<T*>(out), values / 4, parts);
+}
+
+// `parts` > 1 (MODE_DX and MODE_DW of one group): out is the float32 partial sums, one after another.
+int launch_product(const OgExpertProduct& g, int device, void* stream, int parts = 1) {
   char why[256];
   const int mode = g.mode;
   if (mode < MODE_FORWARD || mode > MODE_DW) return experts_fail(OG_ERR_LAUNCH, "mode %d is none of 0..2", mode);
@@ -155,7 +214,17 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
   p.k = mode == MODE_FORWARD ? g.k : g.n;
   p.block_k = 128 / elem;
   p.k_blocks = ceil_div(p.k, p.block_k);
-  const ExpertPlan plan = choose_plan(mode, glu, g.groups, g.rows, p.m_out, p.cols, p.k_blocks, sm_count);
+  const ExpertPlan plan = choose_plan(mode, glu, g.groups, g.rows, p.m_out, p.cols, p.k_blocks, sm_count, parts);
+  p.rows_per_group = g.rows;
+  if (parts > 1) {
+    if (mode == MODE_DW) {
+      p.rows_per_group = ceil_div(ceil_div(g.rows, 64), parts) * 64;
+      p.groups = ceil_div(g.rows, p.rows_per_group);
+    } else {
+      p.split_blocks = ceil_div(p.k_blocks, parts);
+      p.groups = ceil_div(p.k_blocks, p.split_blocks);
+    }
+  }
   p.tile_n = plan.tile_n;
   p.out_tile_n = glu ? plan.tile_n / 2 : plan.tile_n;
   p.tiles_n = ceil_div(p.cols, p.out_tile_n);
@@ -213,8 +282,8 @@ int launch_product(const OgExpertProduct& g, int device, void* stream) {
     configured[device].fetch_or(1ull << index, std::memory_order_release);
   }
   // At most this many tiles: every group may end in a partial one.
-  const int64_t m_tiles = mode == MODE_DW ? int64_t(g.groups) * p.tiles_m_fixed
-                                          : int64_t(g.rows) / (128 * plan.cta_group) + std::min(g.groups, g.rows);
+  const int64_t m_tiles = mode == MODE_DW ? int64_t(p.groups) * p.tiles_m_fixed
+                                          : (int64_t(g.rows) / (128 * plan.cta_group) + std::min(g.groups, g.rows)) * parts;
   const int clusters = int(std::min<int64_t>(sm_count / plan.cta_group, m_tiles * p.tiles_n));
   const int smem = p.stages * p.stage_bytes + XP_EPILOGUE_WARPS * XP_STAGING + 1024;
   const cudaError_t launched = kernel->launch(p, std::max(1, clusters) * plan.cta_group, smem, s);
@@ -231,30 +300,78 @@ extern "C" {
 
 OG_API const char* og_b200_experts_error(void) { return experts_error; }
 
+// A workspace's parts: dz, the bias's partial sums, the products' partial sums
+// (one product after another uses them).  Each starts on a 16-byte boundary.
+struct GradientSpace {
+  int64_t dz, bias, sums;  // bytes
+  int parts_a, parts_b;
+};
+
+static GradientSpace gradient_space(const OgGemmGradients& g, int device) {
+  GradientSpace s{};
+  auto up = [](int64_t bytes) { return (bytes + 15) / 16 * 16; };
+  const int sm_count = device >= 0 && device < XP_DEVICES ? experts_sm_count(device) : 148;
+  s.parts_a = g.grad_a && g.m ? choose_parts(MODE_DX, g.m, g.n, g.k, sm_count) : 1;
+  s.parts_b = g.grad_b && g.m ? choose_parts(MODE_DW, g.m, g.n, g.k, sm_count) : 1;
+  if (g.activation) s.dz = up(int64_t(g.m) * g.n * 2);
+  if (g.grad_bias) s.bias = up(int64_t(ceil_div(g.m, 64)) * g.n * 4);
+  if (s.parts_a > 1) s.sums = up(int64_t(s.parts_a) * g.m * g.k * 4);
+  if (s.parts_b > 1) s.sums = std::max(s.sums, up(int64_t(s.parts_b) * g.n * g.k * 4));
+  return s;
+}
+
+static int check_gradients(const OgGemmGradients& g) {
+  if (std::strncmp(g.dtype, "bf16", 16) && std::strncmp(g.dtype, "f16", 16)) return experts_fail(OG_ERR_LAUNCH, "dtype %.16s is not served: bf16 and f16", g.dtype);
+  if (g.activation < ACT_NONE || g.activation > ACT_SILU) return experts_fail(OG_ERR_LAUNCH, "activation %d is none of 0..%d", g.activation, int(ACT_SILU));
+  if (g.m < 0 || g.n <= 0 || g.k <= 0 || g.n % 8 || g.k % 8) return experts_fail(OG_ERR_LAUNCH, "m = %d, n = %d, k = %d: n and k come in eights", g.m, g.n, g.k);
+  return OG_OK;
+}
+
+OG_API int64_t og_b200_gemm_gradients_workspace(const OgGemmGradients* g, int32_t device) {
+  if (!g) return experts_fail(OG_ERR_LAUNCH, "null OgGemmGradients");
+  if (const int rc = check_gradients(*g)) return rc;
+  const GradientSpace s = gradient_space(*g, device);
+  return s.dz + s.bias + s.sums;
+}
+
 OG_API int32_t og_b200_gemm_gradients(const OgGemmGradients* g, int32_t device, void* stream) {
   if (!g) return experts_fail(OG_ERR_LAUNCH, "null OgGemmGradients");
+  if (const int rc = check_gradients(*g)) return rc;
   const bool bf16 = !std::strncmp(g->dtype, "bf16", 16);
-  if (!bf16 && std::strncmp(g->dtype, "f16", 16)) return experts_fail(OG_ERR_LAUNCH, "dtype %.16s is not served: bf16 and f16", g->dtype);
-  if (g->activation < ACT_NONE || g->activation > ACT_SILU) return experts_fail(OG_ERR_LAUNCH, "activation %d is none of 0..%d", g->activation, int(ACT_SILU));
-  if (g->m < 0 || g->n <= 0 || g->k <= 0 || g->n % 8 || g->k % 8) return experts_fail(OG_ERR_LAUNCH, "m = %d, n = %d, k = %d: n and k come in eights", g->m, g->n, g->k);
+  if ((reinterpret_cast<uintptr_t>(g->grad_a) | reinterpret_cast<uintptr_t>(g->grad_b)) & 15)
+    return experts_fail(OG_ERR_LAUNCH, "gradients must start on 16-byte boundaries");
+  const GradientSpace s = gradient_space(*g, device);
+  if (s.dz + s.bias + s.sums > 0 && (!g->workspace || (reinterpret_cast<uintptr_t>(g->workspace) & 15) || g->workspace_bytes < s.dz + s.bias + s.sums))
+    return experts_fail(OG_ERR_LAUNCH, "these gradients take a 16-byte aligned workspace of %lld bytes, got %lld", (long long)(s.dz + s.bias + s.sums), (long long)g->workspace_bytes);
+  uint8_t* const dz = static_cast<uint8_t*>(g->workspace);
+  float* const bias_sums = reinterpret_cast<float*>(dz + s.dz);
+  uint8_t* const sums = dz + s.dz + s.bias;
   if (g->activation || g->grad_bias) {
-    const int rc = og_b200_activation_gradient(bf16 ? 1 : 2, g->activation, g->grad, g->z, g->dz, g->grad_bias, g->partial, nullptr, g->m, g->n, device, stream);
+    const int rc = og_b200_activation_gradient(bf16 ? 1 : 2, g->activation, g->grad, g->z, dz, g->grad_bias, bias_sums, nullptr, g->m, g->n, device, stream);
     if (rc != OG_OK) return experts_fail(rc, "%s", og_b200_routing_error());
   }
   OgExpertProduct product;
   std::memset(&product, 0, sizeof product);
-  product.x = g->activation ? g->dz : g->grad;
-  product.groups = 1, product.rows = g->m, product.n = g->n, product.k = g->k;
-  product.out_f32 = g->out_f32, product.factor = g->factor;
+  product.x = g->activation ? dz : g->grad;
+  product.groups = 1, product.rows = g->m, product.n = g->n, product.k = g->k, product.factor = g->factor;
   std::memcpy(product.dtype, g->dtype, sizeof product.dtype);
-  if (g->grad_a) {
-    product.mode = MODE_DX, product.w = g->b, product.out = g->grad_a;
-    const int rc = launch_product(product, device, stream);
+  for (int mode = MODE_DX; mode <= MODE_DW; ++mode) {
+    void* const out = mode == MODE_DX ? g->grad_a : g->grad_b;
+    if (!out) continue;
+    const int parts = mode == MODE_DX ? s.parts_a : s.parts_b;
+    product.mode = mode, product.w = mode == MODE_DX ? g->b : g->a;
+    product.out = parts > 1 ? sums : out, product.out_f32 = parts > 1 ? 1 : g->out_f32;
+    int rc = launch_product(product, device, stream, parts);
     if (rc != OG_OK) return rc;
-  }
-  if (g->grad_b) {
-    product.mode = MODE_DW, product.w = g->a, product.out = g->grad_b;
-    return launch_product(product, device, stream);
+    if (parts == 1) continue;
+    // as many parts as have K blocks
+    const int blocks = ceil_div(mode == MODE_DX ? g->n : g->m, 64), live = ceil_div(blocks, ceil_div(blocks, parts));
+    const long long values = (long long)(mode == MODE_DX ? g->m : g->n) * g->k;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const cudaError_t launched = g->out_f32 ? add_parts<float>(sums, out, values, live, st)
+                                 : bf16     ? add_parts<__nv_bfloat16>(sums, out, values, live, st)
+                                            : add_parts<__half>(sums, out, values, live, st);
+    if (launched != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "kernel launch failed: %s", cudaGetErrorString(launched));
   }
   return OG_OK;
 }

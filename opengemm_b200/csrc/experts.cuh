@@ -55,6 +55,9 @@ struct alignas(64) ExpertParams {
   void* preact;
   unsigned long long wait_limit_ns;
   int groups, rows;
+  int rows_per_group;   // without offsets: rows of each group but the last (MODE_DW cut along its rows)
+  int split_blocks;     // MODE_DX of one group cut along its reduction: K blocks of each part, which is then
+                        // a "group" with all rows; 0 otherwise
   int cols;             // output columns
   int m_out;            // MODE_DW: output rows of each group
   int k;                // reduction extent (MODE_DW: the group's rows)
@@ -76,6 +79,7 @@ struct alignas(64) ExpertParams {
 struct ExpertTile {
   int group, first_row, rows;  // rows of the group
   int mi, ni;
+  int k0;  // first K block
 };
 
 // Gathered rows: four rows of `tmap` (one-row boxes) into 512 consecutive bytes.
@@ -179,11 +183,12 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
   // Group table: rows and tiles before each group.  Warp 2 sums; a lane takes a
   // contiguous run of groups.
   const int groups = p.groups;
-  for (int i = threadIdx.x; i <= groups; i += xp_threads(MODE)) group_row[i] = p.offsets ? p.offsets[i] : i * p.rows;
+  for (int i = threadIdx.x; i <= groups; i += xp_threads(MODE)) group_row[i] = p.offsets ? p.offsets[i] : min(i * p.rows_per_group, p.rows);
   __syncthreads();
   if (warp == 2) {
     auto tiles_of = [&](int e) {
-      const int m_tiles = MODE == MODE_DW ? p.tiles_m_fixed : (group_row[e + 1] - group_row[e] + TILE_M - 1) / TILE_M;
+      const int rows = MODE == MODE_DX && p.split_blocks ? p.rows : group_row[e + 1] - group_row[e];
+      const int m_tiles = MODE == MODE_DW ? p.tiles_m_fixed : (rows + TILE_M - 1) / TILE_M;
       return m_tiles * p.tiles_n;
     };
     const int per = (groups + 31) / 32, first = min(lane * per, groups), last = min(first + per, groups);
@@ -217,6 +222,8 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     w.group = lo;
     w.first_row = group_row[lo];
     w.rows = group_row[lo + 1] - w.first_row;
+    w.k0 = 0;
+    if (MODE == MODE_DX && p.split_blocks) w.first_row = 0, w.rows = p.rows, w.k0 = lo * p.split_blocks;
     const int m_tiles = MODE == MODE_DW ? p.tiles_m_fixed : (w.rows + TILE_M - 1) / TILE_M;
     const int local = t - group_tile[lo];
     const int band = local / (p.band * p.tiles_n);
@@ -225,7 +232,10 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     w.ni = rest / height;
     w.mi = band * p.band + rest - w.ni * height;
   };
-  auto k_blocks_of = [&](const ExpertTile& w) { return MODE == MODE_DW ? (w.rows + 63) / 64 : p.k_blocks; };
+  auto k_blocks_of = [&](const ExpertTile& w) {
+    if (MODE == MODE_DW) return (w.rows + 63) / 64;
+    return MODE == MODE_DX && p.split_blocks ? min(p.split_blocks, p.k_blocks - w.k0) : p.k_blocks;
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -284,7 +294,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
               }
             } else if constexpr (MODE == MODE_DX) {
               const int c0 = w.ni * tile_n + int(rank) * y_rows;
-              for (int b = 0; b < y_boxes; ++b) tma_load_3d<CTA_GROUP>(sy + b * 8192, &p.map_y, c0 + 64 * b, kb * 64, w.group, full);
+              for (int b = 0; b < y_boxes; ++b) tma_load_3d<CTA_GROUP>(sy + b * 8192, &p.map_y, c0 + 64 * b, (w.k0 + kb) * 64, p.split_blocks ? 0 : w.group, full);
             } else {
               const int r = w.first_row + kb * 64, m0 = w.mi * TILE_M + int(rank) * 128;
               tma_load_2d<CTA_GROUP>(sx, &p.map_x, m0, r, full);
@@ -293,9 +303,10 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
               for (int b = 0; b < y_boxes; ++b) tma_load_2d<CTA_GROUP>(sy + b * 8192, &p.map_y, c0 + 64 * b, r, full);
             }
             if constexpr (MODE != MODE_DW && !GATHER) {
-              if (mine == 128) tma_load_2d<CTA_GROUP>(sx, &p.map_x, kb * block_k, x_row, full);
+              const int kx = (w.k0 + kb) * block_k;
+              if (mine == 128) tma_load_2d<CTA_GROUP>(sx, &p.map_x, kx, x_row, full);
               else
-                for (int r = 0; r < mine; r += 32) tma_load_2d<CTA_GROUP>(sx + r * 128, &p.map_x32, kb * block_k, x_row + r, full);
+                for (int r = 0; r < mine; r += 32) tma_load_2d<CTA_GROUP>(sx + r * 128, &p.map_x32, kx, x_row + r, full);
             }
           }
           if constexpr (GATHER) {
@@ -347,7 +358,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + slot * p.tile_n;
         uint32_t accumulate = 0;
-        int k_left = MODE == MODE_DW ? w.rows : p.k;
+        int k_left = MODE == MODE_DW ? w.rows : p.k - w.k0 * block_k;
         for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(bar_full + 8 * stage, phase, ctx, SITE_MMA_FULL)) {
             ok = false;
@@ -442,7 +453,8 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
       const int local_row = w.mi * TILE_M + int(rank) * 128 + quarter * 32;  // this warp's first row of the group's output
       const int group_rows = MODE == MODE_DW ? p.m_out : w.rows;
       const int valid = min(max(group_rows - local_row, 0), 32);             // rows this warp stores
-      const size_t row0 = size_t(MODE == MODE_DW ? size_t(w.group) * p.m_out : size_t(w.first_row)) + local_row;
+      const bool by_part = MODE == MODE_DX && p.split_blocks;                // each part has an output of its own
+      const size_t row0 = (MODE == MODE_DW ? size_t(w.group) * p.m_out : by_part ? size_t(w.group) * p.rows : size_t(w.first_row)) + local_row;
       const int col0 = w.ni * out_tile_n;
       const uint32_t acc = tmem_base + lane_base + slot * p.tile_n;
       const bool nothing = MODE == MODE_DW && w.rows == 0;                   // no rows: the sum is zero

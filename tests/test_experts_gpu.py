@@ -197,7 +197,9 @@ def check_gemm_gradients(m, n, k, dtype, activation=None, alpha=None, out_dtype=
     assert_within(grad_bias, dz.sum(0), (16 + m / 64) * 2.0**-24 * dz.abs().sum(0) + eval_error.sum(0), "bias")
 
 
-@pytest.mark.parametrize("shape", [(1, 8, 8), (1, 4096, 256), (300, 520, 768), (77, 40, 128), (1001, 136, 264), (4100, 776, 512)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("shape", [(1, 8, 8), (1, 4096, 256), (300, 520, 768), (77, 40, 128), (1001, 136, 264), (4100, 776, 512),
+                                   (36, 4096, 264), (130, 2056, 128), (5001, 64, 72)],  # cut along the reduction
+                         ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("out_dtype", [None, torch.float32], ids=str)
 def test_gemm_gradients(shape, dtype, out_dtype):

@@ -90,11 +90,26 @@ def test_product_on_a_device_out_of_range():
     refused(lib()._expert_product(ctypes.byref(product()), 64, 0), lib()._experts_error, "out of range")
 
 
-@pytest.mark.parametrize("changes,words", [(dict(dtype=b"tf32"), "dtype"), (dict(activation=5), "activation"), (dict(n=60), "eights"), (dict(k=12), "eights"), (dict(m=-1), "m = -1")], ids=str)
+@pytest.mark.parametrize("changes,words", [(dict(dtype=b"tf32"), "dtype"), (dict(activation=5), "activation"), (dict(n=60), "eights"), (dict(k=12), "eights"), (dict(m=-1), "m = -1"), (dict(activation=1), "workspace")], ids=str)
 def test_gemm_gradients_refuse(changes, words):
-    fields = dict(grad=SOME, a=SOME, b=SOME, z=SOME, dz=SOME, grad_a=SOME, grad_b=SOME, grad_bias=0, partial=0, m=8, n=64, k=64, activation=0, out_f32=0, factor=1.0, dtype=b"f16")
+    fields = dict(grad=SOME, a=SOME, b=SOME, z=SOME, grad_a=SOME, grad_b=SOME, grad_bias=0, workspace=0, m=8, n=64, k=64, activation=0, out_f32=0, factor=1.0, dtype=b"f16")
     fields.update(changes)
     refused(lib()._gemm_gradients(ctypes.byref(capi.OgGemmGradients(**fields)), 0, 0), lib()._experts_error, words)
+    if words != "workspace":
+        assert lib()._gradients_workspace(ctypes.byref(capi.OgGemmGradients(**fields)), 0) < 0
+
+
+def test_gradients_workspace():
+    """dz, the bias's sums, and the partial sums of products cut along their reduction."""
+    def size(m, n, k, activation=0, bias=0, a=SOME, b=SOME):
+        return lib()._gradients_workspace(ctypes.byref(capi.OgGemmGradients(grad_a=a, grad_b=b, grad_bias=bias, m=m, n=n, k=k, activation=activation, dtype=b"bf16")), -1)
+
+    assert size(4096, 8192, 4096) == 0
+    assert size(4096, 8192, 4096, activation=1) == 4096 * 8192 * 2
+    assert size(4096, 8192, 4096, activation=1, bias=SOME) == 4096 * 8192 * 2 + 64 * 8192 * 4
+    few_rows = size(36, 8064, 2680, b=0)
+    assert few_rows > 0 and few_rows % (36 * 2680 * 4) == 0  # whole parts of the rows' gradient
+    assert size(0, 64, 64, activation=1, bias=SOME) == 0
 
 
 @pytest.mark.parametrize("name,m,fields,words", [
