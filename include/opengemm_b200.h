@@ -361,7 +361,7 @@ OG_API int32_t og_b200_expert_combine_gradient(int32_t dtype, const void* grad, 
 /* dz = grad * act'(z) for rows [0, rows), or [0, *row_limit) if row_limit (device) is given.
  * z, dz [rows, n]; grad [rows, n] (gated: n/2).  bias_gradient (float32 [n], or null; not for
  * a gated activation): column sums of dz before it is rounded, through a workspace of
- * ceil(rows / 64) * n floats.  Without an activation z and dz are not used. */
+ * ceil(rows / 16) * n floats.  Without an activation z and dz are not used. */
 OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, const void* grad, const void* z, void* dz,
                                            float* bias_gradient, float* workspace, const int32_t* row_limit,
                                            int64_t rows, int32_t n, int32_t device, void* stream);

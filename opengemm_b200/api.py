@@ -166,6 +166,9 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
     m, n, k = a.size(0), b.size(0), k_of(d, a.size(1))
     check_operands(d, m, n, k, a, b, sfa, sfb)
     lib, g = _bound.get((name, m, n, k, capi.independent_inputs())) or bind(name, m, n, k, a.device)
+    if out is None and residual is not None and residual.dtype is d.out and residual.shape == (m, n) and residual.is_contiguous() \
+            and residual.device == a.device:
+        out = torch.empty_like(residual)  # the cheapest way to one
     out = output(d, m, n, out, a.device)
     if activation is not None or residual is not None or preactivation is not None:
         check_epilogue(name, d, m, n, out, activation, residual, preactivation)

@@ -101,19 +101,31 @@ int experts_sm_count(int device) {
   return count;
 }
 
+const ExpertKernel* kernel_at(int index) {
+  if (index < EXPERT_FORWARD16_COUNT) return &EXPERT_FORWARD16[index];
+  index -= EXPERT_FORWARD16_COUNT;
+  if (index < EXPERT_FORWARD8_COUNT) return &EXPERT_FORWARD8[index];
+  index -= EXPERT_FORWARD8_COUNT;
+  return index < EXPERT_GRADIENT_COUNT ? &EXPERT_GRADIENT[index] : nullptr;
+}
+
 const ExpertKernel* find_kernel(int kind, int cta_group, int mode, bool gather, bool glu, int out_bytes, int* index) {
-  const ExpertKernel* const lists[] = {EXPERT_FORWARD16, EXPERT_FORWARD8, EXPERT_GRADIENT};
-  const int counts[] = {EXPERT_FORWARD16_COUNT, EXPERT_FORWARD8_COUNT, EXPERT_GRADIENT_COUNT};
-  int at = 0;
-  for (int l = 0; l < 3; ++l)
-    for (int i = 0; i < counts[l]; ++i, ++at) {
-      const ExpertKernel& k = lists[l][i];
-      if (k.kind == kind && k.cta_group == cta_group && k.mode == mode && k.gather == int(gather) && k.glu == int(glu) && k.out_bytes == out_bytes) {
-        *index = at;
-        return &k;
-      }
+  for (int i = 0; const ExpertKernel* k = kernel_at(i); ++i)
+    if (k->kind == kind && k->cta_group == cta_group && k->mode == mode && k->gather == int(gather) && k->glu == int(glu) && k->out_bytes == out_bytes) {
+      *index = i;
+      return k;
     }
   return nullptr;
+}
+
+std::atomic<uint64_t> configured[XP_DEVICES];  // bit per kernel
+
+int ensure_expert_kernel(const ExpertKernel& kernel, int index, int device) {
+  if (configured[device].load(std::memory_order_acquire) >> index & 1) return OG_OK;
+  const cudaError_t status = kernel.configure(SMEM_LIMIT - XP_STATIC_SMEM);
+  if (status != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(status));
+  configured[device].fetch_or(1ull << index, std::memory_order_release);
+  return OG_OK;
 }
 
 // Parts that a plain product's gradient is cut into along its reduction: few
@@ -275,12 +287,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   int index = 0;
   const ExpertKernel* kernel = find_kernel(e4m3 ? KIND_F8F6F4 : KIND_F16, plan.cta_group, mode, gather, glu, out_bytes, &index);
   if (!kernel) return experts_fail(OG_ERR_NO_KERNEL, "no kernel for this product");
-  static std::atomic<uint64_t> configured[XP_DEVICES];
-  if (!(configured[device].load(std::memory_order_acquire) >> index & 1)) {
-    const cudaError_t status = kernel->configure(SMEM_LIMIT - XP_STATIC_SMEM);
-    if (status != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(status));
-    configured[device].fetch_or(1ull << index, std::memory_order_release);
-  }
+  if (const int bad = ensure_expert_kernel(*kernel, index, device)) return bad;
   // At most this many tiles: every group may end in a partial one.
   const int64_t m_tiles = mode == MODE_DW ? int64_t(p.groups) * p.tiles_m_fixed
                                           : (int64_t(g.rows) / (128 * plan.cta_group) + std::min(g.groups, g.rows)) * parts;
@@ -292,6 +299,14 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
 }
 
 }  // namespace
+
+// For og_b200_prepare_device, with the device current.
+const char* prepare_experts(int device) {
+  for (int i = 0; const ExpertKernel* k = kernel_at(i); ++i)
+    if (ensure_expert_kernel(*k, i, device) != OG_OK) return experts_error;
+  return nullptr;
+}
+
 }  // namespace og
 
 using namespace og;
@@ -314,7 +329,7 @@ static GradientSpace gradient_space(const OgGemmGradients& g, int device) {
   s.parts_a = g.grad_a && g.m ? choose_parts(MODE_DX, g.m, g.n, g.k, sm_count) : 1;
   s.parts_b = g.grad_b && g.m ? choose_parts(MODE_DW, g.m, g.n, g.k, sm_count) : 1;
   if (g.activation) s.dz = up(int64_t(g.m) * g.n * 2);
-  if (g.grad_bias) s.bias = up(int64_t(ceil_div(g.m, 64)) * g.n * 4);
+  if (g.grad_bias) s.bias = up(int64_t(ceil_div(g.m, gradient_block_rows(g.m, g.n))) * g.n * 4);
   if (s.parts_a > 1) s.sums = up(int64_t(s.parts_a) * g.m * g.k * 4);
   if (s.parts_b > 1) s.sums = std::max(s.sums, up(int64_t(s.parts_b) * g.n * g.k * 4));
   return s;

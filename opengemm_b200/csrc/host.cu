@@ -52,6 +52,9 @@ extern const int FUSED_DENSE_COUNT;
 extern const FixedKernel FUSED_SCALED[];
 extern const int FUSED_SCALED_COUNT;
 
+// Implemented in experts.cu: opts its kernels into their shared memory; null, or what failed.
+const char* prepare_experts(int device);
+
 // One index space over the specialised kernels: fixed-shape dense, fixed-shape
 // scaled, then the feature-free ones, then those with the fused epilogue.
 inline int fixed_count() { return FIXED_DENSE_COUNT + FIXED_SCALED_COUNT; }
@@ -613,6 +616,7 @@ OG_API int32_t og_b200_prepare_device(int32_t device) {
     const int configured = ensure_fixed_configured(device, index);
     if (configured != OG_OK) return configured;
   }
+  if (const char* failed = prepare_experts(device)) return fail(OG_ERR_LAUNCH, "%s", failed);
   const int sm_count = sm_count_of(device);
   std::lock_guard<std::mutex> lock(device_mutex);
   return allocate_workspaces(devices[device], sm_count);

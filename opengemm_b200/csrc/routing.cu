@@ -645,25 +645,29 @@ struct ActGradientParams {
   const void* z;      // [rows, n], or null without an activation
   void* dz;           // [rows, n], or null when it is grad itself
   float* partial;     // [row blocks, n] column sums, or null
+  float* column_sums; // [n] the sums themselves, where one cluster of blocks has all rows
+  int block_rows;     // rows a block works on, a multiple of 8
   const int* limit;   // rows to work on (device), or null for all
   long long rows;
   int n, width, shape, glu;
   float a, b;
 };
 
-constexpr int GRADIENT_ROWS = 64;  // rows a block works on: 8 row lanes of 8 rows
+constexpr int GRADIENT_CLUSTER = 8;  // up to this many blocks add up their column sums among themselves
 
 // dz = grad * act'(z), eight columns a thread; a gated pair writes both halves,
 // gate: grad * up * act'(gate), up: grad * act(gate).  Column sums (of the
 // unrounded values) are added per thread down its rows, across the block's row
-// lanes in a fixed order, and across blocks by column_sum_kernel.
+// lanes in a fixed order, and across blocks by column_sum_kernel; where eight
+// blocks have all rows they are one cluster, whose first adds the others' sums
+// from their shared memory, which saves that launch.
 template <typename T>
 __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientParams p) {
   pdl_wait_prior_grids();
   pdl_launch_dependents();
   const long long rows = p.limit ? *p.limit : p.rows;
-  const long long first = (long long)blockIdx.x * GRADIENT_ROWS;
-  if (first >= rows) return;
+  const long long first = (long long)blockIdx.x * p.block_rows;
+  if (first >= rows) return;  // (never with column_sums: its grid is the blocks that have rows)
   const int lane = threadIdx.x & 31, row_lane = threadIdx.x >> 5;
   const int col = (blockIdx.y * 32 + lane) * 8;
   const bool live = col < p.width;
@@ -684,7 +688,7 @@ __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientPara
     }
   };
 #pragma unroll 2
-  for (int r = row_lane; r < GRADIENT_ROWS; r += 8) {
+  for (int r = row_lane; r < p.block_rows; r += 8) {
     const long long row = first + r;
     if (!live || row >= rows) break;
     float g[8], x[8], value[8], slope[8];
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientPara
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] += g[i];
   }
-  if (!p.partial) return;
+  if (!p.partial && !p.column_sums) return;
   __shared__ float parts[8][256];
 #pragma unroll
   for (int i = 0; i < 8; ++i) parts[row_lane][i * 32 + lane] = sum[i];
@@ -722,7 +726,18 @@ __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientPara
 #pragma unroll
   for (int i = 0; i < 8; ++i) total += parts[i][threadIdx.x];
   const int at = blockIdx.y * 256 + (threadIdx.x & 31) * 8 + (threadIdx.x >> 5);
-  if (at < p.n) p.partial[(long long)blockIdx.x * p.n + at] = total;
+  if (!p.column_sums) {
+    if (at < p.n) p.partial[(long long)blockIdx.x * p.n + at] = total;
+    return;
+  }
+  __syncthreads();  // everyone has read its column of `parts`
+  parts[0][threadIdx.x] = total;
+  cluster_sync_all();
+  if (blockIdx.x == 0 && at < p.n) {
+    for (unsigned b = 1; b < gridDim.x; ++b) total += ld_cluster_f32(map_to_cta(smem_u32(&parts[0][threadIdx.x]), b));
+    p.column_sums[at] = total;
+  }
+  cluster_sync_all();  // the others' shared memory stays until it has been read
 }
 
 // Sums over the row blocks: eight lanes take every eighth block, added in order.
@@ -765,20 +780,29 @@ int use_device(int device) {
 }
 
 template <typename... Args>
-int dependent_launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, void* stream, Args... args) {
+int clustered_launch(void (*kernel)(Args...), dim3 grid, int cluster, int threads, size_t smem, void* stream, Args... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = dim3(threads, 1, 1);
   config.dynamicSmemBytes = smem;
   config.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attr;
-  config.numAttrs = 1;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  config.attrs = attrs;
+  config.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t launched = cudaLaunchKernelEx(&config, kernel, args...);
   if (launched != cudaSuccess) return routing_fail("kernel launch failed: %s", cudaGetErrorString(launched));
   return OG_OK;
+}
+
+template <typename... Args>
+int dependent_launch(void (*kernel)(Args...), dim3 grid, int threads, size_t smem, void* stream, Args... args) {
+  return clustered_launch(kernel, grid, 1, threads, smem, stream, args...);
 }
 
 enum ElementType : int { TYPE_F32 = 0, TYPE_BF16 = 1, TYPE_F16 = 2 };
@@ -930,23 +954,27 @@ OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, co
   const bool glu = activation == ACT_SWIGLU || activation == ACT_GEGLU;
   if (rows < 0 || n < 1 || n % (glu ? 16 : 8)) return routing_fail("rows = %lld, n = %d: columns come in eights", (long long)rows, n);
   if (glu && bias_gradient) return routing_fail("a gated activation has no bias gradient here");
-  if ((rows + GRADIENT_ROWS - 1) / GRADIENT_ROWS > 0x7FFFFFFFll) return routing_fail("rows = %lld are too many", (long long)rows);
+  if (rows > 0x7FFFFFFFll) return routing_fail("rows = %lld are too many", (long long)rows);
   if (const int bad = use_device(device)) return bad;
-  const int blocks = int((rows + GRADIENT_ROWS - 1) / GRADIENT_ROWS);
+  const int block_rows = gradient_block_rows(rows, glu ? n / 2 : n);
+  const int blocks = int((rows + block_rows - 1) / block_rows);
+  const bool one_cluster = bias_gradient && !row_limit && rows && blocks <= GRADIENT_CLUSTER;
   if (rows) {
     if (!grad || (activation && (!z || !dz)) || (bias_gradient && !workspace)) return routing_fail("the gradient's tensors must be device pointers, got null");
     if (!aligned16(grad) || !aligned16(z) || !aligned16(dz)) return routing_fail("gradients and pre-activations must start on 16-byte boundaries");
     ActGradientParams p{};
-    p.grad = grad, p.z = activation ? z : nullptr, p.dz = dz, p.partial = bias_gradient ? workspace : nullptr, p.limit = row_limit;
+    p.grad = grad, p.z = activation ? z : nullptr, p.dz = dz, p.limit = row_limit, p.block_rows = block_rows;
+    if (one_cluster) p.column_sums = bias_gradient;
+    else if (bias_gradient) p.partial = workspace;
     p.rows = rows, p.n = n, p.width = glu ? n / 2 : n, p.glu = glu;
     act_constants(activation, &p.shape, &p.a, &p.b);
     if (!activation && !bias_gradient) return OG_OK;
     const dim3 grid(unsigned(blocks), unsigned((p.width + 255) / 256));
     if (grid.y > 65535) return routing_fail("n = %d is too wide", n);
     const auto kernel = dtype == TYPE_BF16 ? act_gradient_kernel<__nv_bfloat16> : act_gradient_kernel<__half>;
-    if (const int bad = dependent_launch(kernel, grid, 256, 0, stream, p)) return bad;
+    if (const int bad = clustered_launch(kernel, grid, one_cluster ? blocks : 1, 256, 0, stream, p)) return bad;
   }
-  if (!bias_gradient) return OG_OK;
+  if (!bias_gradient || one_cluster) return OG_OK;
   return dependent_launch(column_sum_kernel, dim3(unsigned((n + 31) / 32)), 256, 0, stream, (const float*)workspace, bias_gradient, blocks, int(n));
 }
 

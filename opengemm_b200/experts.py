@@ -18,6 +18,7 @@ from ctypes import byref
 import torch
 
 from . import capi
+from .api import overlap
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
 _GRADIENT_TYPES = {torch.bfloat16: b"bf16", torch.float16: b"f16"}
@@ -35,6 +36,13 @@ def _expect(label, t, dtype, shape, device):
     """Raise unless `t` is a contiguous CUDA tensor of this dtype and shape."""
     if not (t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous() and t.is_cuda):
         raise TypeError(f"{label} must be a contiguous {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _apart(label, t, **others):
+    """Raise if `t`, which a launch writes, shares memory with a tensor that it reads or writes too."""
+    for name, other in others.items():
+        if overlap(t, other):
+            raise ValueError(f"{label} and {name} share memory")
 
 
 def _how(logits, top_k, scores, groups, top_groups, group_top, renormalise, scale):
@@ -184,7 +192,7 @@ def _check_product(x, w, plan, gather, activation, types):
     return name, n, k, gated
 
 
-def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None, out_dtype=None, preactivation=None):
+def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None, preactivation=None):
     """Every row times its own expert's weights: `out[r] = act(alpha[e] * x[r] @ w[e].T)`.
 
     Args:
@@ -199,8 +207,8 @@ def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None,
             has N / 2 columns.
         alpha: float32 `(experts,)`, a factor on each expert's products (the
             dequantisation scales of fp8 operands).
-        out: written instead of a new tensor.
-        out_dtype: bfloat16 or float16; x's own by default, bfloat16 for e4m3.
+        out: written instead of a new tensor; x's dtype, bfloat16 for e4m3.  Neither
+            it nor `preactivation` may share memory with another tensor of the call.
         preactivation: a `(plan.rows, N)` tensor of `out`'s dtype that receives the
             activation's argument, which `expert_gemm_backward` reads.
 
@@ -212,14 +220,14 @@ def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None,
     device, rows = plan.device, plan.rows
     width = n // 2 if gated else n
     own = torch.bfloat16 if x.dtype is torch.float8_e4m3fn else x.dtype
-    if out_dtype not in (None, own):
-        raise TypeError(f"{x.dtype} experts write {own}, not {out_dtype}")
     if out is None:
         out = torch.empty((rows, width), device=device, dtype=own)
     else:
         _expect("out", out, own, (rows, width), device)
+        _apart("out", out, x=x, w=w)
     if preactivation is not None:
         _expect("preactivation", preactivation, own, (rows, n), device)
+        _apart("preactivation", preactivation, out=out, x=x, w=w)
     if alpha is not None:
         _expect("alpha", alpha, torch.float32, (plan.experts,), device)
     if gather and rows > _GATHER_IN_PRODUCT * min(plan.experts, rows):
@@ -326,6 +334,9 @@ def expert_combine(y, weights, plan, residual=None, out=None):
         out = y.new_empty(shape)
     else:
         _expect("out", out, y.dtype, shape, plan.device)
+        _apart("out", out, y=y)
+        if residual is not None and residual.data_ptr() != out.data_ptr():
+            _apart("out", out, residual=residual)
     _combine(y, weights, plan, residual, out, n)
     return out
 

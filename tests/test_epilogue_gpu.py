@@ -17,6 +17,7 @@ PLANS = {
     "heuristic": None,
     "pair256": dict(use_2cta=True, output_n=256),
     "single96": dict(use_2cta=False, output_n=96),
+    "single16": dict(use_2cta=False, output_n=16),
     "swap64": dict(use_2cta=False, output_n=64, swap_ab=True),
     "direct": dict(use_2cta=True, output_n=128, epi_direct=1),
     # schedules that a fused launch leaves for the static one

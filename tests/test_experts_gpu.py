@@ -193,12 +193,13 @@ def check_gemm_gradients(m, n, k, dtype, activation=None, alpha=None, out_dtype=
     a64, b64 = a.double(), b.double()
     assert_within(grad_a, f * (dz @ b64), abs(f) * (sum_error(dz.abs() @ b64.abs(), n + 16) + dz_error @ b64.abs()), "a")
     assert_within(grad_b, f * (dz.T @ a64), abs(f) * (sum_error(dz.abs().T @ a64.abs(), m + 16) + dz_error.T @ a64.abs()), "b")
-    # sums of 8 rows, of 8 row lanes, of blocks of 64 rows
-    assert_within(grad_bias, dz.sum(0), (16 + m / 64) * 2.0**-24 * dz.abs().sum(0) + eval_error.sum(0), "bias")
+    # sums of at most 8 rows, of 8 row lanes, of blocks of 16 or 64 rows in eight lanes
+    assert_within(grad_bias, dz.sum(0), (24 + m / 64) * 2.0**-24 * dz.abs().sum(0) + eval_error.sum(0), "bias")
 
 
 @pytest.mark.parametrize("shape", [(1, 8, 8), (1, 4096, 256), (300, 520, 768), (77, 40, 128), (1001, 136, 264), (4100, 776, 512),
-                                   (36, 4096, 264), (130, 2056, 128), (5001, 64, 72)],  # cut along the reduction
+                                   (36, 4096, 264), (130, 2056, 128), (5001, 64, 72),  # cut along the reduction
+                                   (16, 264, 64), (17, 264, 64), (128, 264, 64), (129, 264, 64), (1024, 264, 64), (9480, 512, 64)],  # the bias's sums
                          ids=lambda s: "x".join(map(str, s)))
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("out_dtype", [None, torch.float32], ids=str)
@@ -234,6 +235,46 @@ def test_gemm_gradients_against_differences_of_the_forward_call():
             want = (loss(*up) - loss(*down)) / 2.0**-11
             # z and dz carry a rounding to float16 each: up to 32 terms of size 4
             assert abs(got.view(-1)[at].item() - want.item()) < 32 * 4 * 2.0**-10
+
+
+def test_no_rows_at_all():
+    plan = og.expert_plan(torch.zeros(0, 2, dtype=torch.int32, device="cuda"), 3)
+    x, w = torch.zeros(0, 64, device="cuda", dtype=torch.bfloat16), torch.ones(3, 32, 64, device="cuda", dtype=torch.bfloat16)
+    for gather in (False, True):
+        assert og.expert_gemm(x, w, plan, gather=gather, activation="swiglu").shape == (0, 16)
+        z = torch.zeros(0, 32, device="cuda", dtype=torch.bfloat16)
+        grad_x, grad_w = og.expert_gemm_backward(z[:, :16].contiguous(), x, w, plan, gather=gather, activation="swiglu", preactivation=z)
+        assert grad_x.shape == (0, 64) and grad_w.shape == w.shape and not grad_w.any()
+    a, b = torch.zeros(0, 64, device="cuda", dtype=torch.float16), torch.ones(32, 64, device="cuda", dtype=torch.float16)
+    z = torch.zeros(0, 32, device="cuda", dtype=torch.float16)
+    grad_a, grad_b, grad_bias = og.gemm_backward(z, a, b, activation="gelu", preactivation=z, want=("a", "b", "bias"))
+    assert grad_a.shape == (0, 64) and not grad_b.any() and not grad_bias.any()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values of output: the last rows are computed and stored in their place."""
+    rows, n, k = 1_100_000, 2048, 64
+    indices = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+    indices[-1000:] = 1
+    plan = og.expert_plan(indices, 2)
+    g = torch.Generator().manual_seed(0)
+    x = torch.zeros(rows, k, device="cuda", dtype=torch.bfloat16)
+    x[-1500:] = values(g, 1500, k, dtype=torch.bfloat16)
+    w = values(g, 2, n, k, dtype=torch.bfloat16)
+    y = og.expert_gemm(x, w, plan)
+    for rows_of, e in ((slice(-1500, -1000), 0), (slice(-1000, None), 1)):
+        want = x[rows_of].double() @ w[e].double().T
+        assert_within(y[rows_of], want, sum_error(x[rows_of].double().abs() @ w[e].double().abs().T, k))
+    assert not y[:-1500].any()
+    out = og.expert_combine(y, torch.full((rows, 1), 2.0, device="cuda"), plan)
+    assert torch.equal(out[-1500:], y[-1500:] * 2)
+    del out
+    residual = torch.zeros_like(y)
+    residual[-700:] = 1
+    c = og.gemm(x, w[1], out_dtype=torch.bfloat16, activation="relu", residual=residual)
+    want = torch.relu(x[-1500:].double() @ w[1].double().T) + residual[-1500:].double()
+    assert_within(c[-1500:], want, sum_error(x[-1500:].double().abs() @ w[1].double().abs().T, k) + 2.0**-23 * want.abs())
+    assert not c[:-1500].any()
 
 
 def layer(x, logits, w1, w2, top_k):
@@ -350,8 +391,13 @@ def test_refusals():
         og.expert_gemm(x, w, plan, alpha=torch.ones(2, device="cuda"))
     with pytest.raises(TypeError, match="out must"):
         og.expert_gemm(x, w, plan, out=torch.zeros(8, 32, device="cuda"))
-    with pytest.raises(TypeError, match="write"):
-        og.expert_gemm(x, w, plan, out_dtype=torch.float32)
+    square = torch.zeros(3, 64, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="share memory"):
+        og.expert_gemm(x, square, plan, out=x)
+    with pytest.raises(ValueError, match="share memory"):
+        og.expert_gemm(x, square, plan, activation="relu", preactivation=x)
+    with pytest.raises(ValueError, match="share memory"):
+        og.expert_combine(x, torch.zeros(4, 2, device="cuda"), plan, out=x[:4])
     with pytest.raises(ValueError, match="16-byte"):
         og.expert_gemm(torch.zeros(8 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(8, 64), w, plan)
     grad = torch.zeros(8, 32, device="cuda", dtype=torch.bfloat16)
