@@ -137,27 +137,28 @@ __device__ __forceinline__ void activate_all(float* v, float a, float b) {
   }
 }
 
-// The activation and its derivative at x.
+// The activation and its derivative at two values.
 template <int SHAPE>
-__device__ __forceinline__ void act_both(float x, float a, float b, float* value, float* slope) {
+__device__ __forceinline__ void act_both2(float2 x, float a, float b, float2* value, float2* slope) {
   if constexpr (SHAPE == SHAPE_RELU) {
-    *value = x < 0.0f ? 0.0f : x;
-    *slope = x > 0.0f ? 1.0f : (x == x ? 0.0f : x);
+    *value = make_float2(x.x < 0.0f ? 0.0f : x.x, x.y < 0.0f ? 0.0f : x.y);
+    *slope = make_float2(x.x > 0.0f ? 1.0f : (x.x == x.x ? 0.0f : x.x), x.y > 0.0f ? 1.0f : (x.y == x.y ? 0.0f : x.y));
   } else if constexpr (SHAPE == SHAPE_PHI) {
-    float e;
-    const float tail = lower_tail(x, &e);
-    const float cdf = x > 0.0f ? 1.0f - tail : tail;
-    *value = x * cdf;
-    *slope = fmaf(x * 0.3989422804014327f, e, cdf);
-  } else if constexpr (SHAPE == SHAPE_SIGMOID) {
-    // p' = p (1 - p) t' with t' = -ln(2) (a + 3 b x^2)
-    const float q = fminf(x * x, 1e8f);
-    const float p = reciprocal_fast(1.0f + exp2_fast(x * fmaf(b, q, a)));
-    *value = x * p;
-    *slope = fmaf(x * p * (1.0f - p), -0.6931471805599453f * fmaf(3.0f * b, q, a), p);
+    float2 e;
+    const float2 tail = make_float2(lower_tail(x.x, &e.x), lower_tail(x.y, &e.y));
+    const float2 cdf = make_float2(x.x > 0.0f ? 1.0f - tail.x : tail.x, x.y > 0.0f ? 1.0f - tail.y : tail.y);
+    *value = mul2(x, cdf);
+    *slope = fma2(mul2(x, both(0.3989422804014327f)), e, cdf);
   } else {
-    *value = x;
-    *slope = 1.0f;
+    // p' = p (1 - p) t' with t = -ln(2) (a x + b x^3)
+    float2 q = mul2(x, x);
+    q = make_float2(fminf(q.x, 1e8f), fminf(q.y, 1e8f));
+    const float2 t = mul2(x, fma2(both(b), q, both(a)));
+    const float2 p = make_float2(reciprocal_fast(1.0f + exp2_fast(t.x)), reciprocal_fast(1.0f + exp2_fast(t.y)));
+    constexpr float LN2 = 0.6931471805599453f;
+    const float2 d = fma2(both(-3.0f * LN2 * b), q, both(-LN2 * a));
+    *value = mul2(x, p);
+    *slope = fma2(mul2(*value, fma2(p, both(-1.0f), both(1.0f))), d, p);
   }
 }
 

@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -675,17 +676,18 @@ __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientPara
   const T* z = static_cast<const T*>(p.z);
   T* dz = static_cast<T*>(p.dz);
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto slopes = [&](const float* x, float* value, float* slope) {
-    if (p.shape == SHAPE_SIGMOID) {
+  auto slopes_as = [&](auto shape, const float* x, float* value, float* slope) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) act_both<SHAPE_SIGMOID>(x[i], p.a, p.b, value + i, slope + i);
-    } else if (p.shape == SHAPE_PHI) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) act_both<SHAPE_PHI>(x[i], 0.f, 0.f, value + i, slope + i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) act_both<SHAPE_RELU>(x[i], 0.f, 0.f, value + i, slope + i);
+    for (int i = 0; i < 8; i += 2) {
+      float2 v, d;
+      act_both2<decltype(shape)::value>(make_float2(x[i], x[i + 1]), p.a, p.b, &v, &d);
+      value[i] = v.x, value[i + 1] = v.y, slope[i] = d.x, slope[i + 1] = d.y;
     }
+  };
+  auto slopes = [&](const float* x, float* value, float* slope) {
+    if (p.shape == SHAPE_SIGMOID) slopes_as(std::integral_constant<int, SHAPE_SIGMOID>{}, x, value, slope);
+    else if (p.shape == SHAPE_PHI) slopes_as(std::integral_constant<int, SHAPE_PHI>{}, x, value, slope);
+    else slopes_as(std::integral_constant<int, SHAPE_RELU>{}, x, value, slope);
   };
 #pragma unroll 2
   for (int r = row_lane; r < p.block_rows; r += 8) {

@@ -208,7 +208,7 @@ def test_plan_of_extreme_indices():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
-@pytest.mark.parametrize("tokens,top_k,n", [(1, 1, 8), (16, 8, 2048), (33, 3, 1037), (130, 2, 264)])
+@pytest.mark.parametrize("tokens,top_k,n", [(1, 1, 8), (16, 8, 2048), (33, 3, 1037), (130, 2, 264), (257, 2, 2056), (300, 5, 4096)])
 @pytest.mark.parametrize("residual", [False, True])
 def test_combine_and_its_gradient(tokens, top_k, n, residual, dtype):
     g = torch.Generator().manual_seed(n)
