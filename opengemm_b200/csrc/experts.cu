@@ -245,7 +245,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   const int y_rows = plan.tile_n / plan.cta_group;  // of the N side, per CTA: a multiple of 64
   p.y_bytes = y_rows * 128;
   p.stage_bytes = 16384 + p.y_bytes;
-  p.stages = std::min(XP_MAX_STAGES, (SMEM_LIMIT - XP_STATIC_SMEM - 1024 - XP_EPILOGUE_WARPS * XP_STAGING) / p.stage_bytes);
+  p.stages = std::min(XP_MAX_STAGES, (SMEM_LIMIT - XP_STATIC_SMEM - 1024 - xp_staging_bytes(out_bytes)) / p.stage_bytes);
   p.tmem_cols = pow2_at_least(2 * plan.tile_n);
   const uint32_t x_columns = mode == MODE_DW, y_columns = mode != MODE_FORWARD;
   const uint32_t fmt = bf16 ? 1u : 0u;  // e4m3 is code 0 of its kind, f16 of its own
@@ -292,7 +292,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   const int64_t m_tiles = mode == MODE_DW ? int64_t(p.groups) * p.tiles_m_fixed
                                           : (int64_t(g.rows) / (128 * plan.cta_group) + std::min(g.groups, g.rows)) * parts;
   const int clusters = int(std::min<int64_t>(sm_count / plan.cta_group, m_tiles * p.tiles_n));
-  const int smem = p.stages * p.stage_bytes + XP_EPILOGUE_WARPS * XP_STAGING + 1024;
+  const int smem = p.stages * p.stage_bytes + xp_staging_bytes(out_bytes) + 1024;
   const cudaError_t launched = kernel->launch(p, std::max(1, clusters) * plan.cta_group, smem, s);
   if (launched != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "kernel launch failed: %s", cudaGetErrorString(launched));
   return OG_OK;

@@ -36,11 +36,11 @@ enum ExpertMode : int { MODE_FORWARD = 0, MODE_DX = 1, MODE_DW = 2 };
 constexpr int XP_MAX_STAGES = 12;
 constexpr int XP_MAX_GROUPS = 1024;
 constexpr int XP_CHUNK = 32;  // columns an epilogue warp works on at a time
-constexpr int XP_STAGING = 32 * XP_CHUNK * 4;  // per epilogue warp: its 32 rows of a chunk
 
 // Two epilogue warps per quarter of the accumulator's rows, taking turns at its
 // columns: a weight gradient over few rows is all stores.
 constexpr int XP_EPILOGUE_WARPS = 8;
+constexpr int xp_staging_bytes(int out_bytes) { return XP_EPILOGUE_WARPS * 32 * XP_CHUNK * out_bytes; }  // each warp's 32 rows of a chunk
 __host__ __device__ constexpr int xp_threads(int mode) { return 64 + 32 * XP_EPILOGUE_WARPS + (mode == MODE_DW ? 32 : 0); }
 
 struct alignas(64) ExpertParams {
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     const int quarter = warp & 3;
     const uint32_t lane_base = uint32_t(quarter * 32) << 16;
     const uint32_t acc_empty_leader = CTA_GROUP == 2 ? map_to_cta(bar_acc_empty, 0) : bar_acc_empty;
-    const uint32_t my_buf = staging + (warp - 2) * XP_STAGING;
+    const uint32_t my_buf = staging + (warp - 2) * 32 * ROW_BYTES;
     const int sub_row = lane / UNITS, unit = lane % UNITS;
     // 16-byte unit u of staging row r, swizzled so that eight lanes on eight rows,
     // or on the units of one row, touch all banks.
