@@ -8,6 +8,8 @@ of the operands' device, and validation raises the same TypeError /
 ValueError texts (api.py:25-63).
 """
 
+from ctypes import addressof
+
 import torch
 
 from . import capi
@@ -29,6 +31,8 @@ def forget(name=None):
     """Drop memoised bindings (after the stored configurations changed)."""
     for key in [key for key in _bound if name is None or base_name(key[0]) == name]:
         del _bound[key]
+    if capi._front:
+        capi._front.forget()
 
 
 def scale_bytes(d, rows, k):
@@ -149,6 +153,14 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
         `out_dtype=torch.bfloat16`, float16 with `out_dtype=torch.float16`), int32
         for s8 and u8, bfloat16 for block-scaled ones.
     """
+    fused = activation is not None or residual is not None or preactivation is not None
+    front = capi.front() if fused and out is None and out_format is None and atype is None and btype is None else None
+    if front is not None:
+        c = front.gemm(a, b, sfa, sfb, out_dtype, alpha, bias, capi.ACTIVATIONS.get(activation), residual, preactivation,
+                       capi._independent_inputs)
+        if c is not None:
+            return c
+    asked = out_dtype
     name = dtype_name(a, b, sfa, atype, btype)
     if out_format is not None:
         if residual is not None or preactivation is not None:
@@ -170,11 +182,14 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
             and residual.device == a.device:
         out = torch.empty_like(residual)  # the cheapest way to one
     out = output(d, m, n, out, a.device)
-    if activation is not None or residual is not None or preactivation is not None:
+    if fused:
         check_epilogue(name, d, m, n, out, activation, residual, preactivation)
         if bias is not None:
             check_bias(bias, n, a.device)
         lib.launch_fused(g, a, b, sfa, sfb, out, alpha, bias, activation, residual, preactivation)
+        if front is not None:
+            scales = (0, 0) if sfa is None else (scale_bytes(d, m, k), scale_bytes(d, n, k))
+            front.learn(a, b, sfa, asked, capi._independent_inputs, addressof(g), d.out, *scales)
         return out
     if alpha is None and bias is None:
         lib.launch(g, a, b, sfa, sfb, out)
@@ -213,6 +228,12 @@ def gemm_backward(grad, a, b, activation=None, preactivation=None, alpha=None, w
         `(grad_a, grad_b, grad_bias)`, None in the place of what is not wanted;
         `grad_bias` is float32.
     """
+    front = capi.front()
+    if front is not None and (out_dtype is None or out_dtype is a.dtype) and set(want) <= {"a", "b", "bias"}:
+        done = front.gemm_backward(grad, a, b, capi.ACTIVATIONS.get(activation), preactivation, alpha, "a" in want, "b" in want,
+                                   "bias" in want)
+        if done is not None:
+            return done
     if not a.is_cuda or a.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"gradients are served for bfloat16 and float16 CUDA operands, got {a.dtype} on {a.device}")
     name = "bf16" if a.dtype is torch.bfloat16 else "f16"

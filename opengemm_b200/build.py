@@ -143,6 +143,63 @@ def compile_library(verbose=False, out=None):
     return target
 
 
+FRONT_NAME = "front.so"
+
+
+def front_hash():
+    """A digest of what the host path's extension is built from: its source, the C header and torch's version."""
+    import torch
+
+    digest = hashlib.blake2s(digest_size=8)
+    for path in (CSRC / "front.cpp", ROOT / "include" / "opengemm_b200.h"):
+        digest.update(path.read_bytes())
+    digest.update(f"{torch.__version__} {sys.version_info[:2]}".encode())
+    return digest.hexdigest()
+
+
+def compile_front(out=None):
+    """Compile the host path's extension (csrc/front.cpp) against the installed torch; `out`
+    defaults to the in-tree file.  A digest beside it says what it was built from."""
+    import sysconfig
+
+    import torch
+
+    target = Path(out) if out is not None else LIB_DIR / FRONT_NAME
+    target.parent.mkdir(parents=True, exist_ok=True)
+    at = Path(torch.__file__).resolve().parent
+    home = Path(os.environ.get("CUDA_HOME") or "/usr/local/cuda")
+    includes = [at / "include", at / "include" / "torch" / "csrc" / "api" / "include", home / "include",
+                sysconfig.get_paths()["include"]]
+    temporary = target.parent / f"{FRONT_NAME}.{os.getpid()}.tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[flag for path in includes for flag in ("-isystem", str(path))], str(CSRC / "front.cpp"), "-o", str(temporary),
+           f"-L{at / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cuda", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    done = subprocess.run(cmd, capture_output=True, text=True)
+    if done.returncode != 0:
+        temporary.unlink(missing_ok=True)
+        raise RuntimeError("the host path's extension does not build:\n" + (done.stderr or done.stdout))
+    temporary.replace(target)
+    target.with_suffix(".stamp").write_text(front_hash())
+    return target
+
+
+def front_path():
+    """The host path's extension, compiled now if missing or stale; None when it cannot be."""
+    for folder in (LIB_DIR, cache_dir() / front_hash()):
+        target = folder / FRONT_NAME
+        try:
+            if not (target.exists() and target.with_suffix(".stamp").read_text() == front_hash()):
+                compile_front(target)
+            return target
+        except PermissionError:
+            continue
+        except (OSError, RuntimeError) as exc:
+            log(f"calls go through the interpreter: {exc}")
+            return None
+    return None
+
+
 def cached_library():
     """The library under the cache directory for this exact build, compiled on first use."""
     out = cache_dir() / build_hash() / LIB_NAME
@@ -178,8 +235,10 @@ def prebuild():
     """Compile the library now rather than on the first gemm() (opengemm/python/build.py:128-132)."""
     if stale():
         compile_library(verbose=True)
+    front_path()
     return library_file()
 
 
 if __name__ == "__main__":
     compile_library(verbose=True)
+    compile_front()

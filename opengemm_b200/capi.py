@@ -470,6 +470,53 @@ def independent_inputs():
     return _independent_inputs
 
 
+_FRONT_SYMBOLS = ("route", "route_gradient", "expert_plan", "expert_gather", "expert_product", "expert_combine",
+                  "expert_combine_gradient", "activation_gradient", "gemm_gradients", "gemm_gradients_workspace",
+                  "launch_fused", "routing_error", "experts_error")
+_front = False  # not looked for yet
+
+
+def front():
+    """The host path's extension (csrc/front.cpp), bound to the loaded library, or None: it is not
+    there, OPENGEMM_FRONT=0, or the library is one without these entry points.  The calls it does
+    not serve, and all of them without it, go through this module; the kernels are the same."""
+    global _front
+    if _front is False:
+        _front = _load_front()
+    return _front
+
+
+def _load_front():
+    import importlib.util
+    import os
+
+    lib = library("mm")
+    if os.environ.get("OPENGEMM_FRONT") == "0" or lib._plan is None:
+        return None
+    path = build.front_path()
+    if path is None:
+        return None
+    try:
+        spec = importlib.util.spec_from_file_location("front", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except ImportError as exc:
+        build.log(f"calls go through the interpreter: {exc}")
+        return None
+    addresses = {"og_b200_" + name: ctypes.cast(getattr(lib._lib, "og_b200_" + name), c_void_p).value for name in _FRONT_SYMBOLS}
+    addresses["og_mm_error"] = ctypes.cast(lib._lib.og_mm_error, c_void_p).value
+    module.bind(addresses)
+    return module
+
+
+def use_front(yes):
+    """Turn the host path's extension on (default) or off for this process; returns the previous setting."""
+    global _front
+    before = _front is not None
+    _front = False if yes else None
+    return before
+
+
 def library(impl):
     """The loaded library for `impl`, loading it on first use."""
     loaded = _libraries.get(impl)

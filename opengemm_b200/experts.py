@@ -78,6 +78,11 @@ def route(logits, top_k, scores="softmax", bias=None, groups=1, top_groups=1, gr
         `top_k` experts to choose from, the places left have index -1 and weight
         0.  A NaN logit ranks first and makes its token's weights NaN.
     """
+    front = capi.front()
+    if front is not None:
+        done = front.route(logits, top_k, _SCORES.get(scores), bias, groups, top_groups, group_top, bool(renormalise), scale)
+        if done is not None:
+            return done
     how = _how(logits, top_k, scores, groups, top_groups, group_top, renormalise, scale)
     if bias is not None:
         _expect("bias", bias, torch.float32, (how.experts,), logits.device)
@@ -95,6 +100,11 @@ def route_backward(grad_weights, logits, indices, scores="softmax", renormalise=
     The choice itself has no gradient: `indices` are those `route` returned, and
     `scores`, `renormalise` and `scale` those it was called with.
     """
+    front = capi.front()
+    if front is not None:
+        done = front.route_backward(grad_weights, logits, indices, _SCORES.get(scores), bool(renormalise), scale)
+        if done is not None:
+            return done
     how = _how(logits, indices.size(1) if indices.dim() == 2 else 0, scores, 1, 1, 1, renormalise, scale)
     _expect("indices", indices, torch.int32, (how.tokens, how.top_k), logits.device)
     _expect("grad_weights", grad_weights, torch.float32, (how.tokens, how.top_k), logits.device)
@@ -115,18 +125,19 @@ class ExpertPlan:
     neither read nor written.  The three int32 tensors are views of one buffer.
     """
 
-    __slots__ = ("experts", "token_count", "top_k", "rows", "device", "_store", "_offsets", "_tokens", "_positions", "_limit")
+    __slots__ = ("experts", "token_count", "top_k", "rows", "device", "_store", "_offsets", "_tokens", "_positions", "_limit",
+                 "_native")
 
-    def __init__(self, indices, experts):
-        self.experts, self.device = experts, indices.device
-        self.token_count, self.top_k = indices.shape
-        rows = self.rows = self.token_count * self.top_k  # of the tensors in the plan's order
-        self._store = torch.empty(experts + 1 + 2 * rows, device=indices.device, dtype=torch.int32)
+    def __init__(self, experts, device, token_count, top_k, store, address):
+        self.experts, self.device, self.token_count, self.top_k = experts, device, token_count, top_k
+        rows = self.rows = token_count * top_k  # of the tensors in the plan's order
+        self._store = store
         # addresses that the launches take: the first rows (and, behind the last of them, how many rows there are) ...
-        self._offsets = self._store.data_ptr()
-        self._limit = self._offsets + 4 * experts
+        self._offsets = address
+        self._limit = address + 4 * experts
         self._tokens = self._limit + 4
         self._positions = self._tokens + 4 * rows
+        self._native = (experts, token_count, top_k, device.index, address)  # ... and what the native host path takes
 
     @property
     def offsets(self):
@@ -152,13 +163,20 @@ def expert_plan(indices, experts):
     Returns:
         An `ExpertPlan`; the same indices always give the same plan.
     """
+    front = capi.front()
+    if front is not None:
+        made = front.expert_plan(indices, experts, _PLAN_CHUNK)
+        if made is not None:
+            store, address, token_count, top_k = made
+            return ExpertPlan(experts, store.device, token_count, top_k, store, address)
     if not (indices.dtype is torch.int32 and indices.is_cuda and indices.dim() == 2 and indices.is_contiguous()):
         raise TypeError("indices must be a contiguous 2-D int32 CUDA tensor")
     if indices.size(1) < 1:
         raise ValueError("indices must name at least one expert per token")
     if not 1 <= experts <= 1024:
         raise ValueError(f"{experts} experts: 1 to 1024 are served")
-    plan = ExpertPlan(indices, experts)
+    store = torch.empty(experts + 1 + 2 * indices.numel(), device=indices.device, dtype=torch.int32)
+    plan = ExpertPlan(experts, indices.device, indices.size(0), indices.size(1), store, store.data_ptr())
     workspace = None
     if plan.rows > _PLAN_CHUNK:
         workspace = torch.empty(-(-plan.rows // _PLAN_CHUNK) * experts, device=indices.device, dtype=torch.int32)
@@ -216,6 +234,11 @@ def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None,
         `(plan.rows, N or N / 2)` rows in the plan's order.  Rows behind the plan's
         last are left as they were.
     """
+    front = capi.front()
+    if front is not None and out is None:
+        done = front.expert_gemm(x, w, plan._native, gather, _ACTIVATIONS.get(activation), alpha, preactivation, _GATHER_IN_PRODUCT)
+        if done is not None:
+            return done
     name, n, k, gated = _check_product(x, w, plan, gather, activation, _PRODUCT_TYPES)
     device, rows = plan.device, plan.rows
     width = n // 2 if gated else n
@@ -276,6 +299,12 @@ def expert_gemm_backward(grad, x, w, plan, gather=False, activation=None, preact
     Returns:
         `(grad_x, grad_w)`, None in the place of what is not wanted.
     """
+    front = capi.front()
+    if front is not None and (out_dtype is None or out_dtype is x.dtype) and set(want) <= {"x", "w"}:
+        done = front.expert_gemm_backward(grad, x, w, plan._native, gather, _ACTIVATIONS.get(activation), preactivation, "x" in want,
+                                          "w" in want)
+        if done is not None:
+            return done
     name, n, k, gated = _check_product(x, w, plan, gather, activation, _GRADIENT_TYPES)
     if n % 8:
         raise ValueError(f"N must be a multiple of 8, got {n}")
@@ -326,6 +355,11 @@ def expert_combine(y, weights, plan, residual=None, out=None):
     Returns:
         `(tokens, N)` of y's dtype, summed in float32 in the order of the choices.
     """
+    front = capi.front()
+    if front is not None and out is None:
+        done = front.expert_combine(y, weights, plan._native, residual)
+        if done is not None:
+            return done
     n = _check_combine(y, weights, plan)
     shape = (plan.token_count, n)
     if residual is not None:
@@ -361,6 +395,11 @@ def expert_combine_backward(grad, y, weights, plan):
     holds `<grad[t], y[row of (t, j)]>`, 0 for a pair that goes nowhere.  The
     residual's gradient is `grad` itself.
     """
+    front = capi.front()
+    if front is not None:
+        done = front.expert_combine_backward(grad, y, weights, plan._native)
+        if done is not None:
+            return done
     n = _check_combine(y, weights, plan)
     _expect("grad", grad, y.dtype, (plan.token_count, n), plan.device)
     grad_y, grad_weights = torch.empty_like(y), torch.empty_like(weights)

@@ -13,6 +13,15 @@ from tests.gemm_util import make_case, to_device
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(params=["native", "interpreter"], autouse=True)
+def host_path(request):
+    """Every test runs through the native host path and through the Python one."""
+    before = capi.use_front(request.param == "native")
+    assert (capi.front() is not None) == (request.param == "native")
+    yield
+    capi.use_front(before)
+
 PLANS = {
     "heuristic": None,
     "pair256": dict(use_2cta=True, output_n=256),
@@ -66,7 +75,13 @@ def check(name, m, n, k, out_dtype, activation, bias=True, residual=True, save=T
     z = torch.full((m, n), float("nan"), device="cuda", dtype=out_dtype) if save else None
     out = torch.full((m, n), float("nan"), device="cuda", dtype=out_dtype)
     if plan is None:
-        og.gemm(a, b, sfa, sfb, out=out, alpha=alpha, bias=bias, activation=activation, residual=residual, preactivation=z, **element_names(name))
+        fused = dict(alpha=alpha, bias=bias, activation=activation, residual=residual, preactivation=z, **element_names(name))
+        og.gemm(a, b, sfa, sfb, out=out, **fused)
+        for _ in range(2):  # the second call finds what the first one bound
+            if save:
+                z.fill_(float("nan"))
+            again = og.gemm(a, b, sfa, sfb, out_dtype=out_dtype, **fused)
+            assert torch.equal(again, out)
     else:
         config = heuristic_config(name, m, n, k)
         config.update(plan, cluster_m=2 if plan["use_2cta"] else 1)

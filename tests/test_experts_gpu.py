@@ -4,9 +4,19 @@ import pytest
 import torch
 
 import opengemm_b200 as og
+from opengemm_b200 import capi
 from tests.feed_forward_util import HALF_STEP, act, act_error, act_gradient, assert_within, sum_error
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "interpreter"], autouse=True)
+def host_path(request):
+    """Every test runs through the native host path and through the Python one."""
+    before = capi.use_front(request.param == "native")
+    assert (capi.front() is not None) == (request.param == "native")
+    yield
+    capi.use_front(before)
 
 
 def routed(tokens, top_k, experts, seed=0, dropped=True):
@@ -62,6 +72,10 @@ def check(tokens, top_k, experts, n, k, dtype=torch.bfloat16, gather=True, activ
     out = torch.full((plan.rows, n // 2 if gated else n), 7.0, device="cuda", dtype=own)
     z = torch.full((plan.rows, n), 7.0, device="cuda", dtype=own) if save else None
     assert og.expert_gemm(x, w, plan, gather=gather, activation=activation, alpha=alpha, out=out, preactivation=z) is out
+    if save:
+        z_too = torch.empty_like(z)
+    again = og.expert_gemm(x, w, plan, gather=gather, activation=activation, alpha=alpha, preactivation=z_too if save else None)
+    assert torch.equal(again[:last], out[:last]) and (not save or torch.equal(z_too[:last], z[:last]))
     rows = x[plan.tokens.clamp(0, tokens - 1).long()] if gather else x
     want_z, error = reference(rows, w, plan, alpha)
     if save:

@@ -152,6 +152,33 @@ def test_structures_match_the_header(tmp_path):
     assert got == want
 
 
+def test_the_native_host_path_leaves_what_it_does_not_serve_to_the_python_one():
+    """It answers None, whatever it is given, and the Python front end raises what there is to raise."""
+    front = capi.front()
+    assert front is not None
+    cpu = torch.zeros(4, 8)
+    plan = (3, 4, 2, 0, SOME)
+    calls = {
+        "route": [(cpu, 2, 0, None, 1, 1, 2, 1, 1.0), (None, 2, 0, None, 1, 1, 2, 1, 1.0), ("logits", "2", 0, None, 1, 1, 2, 1, 1.0), ()],
+        "route_backward": [(cpu, cpu, cpu.int(), 0, 1, 1.0), (None,) * 6],
+        "expert_plan": [(cpu.int(), 3, 8192), (None, 3, 8192), (cpu.int(), "3", 8192)],
+        "expert_gemm": [(cpu, cpu, plan, False, 0, None, None, 16), (cpu, cpu, None, False, 0, None, None, 16), (cpu, cpu, (1, 2), False, 0, None, None, 16)],
+        "expert_gemm_backward": [(cpu, cpu, cpu, plan, False, 0, None, True, True)],
+        "expert_combine": [(cpu, cpu, plan, None), (cpu, cpu, (3, 4, 2, 0, -1), None)],
+        "expert_combine_backward": [(cpu, cpu, cpu, plan)],
+        "gemm": [(cpu, cpu, None, None, None, None, None, 1, None, None, False), (cpu, None, None, None, torch.bfloat16, 1.0, None, None, None, None, False)],
+        "gemm_backward": [(cpu, cpu, cpu, 0, None, None, True, True, True)],
+        "learn": [(cpu, cpu, None, None, False, SOME, torch.float32, 0, 0)],
+    }
+    for name, all_args in calls.items():
+        for args in all_args:
+            assert getattr(front, name)(*args) is None, (name, args)
+    with pytest.raises(RuntimeError, match="missing"):
+        front.bind({})
+    capi.use_front(True)
+    assert capi.front() is not None  # bound again
+
+
 def test_calls_on_cpu_tensors_are_refused():
     x, w = torch.zeros(8, 64, dtype=torch.bfloat16), torch.zeros(3, 32, 64, dtype=torch.bfloat16)
     with pytest.raises(TypeError):

@@ -4,9 +4,19 @@ import pytest
 import torch
 
 import opengemm_b200 as og
+from opengemm_b200 import capi
 from tests.feed_forward_util import assert_within
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "interpreter"], autouse=True)
+def host_path(request):
+    """Every test runs through the native host path and through the Python one."""
+    before = capi.use_front(request.param == "native")
+    assert (capi.front() is not None) == (request.param == "native")
+    yield
+    capi.use_front(before)
 
 INF = float("inf")
 
