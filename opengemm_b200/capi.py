@@ -56,7 +56,7 @@ class OgExpertProduct(ctypes.Structure):
 
     _fields_ = ([(f, c_void_p) for f in ("x", "w", "offsets", "tokens", "alpha", "out", "preactivation")]
                 + [(f, c_int32) for f in ("mode", "groups", "rows", "x_rows", "n", "k", "activation", "out_f32")]
-                + [("factor", ctypes.c_float), ("dtype", c_char * 16)])
+                + [("factor", ctypes.c_float), ("beside_previous", c_int32), ("dtype", c_char * 16)])
 
 
 class OgGemmGradients(ctypes.Structure):
@@ -365,14 +365,15 @@ class Library:
             raise RuntimeError(self.error())
 
     def expert_product(self, mode, dtype, x, w, out, groups, rows, n, k, offsets=0, tokens=0, x_rows=0, alpha=None,
-                       activation=0, preactivation=None):
+                       activation=0, preactivation=None, beside_previous=False):
         """One launch of og_b200_expert_product on CUDA tensors, on the current stream of `out`'s
-        device; `offsets` and `tokens` are addresses."""
+        device; `offsets` and `tokens` are addresses.  `beside_previous` vouches that the stream's
+        previous launch was this method's and writes nothing that this one touches."""
         device = out.get_device()
         product = OgExpertProduct(
             x.data_ptr(), w.data_ptr(), offsets, tokens, 0 if alpha is None else alpha.data_ptr(), out.data_ptr(),
             0 if preactivation is None else preactivation.data_ptr(), mode, groups, rows, x_rows, n, k, activation,
-            out.dtype is torch.float32, 1.0, dtype,
+            out.dtype is torch.float32, 1.0, beside_previous, dtype,
         )
         if self._expert_product(byref(product), device, raw_stream(device)) != OG_OK:
             raise RuntimeError(self._experts_error().decode())

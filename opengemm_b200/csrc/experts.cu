@@ -255,6 +255,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   p.tokens = g.tokens;
   p.alpha = g.alpha;
   p.factor = g.factor;
+  p.beside = g.beside_previous != 0;
   p.d = g.out;
   p.preact = g.preactivation;
   p.wait_limit_ns = current_wait_limit_ns();
@@ -376,6 +377,8 @@ OG_API int32_t og_b200_gemm_gradients(const OgGemmGradients* g, int32_t device, 
     const int parts = mode == MODE_DX ? s.parts_a : s.parts_b;
     product.mode = mode, product.w = mode == MODE_DX ? g->b : g->a;
     product.out = parts > 1 ? sums : out, product.out_f32 = parts > 1 ? 1 : g->out_f32;
+    // The second product reads nothing of the first's, unless they share the partial sums' space.
+    product.beside_previous = mode == MODE_DW && g->grad_a && s.parts_a == 1;
     int rc = launch_product(product, device, stream, parts);
     if (rc != OG_OK) return rc;
     if (parts == 1) continue;

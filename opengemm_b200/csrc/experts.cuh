@@ -73,6 +73,7 @@ struct alignas(64) ExpertParams {
   float act_a, act_b;
   int out_f16;
   int tmem_cols;
+  int beside;           // runs beside the stream's previous launch (see below)
 };
 
 // One tile of work: group, its rows, and the tile's place.
@@ -177,7 +178,13 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     }
   }
   // The offsets are an earlier kernel's output, like everything else read here.
-  pdl_wait_prior_grids();
+  //
+  // `beside`: the stream's previous launch is such a kernel too, and writes
+  // nothing that this one touches.  Its blocks let this grid start only after
+  // their own wait has returned, so whatever came before it is complete: this
+  // grid need not wait, and fills the SMs that the other's last wave leaves
+  // idle.  It waits before it ends, so that completion stays transitive.
+  if (!p.beside) pdl_wait_prior_grids();
   if (threadIdx.x == 0) pdl_launch_dependents();
 
   // Group table: rows and tiles before each group.  Warp 2 sums; a lane takes a
@@ -556,6 +563,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     }
   }
 
+  if (p.beside) pdl_wait_prior_grids();
   tc_fence_before_sync();
   __syncthreads();
   if (CTA_GROUP == 2) cluster_sync_all();

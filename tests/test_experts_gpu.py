@@ -227,6 +227,36 @@ def test_gemm_gradients_through_activations(activation):
     check_gemm_gradients(130, 520, 72, torch.float16, activation)
 
 
+def test_two_gradients_side_by_side_are_those_one_after_the_other():
+    """The second product does not wait for the first: the same bits as when each is alone on the stream."""
+    torch.manual_seed(6)
+    sizes = [(300, 520, 768), (2048, 1024, 512), (1001, 136, 264), (64, 4096, 256), (4100, 776, 512)]
+    sets, alone = [], []
+    for m, n, k in sizes:
+        a, b = torch.randn(m, k).bfloat16().cuda(), torch.randn(n, k).bfloat16().cuda()
+        grad, z = torch.randn(m, n).bfloat16().cuda(), torch.randn(m, n).bfloat16().cuda()
+        sets.append((grad, a, b))
+        each = []
+        for want in ("a", "b"):
+            each.append([t for t in og.gemm_backward(*sets[-1], activation="gelu", preactivation=z, want=(want,)) if t is not None][0].clone())
+            torch.cuda.synchronize()
+        sets[-1] += (z,)
+        alone.append(each)
+    for _ in range(20):
+        gots = [og.gemm_backward(grad, a, b, activation="gelu", preactivation=z, want=("a", "b", "bias")) for grad, a, b, z in sets]
+        for got, want in zip(gots, alone):
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    plan = og.expert_plan(routed(900, 3, 7, seed=5), 7)
+    x, w = torch.randn(900, 264).half().cuda(), torch.randn(7, 320, 264).half().cuda()
+    grad, z = torch.randn(plan.rows, 160).half().cuda(), torch.randn(plan.rows, 320).half().cuda()
+    run = lambda want: og.expert_gemm_backward(grad, x, w, plan, gather=True, activation="swiglu", preactivation=z, want=want)  # noqa: E731
+    want_x, want_w = run(("x",))[0].clone(), run(("w",))[1].clone()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        grad_x, grad_w = run(("x", "w"))
+        assert torch.equal(grad_x, want_x) and torch.equal(grad_w, want_w)
+
+
 def test_gemm_gradients_against_differences_of_the_forward_call():
     torch.manual_seed(0)
     m, n, k = 24, 32, 16

@@ -71,7 +71,7 @@ def test_combine_gather_and_activation_gradient_refuse():
 
 def product(**changes):
     fields = dict(x=SOME, w=SOME, offsets=SOME, tokens=0, alpha=0, out=SOME, preactivation=0, mode=0, groups=4, rows=8, x_rows=8, n=64, k=64, activation=0, out_f32=0,
-                  factor=1.0, dtype=b"bf16")
+                  factor=1.0, beside_previous=0, dtype=b"bf16")
     fields.update(changes)
     return capi.OgExpertProduct(**fields)
 
