@@ -78,7 +78,7 @@ def test_choice_and_weights(scores, tokens, experts, top_k, dtype):
         assert_within(weights.cpu(), want, SCORE_ERROR * want.abs())
 
 
-@pytest.mark.parametrize("groups,each,top_groups,group_top", [(8, 32, 4, 2), (4, 16, 1, 1), (2, 5, 2, 2), (3, 1, 2, 2), (32, 3, 7, 2)])
+@pytest.mark.parametrize("groups,each,top_groups,group_top", [(8, 32, 4, 2), (4, 16, 1, 1), (2, 5, 2, 2), (3, 1, 2, 2), (32, 3, 7, 2), (8, 20, 3, 2), (3, 64, 2, 2), (5, 32, 2, 1), (32, 32, 5, 2), (2, 256, 1, 2)])
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("biased", [False, True])
 def test_groups_and_bias(groups, each, top_groups, group_top, scores, biased):
