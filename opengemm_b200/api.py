@@ -86,8 +86,9 @@ def check_bias(bias, n, device):
         raise TypeError(f"bias must be a contiguous float32 [{n}] on {device}")
 
 
-def check_epilogue(name, d, m, n, out, activation, residual, preactivation):
-    """Raise unless the fused epilogue's arguments fit a C of `d.out` [m, n]."""
+def check_epilogue(name, d, m, n, out, activation, residual, preactivation, **read):
+    """Raise unless the fused epilogue's arguments fit a C of `d.out` [m, n]; `read` are the launch's
+    other inputs, or None, which tiles still to come read while this call writes."""
     if activation not in capi.ACTIVATIONS:
         raise TypeError(f"activation must be one of {[a for a in capi.ACTIVATIONS if a]}, got {activation!r}")
     if d.out is torch.int32:
@@ -104,6 +105,10 @@ def check_epilogue(name, d, m, n, out, activation, residual, preactivation):
                 raise ValueError(f"preactivation and {label} share memory")
     if residual is not None and residual.data_ptr() != out.data_ptr() and overlap(residual, out):
         raise ValueError("residual may be out itself, but not overlap it in part")
+    for label, t in read.items():
+        for written, w in (("out", out), ("preactivation", preactivation)):
+            if t is not None and w is not None and overlap(w, t):
+                raise ValueError(f"{written} and {label} share memory")
 
 
 def overlap(s, t):
@@ -146,7 +151,8 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
         residual: a contiguous `(M, N)` tensor of C's type added after the
             activation, in float32, before the store.  It may be `out` itself.
         preactivation: a contiguous `(M, N)` tensor of C's type that receives
-            the activation's argument, which `gemm_backward` reads.
+            the activation's argument, which `gemm_backward` reads.  With any of
+            these three, neither it nor `out` may share memory with another input.
 
     Returns:
         `(M, N)` row-major: float32 for dense formats (bfloat16 with
@@ -183,7 +189,7 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
         out = torch.empty_like(residual)  # the cheapest way to one
     out = output(d, m, n, out, a.device)
     if fused:
-        check_epilogue(name, d, m, n, out, activation, residual, preactivation)
+        check_epilogue(name, d, m, n, out, activation, residual, preactivation, a=a, b=b, sfa=sfa, sfb=sfb, bias=bias)
         if bias is not None:
             check_bias(bias, n, a.device)
         lib.launch_fused(g, a, b, sfa, sfb, out, alpha, bias, activation, residual, preactivation)

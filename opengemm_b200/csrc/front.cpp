@@ -455,7 +455,9 @@ PyObject* gemm(PyObject*, PyObject* const* v, Py_ssize_t count) {
   const Tensor* bias = optional_tensor(v[6], at::kFloat, device, {key.n}, ok);
   const Tensor* residual = optional_tensor(v[8], e.out, device, {key.m, key.n}, ok);
   const Tensor* z = optional_tensor(v[9], e.out, device, {key.m, key.n}, ok);
-  if (!ok || (z && (!aligned(*z) || (residual && overlap(*z, *residual))))) NOT_SERVED;
+  if (!ok || (z && !aligned(*z))) NOT_SERVED;
+  for (const Tensor* read : {residual, a, b, sfa, sfb, bias})
+    if (z && read && overlap(*z, *read)) NOT_SERVED;
   Tensor out = empty({key.m, key.n}, e.out, device);
   epilogue.bias = data(bias), epilogue.residual = data(residual), epilogue.preactivation = const_cast<void*>(data(z));
   if (api.launch_fused(&e.g, a->data_ptr(), b->data_ptr(), data(sfa), data(sfb), out.data_ptr(), device, stream_of(device), &epilogue)) return failed(api.error());

@@ -231,3 +231,25 @@ def test_refusals():
     ints = torch.zeros(64, 64, device="cuda", dtype=torch.int8)
     with pytest.raises(TypeError, match="integers"):
         og.gemm(ints, ints, activation="relu")
+
+
+def test_what_is_written_is_not_read():
+    """Tiles still to come read the operands: a call may not write over them, not even where its residual is one."""
+    a, b = torch.ones(64, 64, device="cuda"), torch.ones(64, 64, device="cuda")
+    half_a, half_b = a.bfloat16(), b.bfloat16()
+    bias = torch.zeros(64 * 64, device="cuda")
+    for _ in range(2):  # as the first call of its shape, and as one known already
+        with pytest.raises(ValueError, match="out and a share memory"):
+            og.gemm(half_a, half_b, out=half_a, residual=half_a)
+        with pytest.raises(ValueError, match="out and b share memory"):
+            og.gemm(half_a, half_b, out=half_b, activation="relu")
+        with pytest.raises(ValueError, match="out and bias share memory"):
+            og.gemm(half_a, half_b, out=bias.view(64, 64), activation="relu", bias=bias[:64])
+        for label, z in (("a", half_a), ("b", half_b)):
+            with pytest.raises(ValueError, match=f"preactivation and {label} share memory"):
+                og.gemm(half_a, half_b, out_dtype=torch.bfloat16, activation="relu", preactivation=z)
+        with pytest.raises(ValueError, match="preactivation and bias share memory"):
+            og.gemm(half_a, half_b, activation="relu", preactivation=bias.view(64, 64), bias=bias[64:128])
+        assert (half_a == 1).all() and (half_b == 1).all() and not bias.any()
+        c = og.gemm(half_a, half_b, out_dtype=torch.bfloat16, residual=half_a)  # a as its own residual, C elsewhere
+        assert (c == 65).all()
