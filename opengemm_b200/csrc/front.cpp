@@ -256,7 +256,7 @@ PyObject* expert_gemm(PyObject*, PyObject* const* a, Py_ssize_t count) {
   bool ok = true;
   const Tensor* alpha = optional_tensor(a[5], at::kFloat, p.device, {p.experts}, ok);
   const Tensor* z = optional_tensor(a[6], own, p.device, {p.rows, q.n}, ok);
-  if (!ok || (z && (overlap(*z, *q.x) || overlap(*z, *q.w)))) NOT_SERVED;
+  if (!ok || (z && (overlap(*z, *q.x) || overlap(*z, *q.w) || (alpha && overlap(*z, *alpha))))) NOT_SERVED;
   Tensor out = empty({p.rows, q.gated ? q.n / 2 : q.n}, own, p.device), sorted;
   const void* x = q.x->data_ptr();
   bool gather = q.gather != 0;

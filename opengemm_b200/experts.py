@@ -39,9 +39,9 @@ def _expect(label, t, dtype, shape, device):
 
 
 def _apart(label, t, **others):
-    """Raise if `t`, which a launch writes, shares memory with a tensor that it reads or writes too."""
+    """Raise if `t`, which a launch writes, shares memory with a tensor (or None) that it reads or writes too."""
     for name, other in others.items():
-        if overlap(t, other):
+        if other is not None and overlap(t, other):
             raise ValueError(f"{label} and {name} share memory")
 
 
@@ -76,7 +76,8 @@ def route(logits, top_k, scores="softmax", bias=None, groups=1, top_groups=1, gr
         `(weights, indices)`, float32 and int32 `(tokens, top_k)`, the best first
         and the lowest index first among equals.  Where a token has fewer than
         `top_k` experts to choose from, the places left have index -1 and weight
-        0.  A NaN logit ranks first and makes its token's weights NaN.
+        0.  A NaN score ranks first, and its weight is NaN; softmax and `renormalise`
+        make all of that token's weights NaN.
     """
     front = capi.front()
     if front is not None:
@@ -247,10 +248,10 @@ def expert_gemm(x, w, plan, gather=False, activation=None, alpha=None, out=None,
         out = torch.empty((rows, width), device=device, dtype=own)
     else:
         _expect("out", out, own, (rows, width), device)
-        _apart("out", out, x=x, w=w)
+        _apart("out", out, x=x, w=w, alpha=alpha, plan=plan._store)
     if preactivation is not None:
         _expect("preactivation", preactivation, own, (rows, n), device)
-        _apart("preactivation", preactivation, out=out, x=x, w=w)
+        _apart("preactivation", preactivation, out=out, x=x, w=w, alpha=alpha, plan=plan._store)
     if alpha is not None:
         _expect("alpha", alpha, torch.float32, (plan.experts,), device)
     if gather and rows > _GATHER_IN_PRODUCT * min(plan.experts, rows):
@@ -353,7 +354,8 @@ def expert_combine(y, weights, plan, residual=None, out=None):
         weights: float32 `(tokens, top_k)`.
         plan: from `expert_plan`.  A pair that goes nowhere adds nothing.
         residual: `(tokens, N)` of y's dtype, or None; may be `out`.
-        out: written instead of a new tensor.
+        out: written instead of a new tensor; apart from `residual` itself it may
+            share memory with no other tensor of the call.
 
     Returns:
         `(tokens, N)` of y's dtype, summed in float32 in the order of the choices.
@@ -371,7 +373,7 @@ def expert_combine(y, weights, plan, residual=None, out=None):
         out = y.new_empty(shape)
     else:
         _expect("out", out, y.dtype, shape, plan.device)
-        _apart("out", out, y=y)
+        _apart("out", out, y=y, weights=weights, plan=plan._store)
         if residual is not None and residual.data_ptr() != out.data_ptr():
             _apart("out", out, residual=residual)
     _combine(y, weights, plan, residual, out, n)

@@ -463,3 +463,21 @@ def test_refusals():
         og.gemm_backward(grad, a, b, out_dtype=torch.float16)
     with pytest.raises(ValueError, match="multiples of 8"):
         og.gemm_backward(grad[:, :30].contiguous(), a, b[:30])
+
+
+def test_what_is_written_is_not_read():
+    """Neither the factors and weights nor the plan may be written over by the call that reads them."""
+    plan = og.expert_plan(torch.tensor([[0, 1], [2, 0], [1, 2], [0, 1]], device="cuda", dtype=torch.int32), 3)
+    x, w = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(3, 64, 64, device="cuda", dtype=torch.bfloat16)
+    store = torch.zeros(8 * 64, device="cuda")  # as bfloat16 twice the rows
+    alpha, rows = store[:3], store.view(torch.bfloat16)[:8 * 64].view(8, 64)
+    with pytest.raises(ValueError, match="out and alpha share memory"):
+        og.expert_gemm(x, w, plan, alpha=alpha, out=rows)
+    with pytest.raises(ValueError, match="preactivation and alpha share memory"):
+        og.expert_gemm(x, w, plan, alpha=alpha, activation="relu", preactivation=rows)
+    weights, tokens = store[:8].view(4, 2), store.view(torch.bfloat16)[:4 * 64].view(4, 64)
+    with pytest.raises(ValueError, match="out and weights share memory"):
+        og.expert_combine(x, weights, plan, out=tokens)
+    with pytest.raises(ValueError, match="out and plan share memory"):
+        og.expert_combine(x[:, :2].contiguous(), torch.zeros(4, 2, device="cuda"), plan, out=plan.offsets.view(torch.bfloat16).view(4, 2))
+    assert not store.any()
