@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/opengemm_b200.h"
+#include "device_scope.h"
 #include "experts_launch.h"
 #include "launch_common.h"
 
@@ -201,9 +202,8 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   const bool gather = g.tokens != nullptr;
   if (gather && mode != MODE_FORWARD) return experts_fail(OG_ERR_LAUNCH, "only the forward product gathers its rows");
   if (device < 0 || device >= XP_DEVICES) return experts_fail(OG_ERR_LAUNCH, "device %d is out of range: this library serves devices 0..%d", device, XP_DEVICES - 1);
-  int current = -1;
-  if (cudaGetDevice(&current) != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaGetDevice failed");
-  if (current != device && cudaSetDevice(device) != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaSetDevice(%d) failed", device);
+  const DeviceScope on(device);
+  if (on.status() != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaSetDevice(%d): %s", device, cudaGetErrorString(on.status()));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int out_bytes = g.out_f32 ? 4 : 2;
   if (g.rows == 0 || (gather && g.x_rows == 0)) {  // nothing to multiply: sums over no rows are zero
@@ -359,6 +359,8 @@ OG_API int32_t og_b200_gemm_gradients(const OgGemmGradients* g, int32_t device, 
   const GradientSpace s = gradient_space(*g, device);
   if (s.dz + s.bias + s.sums > 0 && (!g->workspace || (reinterpret_cast<uintptr_t>(g->workspace) & 15) || g->workspace_bytes < s.dz + s.bias + s.sums))
     return experts_fail(OG_ERR_LAUNCH, "these gradients take a 16-byte aligned workspace of %lld bytes, got %lld", (long long)(s.dz + s.bias + s.sums), (long long)g->workspace_bytes);
+  const DeviceScope on(device);
+  if (on.status() != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaSetDevice(%d): %s", device, cudaGetErrorString(on.status()));
   uint8_t* const dz = static_cast<uint8_t*>(g->workspace);
   float* const bias_sums = reinterpret_cast<float*>(dz + s.dz);
   uint8_t* const sums = dz + s.dz + s.bias;

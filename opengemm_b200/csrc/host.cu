@@ -20,6 +20,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "device_scope.h"
 #include "kernel.cuh"
 #include "kernels_fixed.cuh"
 #include "launch_common.h"
@@ -591,6 +592,7 @@ OG_API int32_t og_b200_launch_fused(const OgGemm* g, const void* a, const void* 
   io.c_scales = epilogue->out_scales;
   if (io.out_quant < 0 || io.out_quant > 3) return fail(OG_ERR_LAUNCH, "out_format %d is none of 0..3", io.out_quant);
   const float alpha = epilogue->alpha;
+  const DeviceScope on(device);  // launch_impl says what is wrong with it
   return launch_impl(g, io, device, stream, nullptr, -1, alpha != 1.0f ? &alpha : nullptr);
 }
 

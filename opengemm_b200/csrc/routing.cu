@@ -18,6 +18,7 @@
 
 #include "../../include/opengemm_b200.h"
 #include "activation.cuh"
+#include "device_scope.h"
 #include "ptx.cuh"
 
 namespace og {
@@ -793,11 +794,8 @@ int routing_fail(const char* format, ...) {
   return OG_ERR_LAUNCH;
 }
 
-int use_device(int device) {
-  int current = -1;
-  if (cudaGetDevice(&current) != cudaSuccess) return routing_fail("cudaGetDevice failed");
-  if (current != device && cudaSetDevice(device) != cudaSuccess) return routing_fail("cudaSetDevice(%d) failed", device);
-  return OG_OK;
+int check_device(const DeviceScope& on, int device) {
+  return on.status() == cudaSuccess ? int(OG_OK) : routing_fail("cudaSetDevice(%d): %s", device, cudaGetErrorString(on.status()));
 }
 
 template <typename... Args>
@@ -866,7 +864,8 @@ OG_API int32_t og_b200_route(const OgRoute* route, const void* logits, const flo
   if (r.top_k > r.top_groups * (r.experts / r.groups)) return routing_fail("top_k = %d is more than the %d experts of the open groups", r.top_k, r.top_groups * (r.experts / r.groups));
   if (!r.tokens) return OG_OK;
   if (!logits || !weights || !indices) return routing_fail("logits, weights and indices must be device pointers, got null");
-  if (const int bad = use_device(device)) return bad;
+  const DeviceScope on(device);
+  if (const int bad = check_device(on, device)) return bad;
   RouteParams p{};
   p.logits = logits, p.bias = bias, p.weights = weights, p.indices = indices, p.tokens = r.tokens, p.experts = r.experts;
   p.top_k = r.top_k, p.sigmoid = r.sigmoid, p.groups = r.groups, p.each = r.experts / r.groups, p.top_groups = r.top_groups;
@@ -885,7 +884,8 @@ OG_API int32_t og_b200_route_gradient(const OgRoute* route, const float* grad_we
   if (const int bad = check_route(r)) return bad;
   if (!r.tokens) return OG_OK;
   if (!grad_weights || !logits || !indices || !grad_logits) return routing_fail("gradients, logits and indices must be device pointers, got null");
-  if (const int bad = use_device(device)) return bad;
+  const DeviceScope on(device);
+  if (const int bad = check_device(on, device)) return bad;
   RouteParams p{};
   p.logits = logits, p.grad_weights = grad_weights, p.indices = const_cast<int32_t*>(indices), p.grad_logits = grad_logits;
   p.tokens = r.tokens, p.experts = r.experts, p.top_k = r.top_k, p.sigmoid = r.sigmoid, p.renormalise = r.renormalise, p.scale = r.scale;
@@ -902,7 +902,8 @@ OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32
   if (!offsets || (tokens && (!indices || !token_of_row || !positions))) return routing_fail("indices and the plan's arrays must be device pointers, got null");
   if (tokens * top_k > PLAN_CHUNK && !workspace)
     return routing_fail("%lld pairs take a workspace of %lld integers", (long long)(tokens * top_k), (long long)((tokens * top_k + PLAN_CHUNK - 1) / PLAN_CHUNK * experts));
-  if (const int bad = use_device(device)) return bad;
+  const DeviceScope on(device);
+  if (const int bad = check_device(on, device)) return bad;
   PlanParams p{};
   p.indices = indices, p.offsets = offsets, p.tokens = token_of_row, p.positions = positions, p.histogram = workspace;
   p.pairs = int(tokens * top_k), p.top_k = top_k, p.experts = experts;
@@ -926,7 +927,8 @@ OG_API int32_t og_b200_expert_gather(const void* x, const int32_t* token_of_row,
   if (!rows) return OG_OK;
   if (!x || !token_of_row || !row_limit || !out) return routing_fail("x, the plan and out must be device pointers, got null");
   if (!aligned16(x) || !aligned16(out)) return routing_fail("rows must start on 16-byte boundaries");
-  if (const int bad = use_device(device)) return bad;
+  const DeviceScope on(device);
+  if (const int bad = check_device(on, device)) return bad;
   return dependent_launch(gather_kernel, dim3(unsigned((rows + 7) / 8)), 256, 0, stream, static_cast<const uint4*>(x), token_of_row, row_limit,
                           static_cast<uint4*>(out), int(row_bytes / 16), int(rows));
 }
@@ -937,7 +939,8 @@ OG_API int32_t og_b200_expert_combine(int32_t dtype, int32_t y_is_f32, const voi
   if (tokens < 0 || tokens > 0x7FFFFFFFll || top_k < 1 || n < 1) return routing_fail("tokens = %lld, top_k = %d, n = %d", (long long)tokens, top_k, n);
   if (!tokens) return OG_OK;
   if (!positions || !out) return routing_fail("positions and out must be device pointers, got null");
-  if (const int bad = use_device(device)) return bad;
+  const DeviceScope on(device);
+  if (const int bad = check_device(on, device)) return bad;
   CombineParams p{};
   p.y = y, p.weights = weights, p.positions = positions, p.residual = residual, p.out = out, p.tokens = tokens, p.n = n, p.top_k = top_k;
   const bool wide = n % 8 == 0 && aligned16(y) && aligned16(residual) && aligned16(out);
@@ -958,7 +961,8 @@ OG_API int32_t og_b200_expert_combine_gradient(int32_t dtype, const void* grad, 
   if (tokens < 0 || top_k < 1 || n < 1 || tokens * top_k > 0x7FFFFFFFll) return routing_fail("tokens = %lld, top_k = %d, n = %d", (long long)tokens, top_k, n);
   if (!tokens) return OG_OK;
   if (!grad || !weights || !positions || !grad_weights) return routing_fail("the gradient's tensors must be device pointers, got null");
-  if (const int bad = use_device(device)) return bad;
+  const DeviceScope on(device);
+  if (const int bad = check_device(on, device)) return bad;
   CombineParams p{};
   p.y = y, p.weights = weights, p.positions = positions, p.grad = grad, p.out = grad_y, p.grad_weights = grad_weights;
   p.tokens = tokens, p.n = n, p.top_k = top_k;
@@ -976,7 +980,8 @@ OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, co
   if (rows < 0 || n < 1 || n % (glu ? 16 : 8)) return routing_fail("rows = %lld, n = %d: columns come in eights", (long long)rows, n);
   if (glu && bias_gradient) return routing_fail("a gated activation has no bias gradient here");
   if (rows > 0x7FFFFFFFll) return routing_fail("rows = %lld are too many", (long long)rows);
-  if (const int bad = use_device(device)) return bad;
+  const DeviceScope on(device);
+  if (const int bad = check_device(on, device)) return bad;
   const int block_rows = gradient_block_rows(rows, glu ? n / 2 : n);
   const int blocks = int((rows + block_rows - 1) / block_rows);
   const bool one_cluster = bias_gradient && !row_limit && rows && blocks <= GRADIENT_CLUSTER;
