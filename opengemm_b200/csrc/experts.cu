@@ -283,6 +283,13 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
     const uint32_t box_rows = mode == MODE_DX ? 64 : uint32_t(glu ? plan.tile_n / 2 : y_rows);
     map(&p.map_y, g.w, k, n, box_rows, "the weights", uint64_t(g.groups));
   }
+  const int64_t out_rows = mode == MODE_DW ? int64_t(p.groups) * g.n : p.split_blocks ? int64_t(p.groups) * g.rows : int64_t(g.rows);
+  p.direct = p.vec_ok && out_rows <= 0x7FFFFFFF;
+  if (p.direct && rc == OG_OK) {  // swizzled as the epilogue's staging buffers are
+    const int out_type = g.out_f32 ? int(CU_TENSOR_MAP_DATA_TYPE_FLOAT32) : f16 ? int(CU_TENSOR_MAP_DATA_TYPE_FLOAT16) : int(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+    rc = encode_2d(&p.map_d, g.out, out_type, uint64_t(p.cols), uint64_t(out_rows), uint64_t(p.cols) * out_bytes, XP_CHUNK, 32,
+                   g.out_f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, 0, "the output", why, sizeof why);
+  }
   if (rc != OG_OK) return experts_fail(rc, "%s", why);
 
   int index = 0;

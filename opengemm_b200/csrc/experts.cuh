@@ -47,6 +47,7 @@ struct alignas(64) ExpertParams {
   CUtensorMap map_x;    // MMA-M side, boxes of 128 rows (64 x 64 in MODE_DW)
   CUtensorMap map_x32;  // the same in boxes of 32 rows, for a group's last, short tile; gathered: of one row
   CUtensorMap map_y;    // MMA-N side
+  CUtensorMap map_d;    // output, boxes of 32 rows x XP_CHUNK columns (`direct` only)
   const int* offsets;   // [groups + 1] first row of each group; null: one group of all rows
   const int* tokens;    // gathered operand: its row for each sorted row
   const float* alpha;   // [groups], or null
@@ -69,6 +70,7 @@ struct alignas(64) ExpertParams {
   int band;             // M tiles per band of the tile order
   int ldd, ldz;         // elements per row of `d` and `preact`
   int vec_ok;           // rows of d and preact take 16-byte stores
+  int direct;           // whole slabs of 32 output rows leave by TMA
   int act_shape;
   float act_a, act_b;
   int out_f16;
@@ -151,6 +153,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
     prefetch_tmap(&p.map_x);
     prefetch_tmap(&p.map_y);
     if (MODE == MODE_FORWARD) prefetch_tmap(&p.map_x32);
+    if (p.direct) prefetch_tmap(&p.map_d);
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
@@ -469,7 +472,9 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
 
       // CHUNK columns of this lane's row, through the warp's swizzled buffer, as
       // whole row segments; unaligned rows element by element, side by side.
-      auto store = [&](const float* v, uint8_t* base, int ld, int col, int limit) {
+      auto store = [&](const float* v, uint8_t* base, int ld, int col, int limit, bool direct) {
+        if (lane == 0) tma_store_wait_read<0>();  // the buffer's last chunk has left
+        __syncwarp();
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
           uint32_t q[4];
@@ -477,6 +482,15 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
           for (int h = 0; h < 4; ++h)
             q[h] = OUT_BYTES == 4 ? __float_as_uint(v[(4 * u + h) % CHUNK]) : pack2(v[(8 * u + 2 * h) % CHUNK], v[(8 * u + 2 * h + 1) % CHUNK]);
           st_shared_v4(at_unit(lane, u), q[0], q[1], q[2], q[3]);
+        }
+        if (direct && valid == 32) {
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&p.map_d, my_buf, col, int(row0));
+            tma_store_commit();
+          }
+          return;
         }
         __syncwarp();
         if (vec_ok) {
@@ -548,8 +562,8 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
         }
         if constexpr (MODE == MODE_FORWARD) {
           if (p.preact) {
-            store(v, static_cast<uint8_t*>(p.preact), p.ldz, col0 + c, cols);
-            if constexpr (GLU) store(up, static_cast<uint8_t*>(p.preact), p.ldz, p.glu_offset + col0 + c, p.glu_offset + cols);
+            store(v, static_cast<uint8_t*>(p.preact), p.ldz, col0 + c, cols, false);
+            if constexpr (GLU) store(up, static_cast<uint8_t*>(p.preact), p.ldz, p.glu_offset + col0 + c, p.glu_offset + cols, false);
           }
           activate(v);
           if constexpr (GLU) {
@@ -557,10 +571,11 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
             for (int j = 0; j < CHUNK; ++j) v[j] *= up[j];
           }
         }
-        store(v, static_cast<uint8_t*>(p.d), p.ldd, col0 + c, cols);
+        store(v, static_cast<uint8_t*>(p.d), p.ldd, col0 + c, cols, p.direct != 0);
         if (GLU && !last) load(c + STRIDE, coming);
       }
     }
+    if (lane == 0) tma_store_wait<0>();
   }
 
   if (p.beside) pdl_wait_prior_grids();
