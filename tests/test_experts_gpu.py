@@ -481,3 +481,40 @@ def test_what_is_written_is_not_read():
     with pytest.raises(ValueError, match="out and plan share memory"):
         og.expert_combine(x[:, :2].contiguous(), torch.zeros(4, 2, device="cuda"), plan, out=plan.offsets.view(torch.bfloat16).view(4, 2))
     assert not store.any()
+
+
+def test_gradients_past_32_bits():
+    """More than 2^31 values of gradients and pre-activations, and then of weights' gradients."""
+    rows, n, k, tail = 1_100_000, 2048, 64, 700
+    indices = torch.zeros(rows, 1, dtype=torch.int32, device="cuda")
+    indices[-300:] = 1
+    plan = og.expert_plan(indices, 2)
+    g = torch.Generator().manual_seed(1)
+    x = torch.ones(rows, k, device="cuda", dtype=torch.bfloat16)
+    x[-tail:] = values(g, tail, k, dtype=torch.bfloat16)
+    w = values(g, 2, n, k, dtype=torch.bfloat16)
+    grad, z = (torch.zeros(rows, n, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    grad[-tail:], z[-tail:] = values(g, tail, n, dtype=torch.bfloat16), 1.0
+    grad_x, grad_w = og.expert_gemm_backward(grad, x, w, plan, activation="relu", preactivation=z)
+    dz, last = grad[-tail:].double(), x[-tail:].double()
+    for e, at in ((0, slice(0, tail - 300)), (1, slice(tail - 300, tail))):
+        we = w[e].double()
+        assert_within(grad_x[-tail:][at], dz[at] @ we, sum_error(dz[at].abs() @ we.abs(), n), "rows")
+        # the rows of zeros add nothing, and a sum of them loses nothing
+        assert_within(grad_w[e], dz[at].T @ last[at], sum_error(dz[at].abs().T @ last[at].abs(), tail), "weights")
+    assert not grad_x[:-tail].any()
+    grad_a, grad_b, grad_bias = og.gemm_backward(grad, x, w[0], activation="relu", preactivation=z, want=("a", "b", "bias"))
+    assert_within(grad_a[-tail:], dz @ w[0].double(), sum_error(dz.abs() @ w[0].double().abs(), n), "a")
+    assert_within(grad_b, dz.T @ last, sum_error(dz.abs().T @ last.abs(), tail), "b")
+    assert_within(grad_bias, dz.sum(0), (24 + tail / 64) * 2.0**-24 * dz.abs().sum(0), "bias")
+    assert not grad_a[:-tail].any()
+    del grad, z, grad_x, grad_a
+
+    n = k = 33024  # two experts' weights
+    plan = og.expert_plan(torch.tensor([[0], [1], [1]], dtype=torch.int32, device="cuda"), 2)
+    grad, x = values(g, 3, n, dtype=torch.bfloat16), values(g, 3, k, dtype=torch.bfloat16)
+    _, grad_w = og.expert_gemm_backward(grad, x, torch.empty(2, n, k, device="cuda", dtype=torch.bfloat16), plan, want=("w",))
+    for part in (slice(0, 300), slice(n - 300, n)):
+        for e, at in ((0, slice(0, 1)), (1, slice(1, 3))):
+            dz, last = grad[at, part].double(), x[at].double()
+            assert_within(grad_w[e, part], dz.T @ last, sum_error(dz.abs().T @ last.abs(), 2), f"weights of {e}")
