@@ -53,26 +53,31 @@ struct ExpertPlan {
 // With several groups only their number and the number of all rows are known
 // here (the table of offsets is on the device): they are taken as equal, a
 // group's last tile as half full, and the last wave of tiles as half idle.
-// A tile costs its K blocks and some 300 cycles between two tiles (loads run
-// ahead into the next one, and its accumulator is a second one), but no less
-// than storing it takes (16 experts with eight rows each, weights' gradient of
-// 2608 x 2992: 71 us in tiles of 256, 86 us in pairs, 96 and 149 us in narrower
-// ones; clearing that memory takes 66 us).  A K block costs what full waves of such tiles measured: pairs of CTAs share the N-side
-// operand, which lets wide tiles run nearest the tensor pipe's rate (bf16
-// 4096 x 8192 x 4096, rows' gradient: 190 us in pairs, 217 / 237 / 364 us in
-// single CTAs 256 / 128 / 64 wide).  Where a group's rows fit one tile its
-// weights are read from memory once and nothing else is: the block then costs
-// the SM's share of the memory bandwidth, best used by tiles of 128 (16 tokens x
-// 8 of 64 experts, 2048 x 2048 weights: 59 us; 65 us in pairs, 63 us 256 wide,
-// 66 us 64 wide).  Narrow tiles give every SM work when there are few.
+// A tile costs its K blocks and some 2000 cycles (its first loads, its last store),
+// but no less than storing it takes (16 experts with some 20 rows each, weights'
+// gradient of 2608 x 2992: 64 us in tiles of 256, as long as clearing that memory
+// takes, 86 us in pairs, 89 and 141 us in narrower ones).  A K block costs what
+// fits 63 measured launches of 8 to 32 unevenly filled experts, 20 to 1500 rows
+// each, best: pairs of CTAs share the N-side operand, which lets wide tiles run
+// nearest the tensor pipe's rate (bf16 4096 x 8192 x 4096, rows' gradient: 190 us
+// in pairs, 217 / 237 / 364 us in single CTAs 256 / 128 / 64 wide).  Where a
+// group's rows fit one tile its weights are read from memory once and nothing else
+// is: the block then costs the SM's share of the memory bandwidth, best used by
+// tiles of 128 in the forward product (16 tokens x 8 of 64 experts, 2048 x 2048
+// weights: 59 us; 65 us in pairs, 63 us 256 wide, 66 us 64 wide), of 256 in the
+// rows' gradient (64 experts, three rows each: 84 us for 89).  Narrow tiles give
+// every SM work when there are few.  The choice is within 10 % of the best of the
+// four but for single cases (8 experts of 300 to 700 rows, 2048 x 2048: 43 us for 37;
+// 16 of some 100, 1536 x 3000, rows that are no whole lines: 51 us for 41).
 // With `parts` > 1 a single group's work is cut along its reduction into that
 // many launches' worth of tiles.
 ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count, int parts = 1) {
   const int busy = std::max(1, std::min(groups, rows));
   const double rows_each = double(std::max(rows, 1)) / busy;
   static const ExpertPlan menu[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
-  static const int multiply_cycles[] = {560, 640, 420, 325}, stream_cycles[] = {775, 1365, 683, 430};
-  static const int least_cycles[] = {5600, 4800, 3300, 2600};
+  static const int multiply_cycles[3][4] = {{740, 950, 560, 390}, {750, 1025, 615, 535}, {685, 725, 460, 290}};  // by mode
+  static const int stream_cycles[2][4] = {{780, 1430, 680, 525}, {780, 1090, 680, 525}};
+  static const int least_cycles[] = {9200, 4900, 2950, 2450};
   ExpertPlan best = menu[0];
   double best_cost = 0;
   for (int i = 0; i < 4; ++i) {
@@ -83,9 +88,10 @@ ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int 
                                              : std::max(1.0, rows_each / tile_m + 0.5);
     const double tiles = double(parts) * (mode == MODE_DW ? groups : busy) * m_tiles * ceil_div(cols, out_n);
     const double blocks = (mode == MODE_DW ? std::max(1.0, rows_each / 64) : blocks_fixed) / parts;
-    const int block = mode != MODE_DW && rows_each <= tile_m ? stream_cycles[i] : multiply_cycles[i];
+    double block = mode != MODE_DW && rows_each <= tile_m ? stream_cycles[mode][i] : multiply_cycles[mode][i];
+    if (mode != MODE_DW && c.cta_group == 2 && rows_each <= 128) block *= 1.22;  // the second CTA has no rows
     const double waves = tiles / (sm_count / c.cta_group);
-    const double cost = (groups == 1 ? std::ceil(waves) : std::max(1.0, waves + 0.5)) * std::max(blocks * block + 300, double(least_cycles[i]));
+    const double cost = (groups == 1 ? std::ceil(waves) : std::max(1.0, waves + 0.5)) * std::max(blocks * block + 2000, double(least_cycles[i]));
     if (i == 0 || cost < best_cost) best = c, best_cost = cost;
   }
   best.cost = best_cost;

@@ -24,6 +24,20 @@
 // Roles as in kernel.cuh: warp 0 loads (one thread; all lanes when rows are
 // gathered, four rows a lane and instruction), warp 1 issues the MMAs, warps
 // 2-9 store, warp 10 is the weight gradient's.  Every wait is bounded.
+//
+// What bounds it: with many rows the tensor pipe, under the power limit (bf16, 8
+// experts of 960 rows, 4096 x 4096: 200 us, 88-93 % active).  With a few hundred
+// rows an expert the ring of stages: a K block moves 32 KB a CTA in pairs, 48 KB
+// in a CTA of 128 x 256, against 512 cycles of MMAs, and memory or L2 is over a
+// microsecond away (8 experts of 512 rows, weights' gradient 2048 x 2048: 31 us in
+// pairs with six stages, 36 us with four of the larger ones).  Every stage counts:
+// staging two chunks of output a warp, for whole 128-byte lines, takes one and was
+// slower (36 -> 39 us), and asking for the weights a few blocks ahead in L2 costs
+// the copy engine as much as loading them (35 -> 38 us in the rows' product, 34 ->
+// 45 us with eight rows an expert).  Whole slabs of 32 output rows leave by that
+// engine too, straight from the staging buffer, which is swizzled as its map says:
+// 37 -> 36 us there, and 53 -> 45 us where a tile is one load and one store (16
+// experts, 256 rows each); rows by threads where a group ends.
 #pragma once
 
 #include "activation.cuh"
