@@ -309,9 +309,10 @@ typedef struct OgExpertProduct {
   int32_t activation;     /* mode 0 */
   int32_t out_f32;        /* modes 1 and 2: write float32 */
   float factor;           /* on every product, before the activation (beside alpha) */
-  int32_t beside_previous; /* 1: the caller vouches that the stream's previous launch was one of
-                              this call, over as many rows, which writes nothing that this one
-                              reads or writes; the two then run side by side */
+  int32_t beside_previous; /* 1: the caller vouches that a launch of this call, over as many rows,
+                              went to the stream before, that it writes nothing which this one
+                              reads or writes, and that all of this one's memory was the
+                              caller's before that launch; the two then run side by side */
   char dtype[16];
 } OgExpertProduct;
 OG_API int32_t og_b200_expert_product(const OgExpertProduct* product, int32_t device, void* stream);

@@ -367,8 +367,9 @@ class Library:
     def expert_product(self, mode, dtype, x, w, out, groups, rows, n, k, offsets=0, tokens=0, x_rows=0, alpha=None,
                        activation=0, preactivation=None, beside_previous=False):
         """One launch of og_b200_expert_product on CUDA tensors, on the current stream of `out`'s
-        device; `offsets` and `tokens` are addresses.  `beside_previous` vouches that the stream's
-        previous launch was this method's and writes nothing that this one touches."""
+        device; `offsets` and `tokens` are addresses.  `beside_previous` vouches that a
+        launch of this method's went to the stream before, that it writes nothing which this one touches,
+        and that this one's tensors were all allocated before it."""
         device = out.get_device()
         product = OgExpertProduct(
             x.data_ptr(), w.data_ptr(), offsets, tokens, 0 if alpha is None else alpha.data_ptr(), out.data_ptr(),

@@ -289,37 +289,36 @@ PyObject* expert_gemm_backward(PyObject*, PyObject* const* a, Py_ssize_t count) 
   if (!ok || (q.activation != 0) != (z != nullptr) || !is(grad, type, p.device, {p.rows, q.gated ? q.n / 2 : q.n}) || !aligned(*grad) || (z && !aligned(*z)))
     NOT_SERVED;
   void* const stream = stream_of(p.device);
-  Tensor dz = *grad, grad_x, grad_w;
+  // All outputs before the first launch: the weights' gradient, beside the rows', waits for
+  // nothing before it writes (experts.py says what memory from between the two could be).
+  Tensor dz = *grad, rows = *q.x, by_row, grad_x, grad_w;
+  if (want_x) {  // a token's rows are added before anything is rounded
+    by_row = empty({p.rows, q.k}, q.gather ? at::kFloat : type, p.device);
+    grad_x = q.gather ? empty({p.tokens, q.k}, type, p.device) : by_row;
+  }
+  if (want_w) grad_w = empty({p.experts, q.n, q.k}, type, p.device);
   if (z) {
     dz = empty({p.rows, q.n}, type, p.device);
     if (api.activation_gradient(code, q.activation, grad->data_ptr(), z->data_ptr(), dz.data_ptr(), nullptr, nullptr, p.limit, p.rows, int(q.n), p.device, stream))
       return failed(api.routing_error());
   }
-  Tensor rows = *q.x, by_row;
   if (want_w && q.gather) {
     rows = sorted_rows(*q.x, p, q.k);
     if (!rows.defined()) return failed(api.routing_error());
   }
-  if (want_x) {  // a token's rows are added before anything is rounded
-    by_row = empty({p.rows, q.k}, q.gather ? at::kFloat : type, p.device);
+  if (want_x) {
     OgExpertProduct g = launch_of(1, q, p, dz.data_ptr(), q.w->data_ptr(), by_row.data_ptr());
     g.out_f32 = q.gather;
     if (api.expert_product(&g, p.device, stream)) return failed(api.experts_error());
   }
   if (want_w) {
-    grad_w = empty({p.experts, q.n, q.k}, type, p.device);
     OgExpertProduct g = launch_of(2, q, p, dz.data_ptr(), rows.data_ptr(), grad_w.data_ptr());
     g.beside_previous = want_x != 0;
     if (api.expert_product(&g, p.device, stream)) return failed(api.experts_error());
   }
-  if (want_x) {
-    grad_x = by_row;
-    if (q.gather) {
-      grad_x = empty({p.tokens, q.k}, type, p.device);
-      if (api.expert_combine(code, 1, by_row.data_ptr(), nullptr, p.positions, nullptr, grad_x.data_ptr(), p.tokens, p.top_k, int(q.k), p.device, stream))
-        return failed(api.routing_error());
-    }
-  }
+  if (want_x && q.gather &&
+      api.expert_combine(code, 1, by_row.data_ptr(), nullptr, p.positions, nullptr, grad_x.data_ptr(), p.tokens, p.top_k, int(q.k), p.device, stream))
+    return failed(api.routing_error());
   return tuple({grad_x, grad_w});
   END_HANDLE_TH_ERRORS
 }

@@ -323,26 +323,29 @@ def expert_gemm_backward(grad, x, w, plan, gather=False, activation=None, preact
         if t is not None and t.data_ptr() % 16:
             raise ValueError(f"{label} must start on a 16-byte boundary")
     lib = capi.library("mm")
+    # All that the products write is there before the first of them: the weights' gradient, beside the
+    # rows', waits for nothing before it writes, so it may not get memory that another thread frees
+    # between the two launches while a launch of its own there still reads it.
+    grad_x = grad_w = by_row = None
+    if "x" in want:
+        # a token's rows are added before anything is rounded
+        by_row = torch.empty((rows, k), device=device, dtype=torch.float32 if gather else out_dtype or x.dtype)
+        grad_x = torch.empty_like(x) if gather else by_row
+    if "w" in want:
+        grad_w = torch.empty_like(w, dtype=out_dtype or x.dtype)
     dz = grad
     if activation is not None:
         dz = torch.empty_like(preactivation)
         lib.routing(lib._activation_gradient, capi.ELEMENT_TYPES[x.dtype], _ACTIVATIONS[activation], grad.data_ptr(),
                     preactivation.data_ptr(), dz.data_ptr(), 0, 0, plan._limit, rows, n, x.get_device())
-    grad_x = grad_w = by_row = None
     sorted_x = _sorted_rows(x, plan, k) if gather and "w" in want else x
     if "x" in want:
-        # a token's rows are added before anything is rounded
-        by_row = torch.empty((rows, k), device=device, dtype=torch.float32 if gather else out_dtype or x.dtype)
         lib.expert_product(capi.ROWS_GRADIENT, name, dz, w, by_row, plan.experts, rows, n, k, plan._offsets)
     if "w" in want:
-        grad_w = torch.empty_like(w, dtype=out_dtype or x.dtype)
         lib.expert_product(capi.WEIGHTS_GRADIENT, name, dz, sorted_x, grad_w, plan.experts, rows, n, k, plan._offsets,
                            beside_previous=by_row is not None)
-    if "x" in want:
-        grad_x = by_row
-        if gather:
-            grad_x = torch.empty_like(x)
-            _combine(by_row, None, plan, None, grad_x, k)
+    if "x" in want and gather:
+        _combine(by_row, None, plan, None, grad_x, k)
     return grad_x, grad_w
 
 
