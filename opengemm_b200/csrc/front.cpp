@@ -70,10 +70,11 @@ const Tensor* optional_tensor(PyObject* o, ScalarType type, int device, std::ini
 }
 const void* data(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
 bool aligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
-bool overlap(const Tensor& s, const Tensor& t) {
-  const char *a = static_cast<const char*>(s.data_ptr()), *b = static_cast<const char*>(t.data_ptr());
-  return a < b + t.nbytes() && b < a + s.nbytes();
+bool overlap(const Tensor& s, const void* t, size_t bytes) {
+  const char *a = static_cast<const char*>(s.data_ptr()), *b = static_cast<const char*>(t);
+  return a < b + bytes && b < a + s.nbytes();
 }
+bool overlap(const Tensor& s, const Tensor& t) { return overlap(s, t.data_ptr(), t.nbytes()); }
 Tensor empty(at::IntArrayRef shape, ScalarType type, int device) {
   return at::detail::empty_cuda(shape, type, c10::Device(c10::kCUDA, c10::DeviceIndex(device)), std::nullopt);
 }
@@ -211,6 +212,7 @@ bool plan_of(PyObject* o, Plan& p) {
   p.positions = p.token_of_row + p.rows;
   return p.rows <= 0x7FFFFFFF;
 }
+size_t plan_bytes(const Plan& p) { return (size_t(p.experts) + 1 + 2 * size_t(p.rows)) * sizeof(int); }
 
 // The tokens' rows in the plan's order, or an undefined tensor when the launch failed.
 Tensor sorted_rows(const Tensor& x, const Plan& p, int64_t k) {
@@ -256,7 +258,7 @@ PyObject* expert_gemm(PyObject*, PyObject* const* a, Py_ssize_t count) {
   bool ok = true;
   const Tensor* alpha = optional_tensor(a[5], at::kFloat, p.device, {p.experts}, ok);
   const Tensor* z = optional_tensor(a[6], own, p.device, {p.rows, q.n}, ok);
-  if (!ok || (z && (overlap(*z, *q.x) || overlap(*z, *q.w) || (alpha && overlap(*z, *alpha))))) NOT_SERVED;
+  if (!ok || (z && (overlap(*z, *q.x) || overlap(*z, *q.w) || (alpha && overlap(*z, *alpha)) || overlap(*z, p.offsets, plan_bytes(p))))) NOT_SERVED;
   Tensor out = empty({p.rows, q.gated ? q.n / 2 : q.n}, own, p.device), sorted;
   const void* x = q.x->data_ptr();
   bool gather = q.gather != 0;

@@ -53,3 +53,13 @@ def test_both_gradients_are_allocated_before_the_first_product(host_path, gather
             front.bind(addresses)
     assert [mode for mode, _ in seen] == [capi.ROWS_GRADIENT, capi.WEIGHTS_GRADIENT]
     assert seen[0][1] == seen[1][1]
+
+
+def test_a_preactivation_over_the_plan_is_refused(host_path):
+    """The launch would write over the table of rows that its other blocks still read."""
+    plan = og.expert_plan(torch.tensor([[0, 1], [2, 0], [1, 2], [0, 1]], device="cuda", dtype=torch.int32), 3)
+    x, w = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(3, 4, 64, device="cuda", dtype=torch.bfloat16)
+    for part in (plan._store[:16], plan._store[4:]):  # from the offsets on, and from the tokens on
+        over = part[:16].view(torch.bfloat16).view(8, 4)
+        with pytest.raises(ValueError, match="preactivation and plan share memory"):
+            og.expert_gemm(x, w, plan, activation="relu", preactivation=over)
