@@ -938,7 +938,7 @@ OG_API int32_t og_b200_expert_combine(int32_t dtype, int32_t y_is_f32, const voi
   if (dtype != TYPE_BF16 && dtype != TYPE_F16) return routing_fail("dtype %d is none of 1 (bfloat16), 2 (float16)", dtype);
   if (tokens < 0 || tokens > 0x7FFFFFFFll || top_k < 1 || n < 1) return routing_fail("tokens = %lld, top_k = %d, n = %d", (long long)tokens, top_k, n);
   if (!tokens) return OG_OK;
-  if (!positions || !out) return routing_fail("positions and out must be device pointers, got null");
+  if (!y || !positions || !out) return routing_fail("y, positions and out must be device pointers, got null");
   const DeviceScope on(device);
   if (const int bad = check_device(on, device)) return bad;
   CombineParams p{};
@@ -960,7 +960,7 @@ OG_API int32_t og_b200_expert_combine_gradient(int32_t dtype, const void* grad, 
   if (dtype != TYPE_BF16 && dtype != TYPE_F16) return routing_fail("dtype %d is none of 1 (bfloat16), 2 (float16)", dtype);
   if (tokens < 0 || top_k < 1 || n < 1 || tokens * top_k > 0x7FFFFFFFll) return routing_fail("tokens = %lld, top_k = %d, n = %d", (long long)tokens, top_k, n);
   if (!tokens) return OG_OK;
-  if (!grad || !weights || !positions || !grad_weights) return routing_fail("the gradient's tensors must be device pointers, got null");
+  if (!grad || !y || !weights || !positions || !grad_y || !grad_weights) return routing_fail("the gradient's tensors must be device pointers, got null");
   const DeviceScope on(device);
   if (const int bad = check_device(on, device)) return bad;
   CombineParams p{};
