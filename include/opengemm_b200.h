@@ -362,7 +362,8 @@ OG_API int32_t og_b200_expert_combine_gradient(int32_t dtype, const void* grad, 
                                                const int32_t* positions, void* grad_y, float* grad_weights,
                                                int64_t tokens, int32_t top_k, int32_t n, int32_t device, void* stream);
 
-/* dz = grad * act'(z) for rows [0, rows), or [0, *row_limit) if row_limit (device) is given.
+/* dz = grad * act'(z) for rows [0, rows), or [0, min(rows, *row_limit)) if row_limit (device) is
+ * given; other rows are neither read nor written and add nothing to the sums.
  * z, dz [rows, n]; grad [rows, n] (gated: n/2).  bias_gradient (float32 [n], or null; not for
  * a gated activation): column sums of dz before it is rounded, through a workspace of
  * ceil(rows / 16) * n floats.  Without an activation z and dz are not used. */

@@ -674,6 +674,9 @@ struct ActGradientParams {
   float a, b;
 };
 
+// Rows to work on: all, or those before a limit that an earlier kernel left on the device.
+__device__ __forceinline__ long long live_rows(const int* limit, long long rows) { return limit ? min((long long)*limit, rows) : rows; }
+
 constexpr int GRADIENT_CLUSTER = 8;  // up to this many blocks add up their column sums among themselves
 
 // dz = grad * act'(z), eight columns a thread; a gated pair writes both halves,
@@ -686,7 +689,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientParams p) {
   pdl_wait_prior_grids();
   pdl_launch_dependents();
-  const long long rows = p.limit ? *p.limit : p.rows;
+  const long long rows = live_rows(p.limit, p.rows);
   const long long first = (long long)blockIdx.x * p.block_rows;
   if (first >= rows) return;  // (never with column_sums: its grid is the blocks that have rows)
   const int lane = threadIdx.x & 31, row_lane = threadIdx.x >> 5;
@@ -762,10 +765,12 @@ __global__ void __launch_bounds__(256) act_gradient_kernel(const ActGradientPara
   cluster_sync_all();  // the others' shared memory stays until it has been read
 }
 
-// Sums over the row blocks: eight lanes take every eighth block, added in order.
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* partial, float* out, int blocks, int n) {
+// Sums over the row blocks that have rows (the others wrote no sums): eight
+// lanes take every eighth block, added in order.
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* partial, float* out, const int* limit, long long rows, int block_rows, int n) {
   pdl_wait_prior_grids();
   pdl_launch_dependents();
+  const int blocks = int((live_rows(limit, rows) + block_rows - 1) / block_rows);
   const int lane = threadIdx.x & 31, part = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float sum = 0.0f;
   if (col < n) {
@@ -1001,7 +1006,7 @@ OG_API int32_t og_b200_activation_gradient(int32_t dtype, int32_t activation, co
     if (const int bad = clustered_launch(kernel, grid, one_cluster ? blocks : 1, 256, 0, stream, p)) return bad;
   }
   if (!bias_gradient || one_cluster) return OG_OK;
-  return dependent_launch(column_sum_kernel, dim3(unsigned((n + 31) / 32)), 256, 0, stream, (const float*)workspace, bias_gradient, blocks, int(n));
+  return dependent_launch(column_sum_kernel, dim3(unsigned((n + 31) / 32)), 256, 0, stream, (const float*)workspace, bias_gradient, row_limit, (long long)rows, block_rows, int(n));
 }
 
 }  // extern "C"
