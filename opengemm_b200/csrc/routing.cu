@@ -129,6 +129,12 @@ __device__ __forceinline__ float score_of(float l, const RowScale& r, bool sigmo
   return sigmoid ? 1.0f / (1.0f + expf(-l)) : expf(l - r.top) * r.inverse;
 }
 
+// s (1 - s) of the logistic function s = 1 / (1 + e): with e = exp(-|l|) it is e / (1 + e)^2, on either side.
+__device__ __forceinline__ float logistic_slope(float l) {
+  const float e = expf(-fabsf(l)), t = 1.0f + e;
+  return e / (t * t);
+}
+
 constexpr int ROUTE_WARPS = 4;
 
 // The VALUES consecutive logits of a lane, -infinity past the last expert; one
@@ -339,8 +345,9 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RoutePara
 // d weights -> d logits.  q: the chosen scores, S their sum, g' the incoming
 // gradient times the factor:  dq = (g' - sum(g' q) / S) / S when renormalised,
 // else g'.  Softmax: dl = s (ds - sum(ds s)), where the sum vanishes after a
-// renormalisation; logistic: dl = ds s (1 - s).  The few ds are scattered
-// through shared memory (an index may be there twice).
+// renormalisation; logistic: dl = ds s (1 - s), the slope from the exponential
+// itself, as 1 - s has lost its digits where s is next to 1.  The few ds are
+// scattered through shared memory (an index may be there twice).
 template <int VALUES, typename T>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const RouteParams p) {
   __shared__ float scattered[ROUTE_WARPS][32 * VALUES];
@@ -381,8 +388,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const 
   alignas(16) T v[VALUES];
 #pragma unroll
   for (int j = 0; j < VALUES; ++j) {
-    const float s = score_of(l[j], r, sigmoid);
-    v[j] = from_float<T>(sigmoid ? ds[id0 + j] * s * (1.0f - s) : s * (ds[id0 + j] - through));
+    v[j] = from_float<T>(sigmoid ? ds[id0 + j] * logistic_slope(l[j]) : score_of(l[j], r, sigmoid) * (ds[id0 + j] - through));
   }
   constexpr int BYTES = VALUES * int(sizeof(T)), WIDE = BYTES < 16 ? BYTES : 16;
   if (p.experts % VALUES == 0 && reinterpret_cast<uintptr_t>(out) % WIDE == 0) {
