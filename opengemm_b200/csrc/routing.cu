@@ -346,8 +346,12 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const RoutePara
 // gradient times the factor:  dq = (g' - sum(g' q) / S) / S when renormalised,
 // else g'.  Softmax: dl = s (ds - sum(ds s)), where the sum vanishes after a
 // renormalisation; logistic: dl = ds s (1 - s), the slope from the exponential
-// itself, as 1 - s has lost its digits where s is next to 1.  The few ds are
-// scattered through shared memory (an index may be there twice).
+// itself, as 1 - s has lost its digits where s is next to 1.  Both differences
+// are the same with any number taken from all g' (or ds); where one expert has
+// more than half of the weight it is that expert's own, so that the gradient of
+// the largest score, a sum over the others' small ones, is not what is left of
+// two nearly equal numbers.  The few ds are scattered through shared memory (an
+// index may be there twice).
 template <int VALUES, typename T>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const RouteParams p) {
   __shared__ float scattered[ROUTE_WARPS][32 * VALUES];
@@ -370,10 +374,15 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const 
   const RowScale r = row_scale(l, sigmoid);
   const float q = score_of(chosen, r, sigmoid);
   if (p.renormalise) {
-    const float total = warp_sum(q), dot = warp_sum(g * q);
+    const float total = warp_sum(q);
+    const unsigned lead = __ballot_sync(ALL, q > 0.5f * total);
+    if (lead) {
+      const float own = __shfl_sync(ALL, g, __ffs(lead) - 1);
+      g = mine >= 0 ? g - own : 0.0f;
+    }
+    const float dot = warp_sum(g * q);
     g = mine >= 0 && total != 0.0f ? (g - dot / total) / total : 0.0f;
   }
-  const float through = sigmoid || p.renormalise ? 0.0f : warp_sum(g * q);
   __syncwarp();
   // One after another where an index is repeated, in the order of the choices.
   unsigned todo = __ballot_sync(ALL, mine >= 0);
@@ -386,9 +395,24 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const 
   }
   T* out = static_cast<T*>(p.grad_logits) + token * p.experts;
   alignas(16) T v[VALUES];
+  if (sigmoid || p.renormalise) {
 #pragma unroll
-  for (int j = 0; j < VALUES; ++j) {
-    v[j] = from_float<T>(sigmoid ? ds[id0 + j] * logistic_slope(l[j]) : score_of(l[j], r, sigmoid) * (ds[id0 + j] - through));
+    for (int j = 0; j < VALUES; ++j) v[j] = from_float<T>(ds[id0 + j] * (sigmoid ? logistic_slope(l[j]) : score_of(l[j], r, false)));
+  } else {
+    float own = 0.0f, through = 0.0f;  // the leader's ds, in its lane
+    bool leads = false;
+#pragma unroll
+    for (int j = 0; j < VALUES; ++j) {
+      l[j] = score_of(l[j], r, false);
+      if (l[j] > 0.5f) leads = true, own = ds[id0 + j];
+    }
+    const unsigned lead = __ballot_sync(ALL, leads);
+    if (lead) own = __shfl_sync(ALL, own, __ffs(lead) - 1);
+#pragma unroll
+    for (int j = 0; j < VALUES; ++j) through = fmaf(l[j], ds[id0 + j] - own, through);
+    through = warp_sum(through);
+#pragma unroll
+    for (int j = 0; j < VALUES; ++j) v[j] = from_float<T>(l[j] * (ds[id0 + j] - own - through));
   }
   constexpr int BYTES = VALUES * int(sizeof(T)), WIDE = BYTES < 16 ? BYTES : 16;
   if (p.experts % VALUES == 0 && reinterpret_cast<uintptr_t>(out) % WIDE == 0) {
