@@ -91,10 +91,18 @@ bool integer(PyObject* o, T& v) {
   return true;
 }
 bool number(PyObject* o, float& v) {
-  if (PyFloat_CheckExact(o)) v = float(PyFloat_AS_DOUBLE(o));
-  else if (PyLong_CheckExact(o)) v = float(PyLong_AsDouble(o));
-  else return false;
-  return !PyErr_Occurred();
+  if (PyFloat_CheckExact(o)) {
+    v = float(PyFloat_AS_DOUBLE(o));
+    return true;
+  }
+  if (!PyLong_CheckExact(o)) return false;
+  const double x = PyLong_AsDouble(o);
+  if (x == -1.0 && PyErr_Occurred()) {  // past the floating range: the Python front end says so
+    PyErr_Clear();
+    return false;
+  }
+  v = float(x);
+  return true;
 }
 
 int logits_type(ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }

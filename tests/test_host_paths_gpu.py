@@ -63,3 +63,15 @@ def test_a_preactivation_over_the_plan_is_refused(host_path):
         over = part[:16].view(torch.bfloat16).view(8, 4)
         with pytest.raises(ValueError, match="preactivation and plan share memory"):
             og.expert_gemm(x, w, plan, activation="relu", preactivation=over)
+
+
+def test_a_factor_past_the_floating_range_is_refused_alike(host_path):
+    a, b = torch.zeros(8, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(16, 64, device="cuda", dtype=torch.bfloat16)
+    logits = torch.zeros(4, 8, device="cuda")
+    og.gemm(a, b, activation="relu", alpha=1)
+    weights, indices = og.route(logits, 2, scale=2)
+    for call in (lambda f: og.gemm(a, b, activation="relu", alpha=f), lambda f: og.gemm_backward(og.gemm(a, b, out_dtype=torch.bfloat16), a, b, alpha=f),
+                 lambda f: og.route(logits, 2, scale=f), lambda f: og.route_backward(weights, logits, indices, scale=f)):
+        call(3)
+        with pytest.raises(OverflowError):
+            call(10**400)
