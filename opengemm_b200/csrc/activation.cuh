@@ -4,11 +4,17 @@
 // (a, b) = (1, 0) and 2 sqrt(2/pi) (1, 0.044715), since (1 + tanh u) / 2 =
 // sigmoid(2u).  The epilogues therefore carry the two coefficients at run time
 // (times -log2(e), for the base-2 exponential) and compile one code path for
-// both.  gelu itself is x * Phi(x); Phi(-|x|) comes from Abramowitz and Stegun,
-// Handbook of Mathematical Functions, 7.1.26 (|error| <= 1.5e-7 in erf), whose
-// exponential the derivative shares.  Each needs two special-function
-// instructions and 6 to 12 others a value: the epilogue's warps have to keep up
-// with the tensor pipe, and a call of erff or tanhf is two to three times that.
+// both.  gelu itself is x * Phi(x), and Phi(-u) = exp(-u^2 / 2) R(u) with
+// R(u) = erfcx(u / sqrt 2) / 2, which falls from 1/2 like 1 / u: t P(t) with
+// t = 1 / (1 + 0.305 u) and P of degree 7, the coefficients a least-maximum fit
+// of the relative error over 0 <= u <= 14 (9.4e-8; 6.5 units of 2^-24 with
+// float32 coefficients in float32).  So the tail is good relative to itself, to
+// (1.5 u^2 + 20) 2^-24 with the exponential's argument rounded: 1.3e-6 at -1,
+// 3.4e-6 at -5, 6.9e-6 at -8 (an absolute approximation of erf to 1.5e-7 has
+// 1 % there).  The derivative shares the exponential.  Each needs two
+// special-function instructions and 6 to 15 others a value: the epilogue's warps
+// have to keep up with the tensor pipe, and a call of erff or tanhf is two to
+// three times that.
 #pragma once
 
 #include <cstdint>
@@ -58,14 +64,22 @@ __device__ __forceinline__ float gate_of(float x, float a, float b) {
   return reciprocal_fast(1.0f + exp2_fast(x * fmaf(b, fminf(x * x, 1e8f), a)));
 }
 
+// P's coefficients, from the constant term on.
+constexpr float TAIL_SLOPE = 0.305f;
+constexpr float TAIL_0 = 0.121639736f, TAIL_1 = 0.122466817f, TAIL_2 = 0.103420876f, TAIL_3 = 0.121021658f;
+constexpr float TAIL_4 = -0.0379767939f, TAIL_5 = 0.185716867f, TAIL_6 = -0.1529883f, TAIL_7 = 0.0366991907f;
+
 // Phi(-|x|), and exp(-x^2 / 2) through `density`.
 __device__ __forceinline__ float lower_tail(float x, float* density) {
-  const float t = reciprocal_fast(fmaf(0.3275911f * 0.7071067811865476f, fabsf(x), 1.0f));
+  const float t = reciprocal_fast(fmaf(TAIL_SLOPE, fabsf(x), 1.0f));
   const float e = exp2_fast(x * x * -0.7213475204444817f);  // -log2(e) / 2
-  float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-  p = fmaf(p, t, 0.5f * 1.421413741f);
-  p = fmaf(p, t, 0.5f * -0.284496736f);
-  p = fmaf(p, t, 0.5f * 0.254829592f);
+  float p = fmaf(TAIL_7, t, TAIL_6);
+  p = fmaf(p, t, TAIL_5);
+  p = fmaf(p, t, TAIL_4);
+  p = fmaf(p, t, TAIL_3);
+  p = fmaf(p, t, TAIL_2);
+  p = fmaf(p, t, TAIL_1);
+  p = fmaf(p, t, TAIL_0);
   *density = e;
   return p * t * e;
 }
@@ -114,14 +128,17 @@ __device__ __forceinline__ float2 act_value2(float2 x, float a, float b) {
     return mul2(x, make_float2(reciprocal_fast(e.x), reciprocal_fast(e.y)));
   } else if constexpr (SHAPE == SHAPE_PHI) {
     const float2 m = make_float2(fabsf(x.x), fabsf(x.y));
-    const float2 d = fma2(both(0.3275911f * 0.7071067811865476f), m, both(1.0f));
+    const float2 d = fma2(both(TAIL_SLOPE), m, both(1.0f));
     const float2 t = make_float2(reciprocal_fast(d.x), reciprocal_fast(d.y));
     const float2 q = mul2(mul2(x, x), both(-0.7213475204444817f));
     const float2 e = make_float2(exp2_fast(q.x), exp2_fast(q.y));
-    float2 p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
-    p = fma2(p, t, both(0.5f * 1.421413741f));
-    p = fma2(p, t, both(0.5f * -0.284496736f));
-    p = fma2(p, t, both(0.5f * 0.254829592f));
+    float2 p = fma2(both(TAIL_7), t, both(TAIL_6));
+    p = fma2(p, t, both(TAIL_5));
+    p = fma2(p, t, both(TAIL_4));
+    p = fma2(p, t, both(TAIL_3));
+    p = fma2(p, t, both(TAIL_2));
+    p = fma2(p, t, both(TAIL_1));
+    p = fma2(p, t, both(TAIL_0));
     return fma2(make_float2(-fminf(m.x, 1e4f), -fminf(m.y, 1e4f)), mul2(mul2(p, t), e), make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
   } else {
     return make_float2(act_value<SHAPE>(x.x, a, b), act_value<SHAPE>(x.y, a, b));
