@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/opengemm_b200.h"
+#include "dependent_launch.h"
 #include "device_scope.h"
 #include "experts_launch.h"
 #include "launch_common.h"
@@ -180,7 +181,7 @@ cudaError_t add_parts(const void* partial, void* out, long long values, int part
   config.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  attr.val.programmaticStreamSerializationAllowed = dependent_launches();
   config.attrs = &attr;
   config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, add_parts_kernel<T>, static_cast<const float4*>(partial), static_cast<T*>(out), values / 4, parts);

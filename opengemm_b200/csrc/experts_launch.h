@@ -3,6 +3,7 @@
 
 #include <atomic>
 
+#include "dependent_launch.h"
 #include "experts.cuh"
 
 namespace og {
@@ -36,7 +37,7 @@ cudaError_t expert_launch(const ExpertParams& params, int grid, int smem_bytes, 
     ++count;
   }
   attrs[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[count].val.programmaticStreamSerializationAllowed = 1;
+  attrs[count].val.programmaticStreamSerializationAllowed = dependent_launches();
   ++count;
   config.attrs = attrs;
   config.numAttrs = count;

@@ -20,6 +20,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include "dependent_launch.h"
 #include "device_scope.h"
 #include "kernel.cuh"
 #include "kernels_fixed.cuh"
@@ -365,13 +366,12 @@ int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* str
   char why[320];
   if (want_scaled >= 0 && int(p.format->scaled) != want_scaled)
     return fail(OG_ERR_LAUNCH, "dtype %.16s does not belong to this library", g->dtype);
-  static const bool pdl_enabled = [] { const char* e = getenv("OPENGEMM_PDL"); return !(e && e[0] == '0'); }();
   if (fused && skinny_serves(*g, *p.format, io)) {
     const int rc = check_pointers(*g, p, io, alpha, why, sizeof why);
     if (rc != OG_OK) return fail(rc, "%s", why);
     const int followed = follow_device(device);
     if (followed != OG_OK) return followed;
-    const cudaError_t launched = launch_skinny(*g, *p.format, io, alpha, pdl_enabled, sm_count_of(device), static_cast<cudaStream_t>(stream));
+    const cudaError_t launched = launch_skinny(*g, *p.format, io, alpha, dependent_launches(), sm_count_of(device), static_cast<cudaStream_t>(stream));
     if (launched != cudaSuccess) return fail(OG_ERR_LAUNCH, "kernel launch failed: %s", cudaGetErrorString(launched));
     return OG_OK;
   }
@@ -403,7 +403,7 @@ int launch_impl(const OgGemm* g, const LaunchPointers& io, int device, void* str
     params.tx_bytes += overcredit_next;
     overcredit_next = 0;
   }
-  params.pdl = pdl_enabled ? (independent_inputs.load(std::memory_order_relaxed) ? 2 : 1) : 0;
+  params.pdl = dependent_launches() ? (independent_inputs.load(std::memory_order_relaxed) ? 2 : 1) : 0;
 
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sm_count = sm_count_of(device);

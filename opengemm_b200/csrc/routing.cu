@@ -18,6 +18,7 @@
 
 #include "../../include/opengemm_b200.h"
 #include "activation.cuh"
+#include "dependent_launch.h"
 #include "device_scope.h"
 #include "ptx.cuh"
 
@@ -842,7 +843,7 @@ int clustered_launch(void (*kernel)(Args...), dim3 grid, int cluster, int thread
   config.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attrs[2];
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[0].val.programmaticStreamSerializationAllowed = dependent_launches();
   attrs[1].id = cudaLaunchAttributeClusterDimension;
   attrs[1].val.clusterDim.x = cluster;
   attrs[1].val.clusterDim.y = 1;

@@ -1,12 +1,16 @@
-"""The host paths of the feed-forward calls, native and in Python."""
+"""The host paths of the feed-forward calls, native and in Python, and the switch that turns
+dependent launches off."""
 
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import opengemm_b200 as og
-from opengemm_b200 import capi
+from opengemm_b200 import build, capi
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +79,56 @@ def test_a_factor_past_the_floating_range_is_refused_alike(host_path):
         call(3)
         with pytest.raises(OverflowError):
             call(10**400)
+
+
+PROGRAMMATIC_EDGES = """
+import ctypes
+import torch
+import opengemm_b200 as og
+
+def step():
+    weights, indices = og.route(logits, 2)
+    plan = og.expert_plan(indices, 6)
+    z = torch.empty(plan.rows, 128, device="cuda", dtype=torch.bfloat16)
+    h = og.expert_gemm(x, w, plan, gather=True, activation="swiglu", preactivation=z)
+    y = og.expert_combine(h, weights, plan)
+    grad_h, grad_weights = og.expert_combine_backward(y, h, weights, plan)
+    grad_x, grad_w = og.expert_gemm_backward(grad_h, x, w, plan, gather=True, activation="swiglu", preactivation=z)
+    kept = torch.empty(5000, 64, device="cuda", dtype=torch.bfloat16)
+    c = og.gemm(tall, wide, out_dtype=torch.bfloat16, activation="gelu", preactivation=kept)
+    few = og.gemm(tall[:2], wide, out_dtype=torch.bfloat16, activation="gelu")
+    return og.route_backward(grad_weights, logits, indices), grad_x, grad_w, few, *og.gemm_backward(
+        c, tall, wide, activation="gelu", preactivation=kept, want=("a", "b", "bias"))
+
+torch.manual_seed(0)
+x, logits = torch.randn(300, 64).bfloat16().cuda(), torch.randn(300, 6).cuda()
+w, tall, wide = torch.randn(6, 128, 64).bfloat16().cuda(), torch.randn(5000, 72).bfloat16().cuda(), torch.randn(64, 72).bfloat16().cuda()
+eager = [t.clone() for t in step()]
+graph = torch.cuda.CUDAGraph(keep_graph=True)
+with torch.cuda.graph(graph):
+    captured = step()
+edges_of = ctypes.CDLL("libcuda.so.1").cuGraphGetEdges_v2
+handle, count = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t(0)
+assert edges_of(handle, None, None, None, ctypes.byref(count)) == 0
+ends, data = [(ctypes.c_void_p * count.value)() for _ in range(2)], (ctypes.c_uint8 * (8 * count.value))()
+assert edges_of(handle, *ends, data, ctypes.byref(count)) == 0
+graph.instantiate()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(eager, captured))
+print("programmatic", sum(data[8 * i + 2] == 1 for i in range(count.value)), "of", count.value)  # a type behind two ports
+"""
+
+
+@pytest.mark.parametrize("front", ["1", "0"])
+def test_dependent_launches_can_be_turned_off(front):
+    """OPENGEMM_PDL=0 leaves no launch that may start before its predecessor has ended, as a captured graph's edges show."""
+    counts = {}
+    for on in ("1", "0"):
+        done = subprocess.run([sys.executable, "-c", PROGRAMMATIC_EDGES], cwd=build.ROOT, capture_output=True, text=True, timeout=300,
+                              env={**os.environ, "OPENGEMM_PDL": on, "OPENGEMM_FRONT": front})
+        assert done.returncode == 0, done.stderr[-2000:]
+        words = done.stdout.split()
+        counts[on] = int(words[1]), int(words[3])
+    assert counts["1"][0] > counts["1"][1] // 2
+    assert counts["0"][0] == 0 and counts["0"][1] >= 12
