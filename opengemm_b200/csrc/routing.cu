@@ -449,13 +449,18 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_gradient_kernel(const 
 constexpr int PLAN_WARPS = 32;
 constexpr int PLAN_CHUNK = 8192;  // pairs per block; up to this many need no histogram
 constexpr int PLAN_EACH = PLAN_CHUNK / (PLAN_WARPS * 32);
+// Above this many chunks their counts are added up once, by a kernel between the
+// two; up to it each block adds up all of them itself, which saves that launch but
+// grows with the square of the pairs (256 experts: 16 chunks 11.7 us, 13.2 with the
+// kernel between; 64 chunks 13.8 and 13.9; 256 chunks 39 and 24; 1024 chunks 302 and 80).
+constexpr int PLAN_SCAN = 64;
 
 struct PlanParams {
   const int* indices;
   int* offsets;    // [experts + 1]
   int* tokens;     // [pairs] the token of each sorted row
   int* positions;  // [pairs] the sorted row of each pair, -1 for one that goes nowhere
-  int* histogram;  // [chunks, experts]
+  int* histogram;  // [chunks, experts] counts; above PLAN_SCAN chunks then the counts up to and with each chunk
   int pairs, top_k, experts, chunks;
 };
 
@@ -472,6 +477,38 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_histogram_kernel(const P
   }
   __syncthreads();
   for (int e = threadIdx.x; e < p.experts; e += blockDim.x) p.histogram[blockIdx.x * p.experts + e] = counts[e];
+}
+
+// Counts of each chunk -> counts up to and with it, in place.  A block has 32
+// experts, one a lane; its warps each take a run of chunks, add it up, learn from
+// one another what comes before it, and go over it again.
+__global__ void __launch_bounds__(PLAN_WARPS * 32) plan_scan_kernel(const PlanParams p) {
+  __shared__ int sums[PLAN_WARPS][32];
+  pdl_wait_prior_grids();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = blockIdx.x * 32 + lane;
+  const int each = (p.chunks + PLAN_WARPS - 1) / PLAN_WARPS, first = min(warp * each, p.chunks), last = min(first + each, p.chunks);
+  int* const column = p.histogram + e;
+  int sum = 0;
+  if (e < p.experts) {
+#pragma unroll 8
+    for (int c = first; c < last; ++c) sum += column[(long long)c * p.experts];
+  }
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (e >= p.experts) return;
+  int run = 0;
+  for (int w = 0; w < warp; ++w) run += sums[w][lane];
+  for (int c0 = first; c0 < last; c0 += 8) {  // eight loads in flight
+    int n[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n[i] = c0 + i < last ? column[(long long)(c0 + i) * p.experts] : 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      run += n[i];
+      if (c0 + i < last) column[(long long)(c0 + i) * p.experts] = run;
+    }
+  }
 }
 
 __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams p) {
@@ -513,7 +550,10 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_kernel(const PlanParams 
       }
     }
     int before = 0, total = run;
-    if (p.chunks > 1) {
+    if (p.chunks > PLAN_SCAN) {
+      if (blockIdx.x) before = p.histogram[(blockIdx.x - 1) * p.experts + e];
+      total = p.histogram[(p.chunks - 1) * p.experts + e];
+    } else if (p.chunks > 1) {
       total = 0;
 #pragma unroll 8
       for (int c = 0; c < p.chunks; ++c) {
@@ -946,6 +986,9 @@ OG_API int32_t og_b200_expert_plan(const int32_t* indices, int64_t tokens, int32
   p.chunks = std::max(1, (p.pairs + PLAN_CHUNK - 1) / PLAN_CHUNK);
   if (p.chunks > 1) {
     if (const int bad = dependent_launch(plan_histogram_kernel, dim3(p.chunks), PLAN_WARPS * 32, experts * sizeof(int), stream, p)) return bad;
+  }
+  if (p.chunks > PLAN_SCAN) {
+    if (const int bad = dependent_launch(plan_scan_kernel, dim3((experts + 31) / 32), PLAN_WARPS * 32, 0, stream, p)) return bad;
   }
   const size_t smem = size_t(PLAN_WARPS + 2) * experts * sizeof(int);
   if (smem > 48 * 1024) {  // up to 136 KiB for 1024 experts
