@@ -70,18 +70,21 @@ struct ExpertPlan {
 // every SM work when there are few.  The choice is within 10 % of the best of the
 // four but for single cases (8 experts of 300 to 700 rows, 2048 x 2048: 43 us for 37;
 // 16 of some 100, 1536 x 3000, rows that are no whole lines: 51 us for 41).
+// Gathered rows go to single CTAs: with the few rows an expert for which gathering
+// pays, a pair's second CTA has none.
 // With `parts` > 1 a single group's work is cut along its reduction into that
 // many launches' worth of tiles.
-ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count, int parts = 1) {
+ExpertPlan choose_plan(int mode, bool gather, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count, int parts = 1) {
   const int busy = std::max(1, std::min(groups, rows));
   const double rows_each = double(std::max(rows, 1)) / busy;
   static const ExpertPlan menu[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
   static const int multiply_cycles[3][4] = {{740, 950, 560, 390}, {750, 1025, 615, 535}, {685, 725, 460, 290}};  // by mode
   static const int stream_cycles[2][4] = {{780, 1430, 680, 525}, {780, 1090, 680, 525}};
   static const int least_cycles[] = {9200, 4900, 2950, 2450};
-  ExpertPlan best = menu[0];
+  const int first = gather ? 1 : 0;
+  ExpertPlan best = menu[first];
   double best_cost = 0;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = first; i < 4; ++i) {
     const ExpertPlan& c = menu[i];
     const int out_n = glu ? c.tile_n / 2 : c.tile_n, tile_m = 128 * c.cta_group;
     const double m_tiles = mode == MODE_DW   ? ceil_div(m_out, tile_m)
@@ -93,7 +96,7 @@ ExpertPlan choose_plan(int mode, bool glu, int groups, int rows, int m_out, int 
     if (mode != MODE_DW && c.cta_group == 2 && rows_each <= 128) block *= 1.22;  // the second CTA has no rows
     const double waves = tiles / (sm_count / c.cta_group);
     const double cost = (groups == 1 ? std::ceil(waves) : std::max(1.0, waves + 0.5)) * std::max(blocks * block + 2000, double(least_cycles[i]));
-    if (i == 0 || cost < best_cost) best = c, best_cost = cost;
+    if (i == first || cost < best_cost) best = c, best_cost = cost;
   }
   best.cost = best_cost;
   return best;
@@ -146,7 +149,7 @@ int choose_parts(int mode, int m, int n, int k, int sm_count) {
   double best_cost = 0;
   for (int parts = 1; parts <= 16 && parts * 4 <= std::max(4, blocks); parts *= 2) {
     const double sums = parts > 1 ? 6000 + double(parts) * m_out * k * 8 / 3400 : 0;
-    const double cost = choose_plan(mode, false, 1, m, n, k, blocks, sm_count, parts).cost + sums;
+    const double cost = choose_plan(mode, false, false, 1, m, n, k, blocks, sm_count, parts).cost + sums;
     if (parts == 1 || cost < 0.9 * best_cost) best = parts, best_cost = cost;
   }
   return best;
@@ -233,7 +236,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   p.k = mode == MODE_FORWARD ? g.k : g.n;
   p.block_k = 128 / elem;
   p.k_blocks = ceil_div(p.k, p.block_k);
-  const ExpertPlan plan = choose_plan(mode, glu, g.groups, g.rows, p.m_out, p.cols, p.k_blocks, sm_count, parts);
+  const ExpertPlan plan = choose_plan(mode, gather, glu, g.groups, g.rows, p.m_out, p.cols, p.k_blocks, sm_count, parts);
   p.rows_per_group = g.rows;
   if (parts > 1) {
     if (mode == MODE_DW) {

@@ -100,18 +100,11 @@ struct ExpertTile {
 };
 
 // Gathered rows: four rows of `tmap` (one-row boxes) into 512 consecutive bytes.
-template <int CTA_GROUP>
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
-  if constexpr (CTA_GROUP == 1)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(tmap), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(tmap), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
-        : "memory");
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst), "l"(tmap), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+      : "memory");
 }
 
 template <int CTA_GROUP>
@@ -135,9 +128,10 @@ __device__ __forceinline__ uint64_t column_operand_desc(uint32_t smem_addr) {
   return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(8192 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// GATHER and GLU: MODE_FORWARD only.
+// GATHER and GLU: MODE_FORWARD only; GATHER: single CTAs only.
 template <int KIND, int CTA_GROUP, int MODE, bool GATHER, bool GLU, int OUT_BYTES>
 __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __grid_constant__ ExpertParams p) {
+  static_assert(!GATHER || (MODE == MODE_FORWARD && CTA_GROUP == 1));
   constexpr int TILE_M = 128 * CTA_GROUP;
   constexpr bool X_COLUMNS = MODE == MODE_DW, Y_COLUMNS = MODE != MODE_FORWARD;
   constexpr int CHUNK = XP_CHUNK, ROW_BYTES = CHUNK * OUT_BYTES, UNITS = ROW_BYTES / 16, UNIT = 16 / OUT_BYTES;
@@ -335,7 +329,7 @@ __global__ void __launch_bounds__(xp_threads(MODE), 1) expert_kernel(const __gri
           }
           if constexpr (GATHER) {
             if (4 * lane < mine)
-              tma_gather4<CTA_GROUP>(sx + lane * 512, &p.map_x32, kb * block_k, token[0], token[1], token[2], token[3], full);
+              tma_gather4(sx + lane * 512, &p.map_x32, kb * block_k, token[0], token[1], token[2], token[3], full);
           }
           if constexpr (MODE == MODE_DW) {  // a short block is on its way: the clearing warp may look for it
             if (leads && rank == 0 && kb == blocks - 1 && (w.rows & 63)) mbar_arrive(bar_go + 8 * stage);

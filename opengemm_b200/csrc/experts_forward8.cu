@@ -5,9 +5,8 @@ namespace og {
 
 extern const ExpertKernel EXPERT_FORWARD8[] = {
     OG_EXPERT_KERNEL(KIND_F8F6F4, 1, MODE_FORWARD, 0, 0, 2), OG_EXPERT_KERNEL(KIND_F8F6F4, 2, MODE_FORWARD, 0, 0, 2),
-    OG_EXPERT_KERNEL(KIND_F8F6F4, 1, MODE_FORWARD, 1, 0, 2), OG_EXPERT_KERNEL(KIND_F8F6F4, 2, MODE_FORWARD, 1, 0, 2),
     OG_EXPERT_KERNEL(KIND_F8F6F4, 1, MODE_FORWARD, 0, 1, 2), OG_EXPERT_KERNEL(KIND_F8F6F4, 2, MODE_FORWARD, 0, 1, 2),
-    OG_EXPERT_KERNEL(KIND_F8F6F4, 1, MODE_FORWARD, 1, 1, 2), OG_EXPERT_KERNEL(KIND_F8F6F4, 2, MODE_FORWARD, 1, 1, 2),
+    OG_EXPERT_KERNEL(KIND_F8F6F4, 1, MODE_FORWARD, 1, 0, 2), OG_EXPERT_KERNEL(KIND_F8F6F4, 1, MODE_FORWARD, 1, 1, 2),
 };
 extern const int EXPERT_FORWARD8_COUNT = sizeof(EXPERT_FORWARD8) / sizeof(EXPERT_FORWARD8[0]);
 
