@@ -313,6 +313,8 @@ typedef struct OgExpertProduct {
                               went to the stream before, that it writes nothing which this one
                               reads or writes, and that all of this one's memory was the
                               caller's before that launch; the two then run side by side */
+  int32_t tile;           /* 0: chosen by an estimate; to measure or test one: 1 a pair of CTAs with
+                             256 columns (not with `tokens`), 2 one CTA with 256, 3 with 128, 4 with 64 */
   char dtype[16];
 } OgExpertProduct;
 OG_API int32_t og_b200_expert_product(const OgExpertProduct* product, int32_t device, void* stream);

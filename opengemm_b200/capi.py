@@ -56,7 +56,7 @@ class OgExpertProduct(ctypes.Structure):
 
     _fields_ = ([(f, c_void_p) for f in ("x", "w", "offsets", "tokens", "alpha", "out", "preactivation")]
                 + [(f, c_int32) for f in ("mode", "groups", "rows", "x_rows", "n", "k", "activation", "out_f32")]
-                + [("factor", ctypes.c_float), ("beside_previous", c_int32), ("dtype", c_char * 16)])
+                + [("factor", ctypes.c_float), ("beside_previous", c_int32), ("tile", c_int32), ("dtype", c_char * 16)])
 
 
 class OgGemmGradients(ctypes.Structure):
@@ -374,7 +374,7 @@ class Library:
         product = OgExpertProduct(
             x.data_ptr(), w.data_ptr(), offsets, tokens, 0 if alpha is None else alpha.data_ptr(), out.data_ptr(),
             0 if preactivation is None else preactivation.data_ptr(), mode, groups, rows, x_rows, n, k, activation,
-            out.dtype is torch.float32, 1.0, beside_previous, dtype,
+            out.dtype is torch.float32, 1.0, beside_previous, 0, dtype,
         )
         if self._expert_product(byref(product), device, raw_stream(device)) != OG_OK:
             raise RuntimeError(self._experts_error().decode())

@@ -49,6 +49,8 @@ struct ExpertPlan {
   double cost = 0;
 };
 
+constexpr ExpertPlan TILES[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
+
 // The tile of a launch: the cheapest of a short menu by an estimate.
 //
 // With several groups only their number and the number of all rows are known
@@ -77,15 +79,14 @@ struct ExpertPlan {
 ExpertPlan choose_plan(int mode, bool gather, bool glu, int groups, int rows, int m_out, int cols, int blocks_fixed, int sm_count, int parts = 1) {
   const int busy = std::max(1, std::min(groups, rows));
   const double rows_each = double(std::max(rows, 1)) / busy;
-  static const ExpertPlan menu[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
   static const int multiply_cycles[3][4] = {{740, 950, 560, 390}, {750, 1025, 615, 535}, {685, 725, 460, 290}};  // by mode
   static const int stream_cycles[2][4] = {{780, 1430, 680, 525}, {780, 1090, 680, 525}};
   static const int least_cycles[] = {9200, 4900, 2950, 2450};
   const int first = gather ? 1 : 0;
-  ExpertPlan best = menu[first];
+  ExpertPlan best = TILES[first];
   double best_cost = 0;
   for (int i = first; i < 4; ++i) {
-    const ExpertPlan& c = menu[i];
+    const ExpertPlan& c = TILES[i];
     const int out_n = glu ? c.tile_n / 2 : c.tile_n, tile_m = 128 * c.cta_group;
     const double m_tiles = mode == MODE_DW   ? ceil_div(m_out, tile_m)
                            : groups == 1     ? ceil_div(std::max(rows, 1), tile_m)
@@ -211,6 +212,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   if (g.out_f32 && mode == MODE_FORWARD) return experts_fail(OG_ERR_LAUNCH, "the forward product writes 16-bit values");
   const bool gather = g.tokens != nullptr;
   if (gather && mode != MODE_FORWARD) return experts_fail(OG_ERR_LAUNCH, "only the forward product gathers its rows");
+  if (g.tile < 0 || g.tile > 4 || (gather && g.tile == 1)) return experts_fail(OG_ERR_LAUNCH, "tile %d is none of 0..4, or a pair for gathered rows", g.tile);
   if (device < 0 || device >= XP_DEVICES) return experts_fail(OG_ERR_LAUNCH, "device %d is out of range: this library serves devices 0..%d", device, XP_DEVICES - 1);
   const DeviceScope on(device);
   if (on.status() != cudaSuccess) return experts_fail(OG_ERR_LAUNCH, "cudaSetDevice(%d): %s", device, cudaGetErrorString(on.status()));
@@ -236,7 +238,7 @@ int launch_product(const OgExpertProduct& g, int device, void* stream, int parts
   p.k = mode == MODE_FORWARD ? g.k : g.n;
   p.block_k = 128 / elem;
   p.k_blocks = ceil_div(p.k, p.block_k);
-  const ExpertPlan plan = choose_plan(mode, gather, glu, g.groups, g.rows, p.m_out, p.cols, p.k_blocks, sm_count, parts);
+  const ExpertPlan plan = g.tile ? TILES[g.tile - 1] : choose_plan(mode, gather, glu, g.groups, g.rows, p.m_out, p.cols, p.k_blocks, sm_count, parts);
   p.rows_per_group = g.rows;
   if (parts > 1) {
     if (mode == MODE_DW) {
