@@ -154,6 +154,9 @@ def gemm(a, b, sfa=None, sfb=None, out=None, atype=None, btype=None, out_dtype=N
             the activation's argument, which `gemm_backward` reads.  With any of
             these three, neither it nor `out` may share memory with another input.
 
+    Nothing is recorded for automatic differentiation (`gemm_backward` computes the
+    gradients): the result does not require one, whatever the operands do.
+
     Returns:
         `(M, N)` row-major: float32 for dense formats (bfloat16 with
         `out_dtype=torch.bfloat16`, float16 with `out_dtype=torch.float16`), int32

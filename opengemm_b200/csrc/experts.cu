@@ -69,9 +69,17 @@ constexpr ExpertPlan TILES[] = {{2, 256}, {1, 256}, {1, 128}, {1, 64}};
 // tiles of 128 in the forward product (16 tokens x 8 of 64 experts, 2048 x 2048
 // weights: 59 us; 65 us in pairs, 63 us 256 wide, 66 us 64 wide), of 256 in the
 // rows' gradient (64 experts, three rows each: 84 us for 89).  Narrow tiles give
-// every SM work when there are few.  The choice is within 10 % of the best of the
-// four but for single cases (8 experts of 300 to 700 rows, 2048 x 2048: 43 us for 37;
-// 16 of some 100, 1536 x 3000, rows that are no whole lines: 51 us for 41).
+// every SM work when there are few.
+//
+// Measured with every tile (OgExpertProduct.tile) over 27 launches, 8 to 64 experts
+// of 2 to 1670 rows: the choice is within 8 % of the best of the four in 19 of them.
+// The others are experts of some 100 to 700 rows, where the last, half-filled tile
+// counts most: the forward product and the rows' gradient take pairs where one CTA
+// of 256 would do (4 x 300 and 4 x 700 rows, 2048 x 2048: rows' gradient 49 us for 36,
+// forward 40 for 36; 16 x 100, 1536 x 3000: forward 58 for 45, rows' gradient 40 for
+// 34), and the weights' gradient one CTA where a pair would (8 x 512, 2048 x 2048: 36
+// us for 31.5): a single cost a block prices a pair's second CTA and its longer
+// store alike.
 // Gathered rows go to single CTAs: with the few rows an expert for which gathering
 // pays, a pair's second CTA has none.
 // With `parts` > 1 a single group's work is cut along its reduction into that

@@ -30,7 +30,8 @@
 // rows an expert the ring of stages: a K block moves 32 KB a CTA in pairs, 48 KB
 // in a CTA of 128 x 256, against 512 cycles of MMAs, and memory or L2 is over a
 // microsecond away (8 experts of 512 rows, weights' gradient 2048 x 2048: 31 us in
-// pairs with six stages, 36 us with four of the larger ones).  Every stage counts:
+// pairs with six stages, 36 us with four of the larger ones, which the estimate of
+// experts.cu takes there).  Every stage counts:
 // staging two chunks of output a warp, for whole 128-byte lines, takes one and was
 // slower (36 -> 39 us), and asking for the weights a few blocks ahead in L2 costs
 // the copy engine as much as loading them (35 -> 38 us in the rows' product, 34 ->

@@ -11,6 +11,10 @@ As in `gemm`, operands are contiguous CUDA tensors, K is innermost, sums are
 float32, and calls are asynchronous on the current stream of the operands'
 device.  How many rows each expert gets is known on the device only: nothing
 here synchronises, and all calls can be captured into a CUDA graph.
+
+Nothing is recorded for automatic differentiation: results do not require a
+gradient, whatever the operands do.  Call the `_backward`s, or wrap a pair of
+calls in a `torch.autograd.Function`.
 """
 
 from ctypes import byref
@@ -298,7 +302,8 @@ def expert_gemm_backward(grad, x, w, plan, gather=False, activation=None, preact
             operands' (default) or `torch.float32`.
 
     Returns:
-        `(grad_x, grad_w)`, None in the place of what is not wanted.
+        `(grad_x, grad_w)`, None in the place of what is not wanted.  Without
+        `gather` the rows of `grad_x` behind the plan's last are not written.
     """
     front = capi.front()
     if front is not None and (out_dtype is None or out_dtype is x.dtype) and set(want) <= {"x", "w"}:
