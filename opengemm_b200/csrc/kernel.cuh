@@ -401,7 +401,8 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
       for (int u = 0; u < UNITS; ++u) res[u] = src[u];
     };
     ask_residual(chunk0);
-    float my_bias = bias ? __ldg(bias + min(col0 + chunk0 + lane, rows_n - 1)) : 0.0f;
+    // Ordinary loads, as of everything an earlier kernel may still have been writing when this one started.
+    float my_bias = bias ? bias[min(col0 + chunk0 + lane, rows_n - 1)] : 0.0f;
     const int slot = (p.acc_slots == 2) ? (tile_idx & 1) : 0;
     const uint32_t use = (p.acc_slots == 2) ? (tile_idx >> 1) : tile_idx;
     const bool ready = mbar_wait(bar_acc_full + 8 * slot, use & 1, ctx, SITE_EPI_ACC_FULL);
@@ -475,7 +476,7 @@ __device__ __forceinline__ void fused_epilogue(const GemmParams& p, const WaitCt
       if (bias) {
         st_shared_u32(bias_buf + lane * 4, __float_as_uint(my_bias));
         __syncwarp();
-        my_bias = __ldg(bias + min(col0 + next + lane, rows_n - 1));
+        my_bias = bias[min(col0 + next + lane, rows_n - 1)];
 #pragma unroll
         for (int u = 0; u < CHUNK / 4; ++u) {
           const uint4 q = ld_shared_v4(bias_buf + u * 16);
@@ -1187,9 +1188,9 @@ __global__ void __launch_bounds__(kernel_threads(FUSED), 1) gemm_kernel(const __
           if (!transpose_out) {
 #pragma unroll
             for (int j = 0; j < CHUNK; ++j)
-              v[j] = __float_as_uint(__uint_as_float(v[j]) + __ldg(bias + min(col0 + c + j, rows_n - 1)));
+              v[j] = __float_as_uint(__uint_as_float(v[j]) + bias[min(col0 + c + j, rows_n - 1)]);
           } else {
-            const float mine = __ldg(bias + min(row, rows_m - 1));
+            const float mine = bias[min(row, rows_m - 1)];
 #pragma unroll
             for (int j = 0; j < CHUNK; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + mine);
           }

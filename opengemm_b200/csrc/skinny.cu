@@ -52,9 +52,12 @@ __device__ __forceinline__ void widen2(uint32_t w, float& lo, float& hi) {
   }
 }
 
-__device__ __forceinline__ uint4 load_streamed(const uint4* p) {  // read once: no place in L1, which A keeps
+// Read once: no place in L1, which A keeps.  Not a read-only (.nc) load: the
+// block may have started while an earlier kernel was still writing B, and such a
+// load asks for memory that nobody writes as long as this kernel runs.
+__device__ __forceinline__ uint4 load_streamed(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 

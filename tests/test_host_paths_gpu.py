@@ -132,3 +132,30 @@ def test_dependent_launches_can_be_turned_off(front):
         counts[on] = int(words[1]), int(words[3])
     assert counts["1"][0] > counts["1"][1] // 2
     assert counts["0"][0] == 0 and counts["0"][1] >= 12
+
+
+@pytest.mark.parametrize("m", [2, 200])
+def test_a_weight_and_a_bias_that_the_launch_before_writes(m):
+    """A launch starts while the one before still writes: its weight, its residual and its bias may be what that one writes."""
+    g = torch.Generator().manual_seed(m)
+    x = torch.randn(m, 512, generator=g).bfloat16().cuda()
+    sources = [torch.randn(1024, 256, generator=g).bfloat16().cuda() for _ in range(8)]
+    middle = torch.randn(512, 256, generator=g).bfloat16().cuda()
+    one, bias = torch.ones(1, 256, device="cuda", dtype=torch.bfloat16), torch.empty(1, 1024, device="cuda")
+    weight, residual = torch.empty(1024, 512, device="cuda", dtype=torch.bfloat16), torch.empty(m, 1024, device="cuda", dtype=torch.bfloat16)
+
+    def step(source, wait):
+        og.gemm(one, source, out=bias)
+        wait()
+        og.gemm(x[:, :256].contiguous(), source, out=residual)
+        wait()
+        og.gemm(source, middle, out=weight)
+        wait()
+        return og.gemm(x, weight, out_dtype=torch.bfloat16, bias=bias[0], activation="silu", residual=residual)
+
+    wants = [step(source, torch.cuda.synchronize) for source in sources]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        gots = [step(source, lambda: None) for source in sources]
+        for got, want in zip(gots, wants):
+            assert torch.equal(got, want)
