@@ -5,6 +5,7 @@ import ctypes
 import os
 import subprocess
 import sys
+import threading
 
 import pytest
 import torch
@@ -159,3 +160,41 @@ def test_a_weight_and_a_bias_that_the_launch_before_writes(m):
         gots = [step(source, lambda: None) for source in sources]
         for got, want in zip(gots, wants):
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("out_dtype", [None, torch.float32], ids=str)
+def test_two_threads_on_one_stream(host_path, out_dtype):
+    """Gradients side by side in one thread, products whose operands are dropped at once in another: memory passes
+    from one to the other in the order of the stream, which every launch has to keep."""
+    torch.manual_seed(3)
+    plan = og.expert_plan(torch.randint(0, 4, (600, 2), device="cuda", dtype=torch.int32), 4)
+    x, w = torch.randn(600, 256, device="cuda").bfloat16(), torch.randn(4, 512, 256, device="cuda").bfloat16()
+    grad, z = torch.randn(1200, 256, device="cuda").bfloat16(), torch.randn(1200, 512, device="cuda").bfloat16()
+    a, b = torch.randn(2048 if out_dtype is None else 4096, 256, device="cuda").bfloat16(), torch.randn(512, 256, device="cuda").bfloat16()
+
+    def gradients():
+        return og.expert_gemm_backward(grad, x, w, plan, gather=True, activation="swiglu", preactivation=z, out_dtype=out_dtype)
+
+    def product():
+        dropped = a.clone()  # as large as the weights' gradient
+        return (og.gemm(dropped, b, out_dtype=torch.bfloat16),)
+
+    calls = {"gradients": gradients, "product": product}
+    wants = {name: call() for name, call in calls.items()}
+    torch.cuda.synchronize()
+    wrong, failed = [], []
+
+    def run(name):
+        try:
+            for _ in range(150):
+                wrong.extend((got != want).any() for got, want in zip(calls[name](), wants[name]))
+        except Exception as exc:  # a thread's failure is the test's
+            failed.append(exc)
+
+    threads = [threading.Thread(target=run, args=(name,)) for name in ("gradients", "product", "gradients", "product")]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failed, failed
+    assert not torch.stack(wrong).any()
